@@ -166,7 +166,9 @@ def prepare(case, seed):
         by_length = torch.sort(lengths, descending=True, stable=True)[1]
         st['key_valid'] = (torch.arange(t, device=dev) >= start[:, None]).to(torch.uint8)
         st['seq_range'] = torch.stack([start, torch.ones_like(start), by_length], 1).to(torch.int32)
-        st['row_base'] = torch.cumsum(lengths, 0) - lengths - start
+        # token (b, t) lies at row_base[b] + t; the last entry counts the rows
+        ends = torch.cumsum(lengths, 0)
+        st['row_base'] = torch.cat([ends - lengths - start, ends[-1:]])
     if case['op'] == 'prompt':
         st['state'] = normal(b, h, d, d, dtype=torch.float32, std=2.0) if case['carry'] else None
     else:
@@ -225,7 +227,7 @@ def _split(st, x):
     case = st['case']
     b, t, h, d = case['batch'], case['length'], case['heads'], case['dim']
     if st['row_base'] is not None:
-        at = st['row_base'][:, None] + torch.arange(t, device=x.device)
+        at = st['row_base'][:-1, None] + torch.arange(t, device=x.device)
         x = x.float()[at.clamp(min=0)]
     else:
         x = x.float().view(b, t, h * d)
