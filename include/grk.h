@@ -600,6 +600,83 @@ int grk_add_norm_bwd(const void* gx, int64_t ldgx, int gx_dtype, const void* gs,
                      int64_t ldds, float* dgamma, float* dbeta, void* ws, size_t ws_bytes, void* stream);
 
 /* ------------------------------------------------------------------------
+ * The decay block (no reference): rotary positions, linear attention with a
+ * decay for each head, and the norm of each head with a SiLU gate.  Rows hold
+ * heads side by side: head h at columns [h * head_dim, (h + 1) * head_dim).
+ * dtype (GRK_F32, GRK_BF16, GRK_F16) is the type of every row operand of a call;
+ * arithmetic and sums are fp32, outputs rounded once.  Any row stride of at
+ * least heads * head_dim elements; rows, strides and head_dim made of 16-byte
+ * vectors take the vector kernels.
+ * ------------------------------------------------------------------------ */
+/* Each head's first rotary_dim columns (even, <= head_dim) as rotary_dim / 2
+ * pairs -- (i, i + rotary_dim / 2), or (2 i, 2 i + 1) with interleaved -- turned by
+ * the angle positions[row] * freqs[i] (radians, fp64 product) and multiplied by
+ * scale; the other columns are copied.  inverse: turned back -- the gradient of
+ * the forward call with the same scale.  positions [rows] itype, freqs fp64
+ * [rotary_dim / 2].  y may be x (with the same stride); otherwise the two must not
+ * overlap. */
+int grk_rotary(const void* x, int64_t ldx, void* y, int64_t ldy, int dtype, const void* positions, int itype,
+               const double* freqs, int64_t rows, int heads, int head_dim, int rotary_dim, int interleaved,
+               float scale, int inverse, void* stream);
+
+/* S_t = g S_{t-1} + k_t v_t^T, o_t = scale * q_t S_t with g = exp(min(log_decay[h], 0))
+ * for every (sequence, head); head_dim in [1, 128] (GRK_EUNSUPPORTED above).
+ * Positions with key_valid 0 hold no event: their q / k / v are not read (whatever
+ * they hold), their output and gradient rows are zero, and the state decays over
+ * them.  seq_range (int32 [batch, 3], grk_seq_ranges; optional): the same for the
+ * positions before seq_range[b][0], without reading key_valid there.
+ * row_base / num_rows / capacity: the packed rows of grk_attn_args (seq_range
+ * required; rows [*num_rows, capacity) of every output are zeroed); else the rows are
+ * [batch * seq_len].
+ * state_in / state_out (optional, fp32 [batch, heads, head_dim, head_dim], S[k][v]): the
+ * state before the first and behind the last position; they may be one buffer.
+ * Deterministic: no atomics, the order of every sum is fixed by the shapes. */
+typedef struct grk_decay_args {
+  int32_t batch, heads, seq_len, head_dim;
+  int32_t dtype;                   /* q / k / v / out and their gradients */
+  float scale;
+  const void* q; const void* k; const void* v;
+  int64_t ldq, ldk, ldv;
+  const float* log_decay;          /* [heads], log g; above 0 counts as 0, -inf as g = 0 */
+  const uint8_t* key_valid;        /* [batch, seq_len] or NULL */
+  const int32_t* seq_range;
+  const int64_t* row_base;
+  const int64_t* num_rows;
+  int64_t capacity;
+} grk_decay_args;
+size_t grk_decay_attn_workspace(const grk_decay_args* a, int backward);
+int grk_decay_attn_fwd(const grk_decay_args* a, const float* state_in, float* state_out, void* out, int64_t ldo,
+                       void* workspace, size_t workspace_bytes, void* stream);
+/* dq / dk / dv of a forward call without states (log_decay gets no gradient). */
+int grk_decay_attn_bwd(const grk_decay_args* a, const void* dout, int64_t lddo, void* dq, int64_t lddq, void* dk,
+                       int64_t lddk, void* dv, int64_t lddv, void* workspace, size_t workspace_bytes, void* stream);
+/* One event of each of n users: state[slots[i]] <- g state + k_i v_i^T in place, out_i =
+ * scale * q_i state.  state fp32 [num_slots, heads, head_dim, head_dim]; slots [n] itype,
+ * NULL: event i takes state i.  Events of one slot are that user's next events, taken in
+ * the order of their index.  A negative slot holds no event (output row zero); one at or
+ * past num_slots as well, and sets *err_flag (optional).  Workspace:
+ * grk_decay_attn_step_workspace(n, slots != NULL) bytes. */
+size_t grk_decay_attn_step_workspace(int64_t n, int has_slots);
+int grk_decay_attn_step(const void* q, int64_t ldq, const void* k, int64_t ldk, const void* v, int64_t ldv, int dtype,
+                        const float* log_decay, int64_t n, int heads, int head_dim, float scale, float* state,
+                        int64_t num_slots, const void* slots, int itype, int32_t* err_flag, void* out, int64_t ldo,
+                        void* workspace, size_t workspace_bytes, void* stream);
+
+/* y = ((x - mean_h) / sqrt(var_h + eps) * weight + bias) * SiLU(gate) over the
+ * head_dim columns (in [1, 2048]) of each (row, head); gate / weight / bias optional
+ * (NULL: 1 / 1 / 0).  weight / bias / dweight / dbias fp32 [heads * head_dim].  The
+ * backward writes dx, dgate (with a gate) and, where given, dweight / dbias (fixed-order
+ * sums; grk_head_norm_bwd_workspace bytes, needed only for them). */
+int grk_head_norm_fwd(const void* x, int64_t ldx, const void* gate, int64_t ldg, const float* weight,
+                      const float* bias, float eps, int64_t rows, int heads, int head_dim, int dtype, void* y,
+                      int64_t ldy, void* stream);
+size_t grk_head_norm_bwd_workspace(int64_t rows, int heads, int head_dim);
+int grk_head_norm_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* gate, int64_t ldg,
+                      const float* weight, const float* bias, float eps, int64_t rows, int heads, int head_dim,
+                      int dtype, void* dx, int64_t lddx, void* dgate, int64_t lddg, float* dweight, float* dbias,
+                      void* workspace, size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------
  * Pair logits + BCE (model/BaseLine/model.py:379-382; main.py:177-182)
  * ------------------------------------------------------------------------ */
 /* Floats of `partials` workspace needed for num_rows rows. */

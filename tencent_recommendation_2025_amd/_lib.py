@@ -98,6 +98,14 @@ class GrkGemmGroup(C.Structure):
                 ('ldc', C.c_int64), ('rows', C.c_int64), ('b_rows', C.c_int64)]
 
 
+class GrkDecayArgs(C.Structure):
+    _fields_ = [('batch', C.c_int32), ('heads', C.c_int32), ('seq_len', C.c_int32), ('head_dim', C.c_int32),
+                ('dtype', C.c_int32), ('scale', C.c_float), ('q', C.c_void_p), ('k', C.c_void_p), ('v', C.c_void_p),
+                ('ldq', C.c_int64), ('ldk', C.c_int64), ('ldv', C.c_int64), ('log_decay', C.c_void_p),
+                ('key_valid', C.c_void_p), ('seq_range', C.c_void_p), ('row_base', C.c_void_p),
+                ('num_rows', C.c_void_p), ('capacity', C.c_int64)]
+
+
 class GrkStoreView(C.Structure):
     _fields_ = [('sparse', C.c_void_p), ('arr', C.c_void_p), ('arr_len', C.c_void_p), ('mm', C.c_void_p),
                 ('tokens', C.c_int64), ('f_sparse', C.c_int32), ('f_array', C.c_int32), ('a_cap', C.c_int32),
@@ -166,6 +174,17 @@ SIGNATURES = {
     'grk_norm_gate_bwd_workspace': (_SZ, [_I64, _I]),
     'grk_norm_gate_bwd': (_I, [_P, _I64, _P, _I64, _P, _I64, _P, _P, _P, _I64, _I, _F, C.c_uint64, _P, _P, _I64, _P,
                                _I64, _P, _P, _P, _SZ, _P]),
+    'grk_rotary': (_I, [_P, _I64, _P, _I64, _I, _P, _I, _P, _I64, _I, _I, _I, _I, _F, _I, _P]),
+    'grk_decay_attn_workspace': (_SZ, [C.POINTER(GrkDecayArgs), _I]),
+    'grk_decay_attn_fwd': (_I, [C.POINTER(GrkDecayArgs), _P, _P, _P, _I64, _P, _SZ, _P]),
+    'grk_decay_attn_bwd': (_I, [C.POINTER(GrkDecayArgs), _P, _I64, _P, _I64, _P, _I64, _P, _I64, _P, _SZ, _P]),
+    'grk_decay_attn_step_workspace': (_SZ, [_I64, _I]),
+    'grk_decay_attn_step': (_I, [_P, _I64, _P, _I64, _P, _I64, _I, _P, _I64, _I, _I, _F, _P, _I64, _P, _I, _P, _P,
+                                 _I64, _P, _SZ, _P]),
+    'grk_head_norm_fwd': (_I, [_P, _I64, _P, _I64, _P, _P, _F, _I64, _I, _I, _I, _P, _I64, _P]),
+    'grk_head_norm_bwd_workspace': (_SZ, [_I64, _I, _I]),
+    'grk_head_norm_bwd': (_I, [_P, _I64, _P, _I64, _P, _I64, _P, _P, _F, _I64, _I, _I, _I, _P, _I64, _P, _I64, _P,
+                               _P, _P, _SZ, _P]),
     'grk_seq_ranges': (_I, [_P, _I, _I, _P, _P]),
     'grk_jagged_layout': (_I, [_P, _I, _I, _I64, _P, _P, _P, _P, _P, _P, _P]),
     'grk_gather_rows': (_I, [C.POINTER(GrkRowCopy), _I, _P, _I64, _P]),

@@ -1,0 +1,549 @@
+// Decayed linear attention for gfx950 (the formulas: grk_decay.h): the general kernel --
+// fp32, bf16 or fp16 rows, any head_dim up to 128 -- on the fp32 matrix instruction, the
+// segments' scan and the single-step kernel.
+#include "grk_decay.h"
+
+namespace grk {
+
+// ---------------------------------------------------------- general kernel --
+// One workgroup walks a segment chunk by chunk; wave w owns columns [16 w, 16 w + 16) of
+// the state (head_dim padded to DP with zeros: DP / 16 waves), its 16-row tiles in
+// registers.  v_mfma_f32_16x16x4_f32: lane l = 16 g + c holds A[c][g], B[g][c] and
+// D[4 g + i][c], i < 4.  The four k of a 16-deep step are taken as 4 g + s (s = 0..3)
+// instead of 4 s + g: then register s of a state tile IS the B operand of step s, and the
+// row-major A operands are one 16-byte LDS read.
+constexpr int kDecayPad = 4;   // floats after each LDS row: rows 4 apart fall 16 banks apart
+
+template <int DP> constexpr size_t decay_lds_f32(bool state_only) {
+  return (size_t)(state_only ? 2 : 3) * kDecayChunk * (DP + kDecayPad) * 4 +
+         (state_only ? 0 : (size_t)kDecayChunk * (kDecayChunk + kDecayPad) * 4);
+}
+
+template <typename T, int V, int DP>
+__device__ __forceinline__ void decay_stage(const DecayParams& p, const DecayPlace& w, int rev, const void* src,
+                                            int64_t ld, int t0, float* dst) {
+  constexpr int ST = DP + kDecayPad, U = DP / (V > 4 ? 4 : V);   // 4-column units of a row (1 without vectors)
+  constexpr int W = DP / U;
+  for (int a = threadIdx.x; a < kDecayChunk * U; a += DP * 4) {
+    const int t = a / U, c = a % U * W;
+    const int64_t row = c < p.head_dim ? decay_row(p, w, rev, t0 + t) : -1;
+    float f[W];
+#pragma unroll
+    for (int e = 0; e < W; ++e) f[e] = 0.f;
+    if (row >= 0) {
+      const T* s = reinterpret_cast<const T*>(src) + row * ld + (int64_t)w.h * p.head_dim + c;
+      if constexpr (W == 1) {
+        f[0] = to_f32(*s);
+      } else if constexpr (sizeof(T) == 4) {
+        vload<T, 4>(s, f);
+      } else {
+        const uint2 x = *reinterpret_cast<const uint2*>(s);
+        T h[4];
+        __builtin_memcpy(h, &x, 8);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) f[e] = to_f32(h[e]);
+      }
+    }
+    if constexpr (W == 1) dst[t * ST + c] = f[0];
+    else *reinterpret_cast<float4*>(dst + t * ST + c) = make_float4(f[0], f[1], f[2], f[3]);
+  }
+}
+
+__device__ __forceinline__ f32x4 mfma4(float a, float b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
+}
+
+// c += A B over 16 of the contraction: step s takes element s of both.
+__device__ __forceinline__ void mfma16(f32x4 a, f32x4 b, f32x4& c) {
+#pragma unroll
+  for (int s = 0; s < 4; ++s) c = mfma4(a[s], b[s], c);
+  mfma_keep(c, a, b);
+}
+
+template <typename T, int V, int DP, bool STATE>
+__global__ void __launch_bounds__(DP * 4) k_decay_f32(DecayParams p) {
+  constexpr int C = kDecayChunk, ST = DP + kDecayPad, PT = C + kDecayPad, NT = DP / 16;
+  extern __shared__ __attribute__((aligned(16))) float sm[];
+  float* sb = sm;
+  float* sc = sb + C * ST;
+  float* sa = sc + C * ST;
+  float* sp = sa + C * ST;
+  const DecayPlace w = decay_place(p);
+  if (!w.on) return;
+  const DecayRole r = p.role[w.role];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, c = lane & 15;
+  const int64_t bh = (int64_t)w.b * p.heads + w.h;
+  const int col = 16 * wave + c;   // the state column (and output column) of this lane
+  f32x4 st[NT];
+  float* frag = p.ws + (((int64_t)w.role * p.batch * p.heads + bh) * p.nseg + w.seg) * DP * DP;
+#pragma unroll
+  for (int dt = 0; dt < NT; ++dt) {
+    st[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+    if (!STATE && p.nseg > 1) {
+      st[dt] = *reinterpret_cast<const f32x4*>(frag + ((dt * NT + wave) * 64 + lane) * 4);
+    } else if (!STATE && p.state_in) {
+      const float f = decay_pow(w.lg, w.start);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int d = 16 * dt + 4 * g + i;
+        if (d < p.head_dim && col < p.head_dim)
+          st[dt][i] = f * p.state_in[(bh * p.head_dim + d) * p.head_dim + col];
+      }
+    }
+  }
+  if (!STATE) decay_zero_rows<T>(p, w, r);
+  for (int t0 = w.t0; t0 < w.t1; t0 += C) {
+    const int n = w.t1 - t0 < C ? w.t1 - t0 : C;
+    __syncthreads();
+    decay_stage<T, V, DP>(p, w, r.rev, r.b, r.ldb, t0, sb);
+    decay_stage<T, V, DP>(p, w, r.rev, r.c, r.ldc, t0, sc);
+    if (!STATE) decay_stage<T, V, DP>(p, w, r.rev, r.a, r.lda, t0, sa);
+    __syncthreads();
+    if constexpr (!STATE) {
+      // P: the 10 tiles on and below the diagonal, shared out over the waves
+      for (int tile = wave; tile < 10; tile += NT) {
+        int it = 0, jt = tile;
+        while (jt > it) { jt -= it + 1; ++it; }
+        f32x4 x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int dt = 0; dt < NT; ++dt) {
+          mfma16(*reinterpret_cast<const f32x4*>(sa + (16 * it + c) * ST + 16 * dt + 4 * g),
+                 *reinterpret_cast<const f32x4*>(sb + (16 * jt + c) * ST + 16 * dt + 4 * g), x);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int lag = 16 * (it - jt) + 4 * g + i - c;
+          sp[(16 * it + 4 * g + i) * PT + 16 * jt + c] = lag >= 0 ? x[i] * decay_pow(w.lg, lag) : 0.f;
+        }
+      }
+      __syncthreads();
+#pragma unroll
+      for (int it = 0; it < C / 16; ++it) {
+        f32x4 x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int dt = 0; dt < NT; ++dt) {
+          mfma16(*reinterpret_cast<const f32x4*>(sa + (16 * it + c) * ST + 16 * dt + 4 * g), st[dt], x);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] *= decay_pow(w.lg, 16 * it + 4 * g + i + 1);
+        for (int jt = 0; jt <= it; ++jt) {
+          const float* b = sc + (16 * jt + 4 * g) * ST + col;
+          mfma16(*reinterpret_cast<const f32x4*>(sp + (16 * it + c) * PT + 16 * jt + 4 * g),
+                 f32x4{b[0], b[ST], b[2 * ST], b[3 * ST]}, x);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          bool live;
+          const int64_t row = decay_out_row(p, w, r.rev, t0 + 16 * it + 4 * g + i, &live);
+          if (row >= 0 && col < p.head_dim)
+            reinterpret_cast<T*>(r.out)[row * r.ldo + (int64_t)w.h * p.head_dim + col] =
+                from_f32<T>(live ? p.scale * x[i] : 0.f);
+        }
+      }
+    }
+    const float gn = decay_pow(w.lg, n);
+#pragma unroll
+    for (int dt = 0; dt < NT; ++dt) st[dt] *= gn;
+#pragma unroll
+    for (int jt = 0; jt < C / 16; ++jt) {
+      const int j0 = 16 * jt + 4 * g;
+      f32x4 v;
+#pragma unroll
+      for (int s = 0; s < 4; ++s) v[s] = j0 + s < n ? sc[(j0 + s) * ST + col] * decay_pow(w.lg, n - 1 - j0 - s) : 0.f;
+#pragma unroll
+      for (int dt = 0; dt < NT; ++dt) {
+        const float* k = sb + j0 * ST + 16 * dt + c;
+        mfma16(f32x4{k[0], k[ST], k[2 * ST], k[3 * ST]}, v, st[dt]);
+      }
+    }
+  }
+  if (STATE) {
+#pragma unroll
+    for (int dt = 0; dt < NT; ++dt)
+      *reinterpret_cast<f32x4*>(frag + ((dt * NT + wave) * 64 + lane) * 4) = st[dt];
+  } else if (p.nseg == 1 && p.state_out) {
+#pragma unroll
+    for (int dt = 0; dt < NT; ++dt)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int d = 16 * dt + 4 * g + i;
+        if (d < p.head_dim && col < p.head_dim)
+          p.state_out[(bh * p.head_dim + d) * p.head_dim + col] = st[dt][i];
+      }
+  }
+}
+
+// The segments' own states -> the state before each segment (and behind the last one):
+// run <- g^len run + own, four elements of the state to a thread.
+template <int DP>
+__global__ void __launch_bounds__(256) k_decay_scan(DecayParams p) {
+  constexpr int NT = DP / 16;
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;   // (role, b, h, fragment)
+  const int f = (int)(i % (DP * DP / 4));
+  const int64_t rbh = i / (DP * DP / 4);
+  if (rbh >= (int64_t)p.roles * p.batch * p.heads) return;
+  const int64_t bh = rbh % ((int64_t)p.batch * p.heads);
+  const int b = (int)(bh / p.heads), h = (int)(bh % p.heads);
+  const int lane = f & 63, wave = f >> 6 & (NT - 1), dt = f >> 6 >> __builtin_ctz(NT);
+  const int col = 16 * wave + (lane & 15), d0 = 16 * dt + 4 * (lane >> 4);
+  int start = p.seq_range ? p.seq_range[3 * (int64_t)b] : 0;
+  start = start < 0 ? 0 : (start > p.seq_len ? p.seq_len : start);
+  const int len = p.seq_len - start;
+  const float lg = fminf(p.log_decay[h], 0.f);
+  f32x4 run = {0.f, 0.f, 0.f, 0.f};
+  if (p.state_in) {
+    const float g0 = decay_pow(lg, start);
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (d0 + e < p.head_dim && col < p.head_dim)
+        run[e] = g0 * p.state_in[(bh * p.head_dim + d0 + e) * p.head_dim + col];
+  }
+  f32x4* own = reinterpret_cast<f32x4*>(p.ws + rbh * p.nseg * DP * DP) + f;
+  for (int s = 0; s < p.nseg; ++s) {
+    const int left = len - s * p.seg_len, n = left < 0 ? 0 : (left < p.seg_len ? left : p.seg_len);
+    const f32x4 x = own[(int64_t)s * (DP * DP / 4)];
+    own[(int64_t)s * (DP * DP / 4)] = run;
+    run = run * decay_pow(lg, n) + x;
+  }
+  if (p.state_out) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (d0 + e < p.head_dim && col < p.head_dim)
+        p.state_out[(bh * p.head_dim + d0 + e) * p.head_dim + col] = run[e];
+  }
+}
+
+// -------------------------------------------------------------- single step --
+// One workgroup per (event, head): S <- g S + k v^T in place, o = scale q S.  The state
+// is read and written once, in rows of `lanes` threads of V columns; a thread keeps its
+// columns, so o is a sum over the thread rows in LDS.  Bound: memory, 8 head_dim^2 bytes
+// of state per (event, head).
+constexpr int kStepThreads = 256;
+constexpr int kStepInline = 256;   // events up to which every workgroup looks for its slot's others itself
+
+struct StepParams {
+  const void* q; int64_t ldq;
+  const void* k; int64_t ldk;
+  const void* v; int64_t ldv;
+  const float* log_decay;
+  float* state; int64_t num_slots;
+  const void* slots; int slots64;
+  int64_t n;
+  int heads, hd;
+  float scale;
+  int32_t* err;
+  void* out; int64_t ldo;
+  int32_t* links;                // [n, 2]: has an earlier event of its slot, the next one (or -1); or NULL
+};
+
+__device__ __forceinline__ int64_t step_slot(const StepParams& p, int64_t i) {
+  if (!p.slots) return i;
+  return p.slots64 ? reinterpret_cast<const int64_t*>(p.slots)[i]
+                   : (int64_t)reinterpret_cast<const int32_t*>(p.slots)[i];
+}
+
+// Events of one slot are consecutive events of that user: the first one's workgroup
+// takes them all, in order.  links[i] = (an earlier event has this slot, the next event
+// that has it), by comparing every pair.
+__global__ void __launch_bounds__(kStepThreads) k_step_links(StepParams p) {
+  __shared__ int64_t tile[kStepThreads];
+  const int64_t i = (int64_t)blockIdx.x * kStepThreads + threadIdx.x;
+  const int64_t mine = i < p.n ? step_slot(p, i) : -1;
+  int before = 0;
+  int64_t next = -1;
+  for (int64_t j0 = 0; j0 < p.n; j0 += kStepThreads) {
+    __syncthreads();
+    tile[threadIdx.x] = j0 + threadIdx.x < p.n ? step_slot(p, j0 + threadIdx.x) : -1;
+    __syncthreads();
+    const int m = (int)(p.n - j0 < kStepThreads ? p.n - j0 : kStepThreads);
+    if (mine >= 0)
+      for (int t = 0; t < m; ++t)
+        if (tile[t] == mine) {
+          if (j0 + t < i) before = 1;
+          else if (j0 + t > i && next < 0) next = j0 + t;
+        }
+  }
+  if (i < p.n) {
+    p.links[2 * i] = before;
+    p.links[2 * i + 1] = (int)next;
+  }
+}
+
+template <typename T, int V>
+__global__ void __launch_bounds__(kStepThreads) k_decay_step(StepParams p) {
+  __shared__ float sq[128], sk[128], sv[128], red[kStepThreads * V];
+  __shared__ int found[2];
+  const int64_t i0 = blockIdx.x / p.heads;
+  const int h = (int)(blockIdx.x % p.heads), hd = p.hd;
+  const int lanes = hd / V, rows = kStepThreads / lanes;
+  const int lr = threadIdx.x / lanes, e = threadIdx.x % lanes * V;
+  const bool on = lr < rows;
+  const int64_t slot = step_slot(p, i0);
+  if (slot < 0 || slot >= p.num_slots) {
+    if (slot >= 0 && p.err && threadIdx.x == 0) *p.err = 1;
+    for (int c = threadIdx.x; c < hd; c += kStepThreads)
+      reinterpret_cast<T*>(p.out)[i0 * p.ldo + (int64_t)h * hd + c] = from_f32<T>(0.f);
+    return;
+  }
+  const float g = expf(fminf(p.log_decay[h], 0.f));
+  float* S = p.state + (slot * p.heads + h) * hd * hd;
+  for (int64_t i = i0; i >= 0;) {
+    // the slot's other events
+    int64_t next = -1;
+    if (p.slots) {
+      if (p.links) {
+        if (i == i0 && p.links[2 * i]) return;
+        next = p.links[2 * i + 1];
+      } else {
+        if (threadIdx.x == 0) { found[0] = 0; found[1] = 0x7fffffff; }
+        __syncthreads();
+        for (int64_t j = threadIdx.x; j < p.n; j += kStepThreads)
+          if (j != i && step_slot(p, j) == slot) {
+            if (j < i) found[0] = 1;
+            else atomicMin(&found[1], (int)j);
+          }
+        __syncthreads();
+        const int first = found[0], nx = found[1];
+        __syncthreads();
+        if (i == i0 && first) return;
+        next = nx == 0x7fffffff ? -1 : nx;
+      }
+    }
+    const int64_t at = (int64_t)h * hd;
+    for (int c = threadIdx.x; c < hd; c += kStepThreads) {
+      sq[c] = to_f32(reinterpret_cast<const T*>(p.q)[i * p.ldq + at + c]);
+      sk[c] = to_f32(reinterpret_cast<const T*>(p.k)[i * p.ldk + at + c]);
+      sv[c] = to_f32(reinterpret_cast<const T*>(p.v)[i * p.ldv + at + c]);
+    }
+    __syncthreads();
+    float o[V], v[V];
+#pragma unroll
+    for (int x = 0; x < V; ++x) { o[x] = 0.f; v[x] = on ? sv[e + x] : 0.f; }
+    if (on)
+#pragma unroll 4
+      for (int d = lr; d < hd; d += rows) {
+        float s[V];
+        vload<float, V>(S + d * hd + e, s);
+        const float kd = sk[d], qd = sq[d];
+#pragma unroll
+        for (int x = 0; x < V; ++x) {
+          s[x] = g * s[x] + kd * v[x];
+          o[x] += qd * s[x];
+        }
+        vstore<float, V>(S + d * hd + e, s);
+      }
+#pragma unroll
+    for (int x = 0; x < V; ++x)
+      if (on) red[lr * hd + e + x] = o[x];
+    __syncthreads();
+    for (int c = threadIdx.x; c < hd; c += kStepThreads) {
+      float t = 0.f;
+      for (int r = 0; r < rows; ++r) t += red[r * hd + c];
+      reinterpret_cast<T*>(p.out)[i * p.ldo + at + c] = from_f32<T>(p.scale * t);
+    }
+    __syncthreads();
+    i = next;
+  }
+}
+
+// ------------------------------------------------------------------ launch --
+static int decay_dp(int hd) { return hd <= 16 ? 16 : hd <= 32 ? 32 : hd <= 64 ? 64 : 128; }
+
+// Segments: a workgroup walks a sequence alone where the (sequence, head) pairs already
+// fill the card; else the sequence is cut, at least 4 chunks to a segment.
+static void decay_segments(DecayParams& p) {
+  const int64_t units = (int64_t)p.roles * p.batch * p.heads;
+  int64_t nseg = units >= 512 ? 1 : 1024 / (units > 0 ? units : 1);
+  const int64_t most = p.seq_len / (4 * kDecayChunk);
+  if (nseg > most) nseg = most;
+  if (nseg < 1) nseg = 1;
+  const int64_t chunks = (p.seq_len + kDecayChunk - 1) / kDecayChunk;
+  const int64_t per = (chunks + nseg - 1) / nseg;
+  p.seg_len = (int)((per < 1 ? 1 : per) * kDecayChunk);
+  p.nseg = (int)((chunks + per - 1) / (per < 1 ? 1 : per));
+  if (p.nseg < 1) p.nseg = 1;
+}
+
+static size_t decay_ws(const DecayParams& p) {
+  if (p.nseg <= 1) return 0;
+  const size_t dp = decay_dp(p.head_dim);
+  return (size_t)p.roles * p.batch * p.heads * p.nseg * dp * dp * sizeof(float);
+}
+
+static int decay_check(const grk_decay_args* a) {
+  GRK_CHECK_ARG(a, "args required");
+  GRK_CHECK_ARG(known_dtype(a->dtype), "dtype must be fp32, bf16 or fp16");
+  GRK_CHECK_ARG(a->batch >= 0 && a->heads > 0 && a->seq_len >= 0, "batch >= 0, heads > 0 and seq_len >= 0 required");
+  if (a->head_dim < 1 || a->head_dim > 128) {
+    set_error("head_dim must be in [1, 128]");
+    return GRK_EUNSUPPORTED;
+  }
+  GRK_CHECK_ARG((int64_t)a->batch * a->heads < (1 << 21) && a->seq_len < (1 << 30),
+                "batch * heads must be below 2^21 and seq_len below 2^30");
+  return GRK_OK;
+}
+
+static int decay_rows_ok(const void* q, int64_t ld, const grk_decay_args* a, int64_t capacity, const char* name) {
+  GRK_CHECK_ARG(q, "%s required", name);
+  GRK_CHECK_ARG(capacity == 1 ? ld >= 0 : ld >= (int64_t)a->heads * a->head_dim,
+                "%s: row stride below heads * head_dim", name);
+  return GRK_OK;
+}
+
+static void decay_params(const grk_decay_args* a, DecayParams& p) {
+  memset(&p, 0, sizeof(p));
+  p.batch = a->batch; p.heads = a->heads; p.seq_len = a->seq_len; p.head_dim = a->head_dim; p.scale = a->scale;
+  p.log_decay = a->log_decay; p.key_valid = a->key_valid; p.seq_range = a->seq_range;
+  p.row_base = a->row_base; p.num_rows = a->num_rows;
+  p.capacity = a->row_base ? a->capacity : (int64_t)a->batch * a->seq_len;
+}
+
+template <typename T, int V, int DP>
+static int decay_run(const DecayParams& p, hipStream_t s) {
+  const int64_t groups = (int64_t)p.batch * p.heads * p.nseg;
+  const unsigned grid = (unsigned)((groups + 7) / 8 * 8 * p.roles);
+  if (p.nseg > 1) {
+    constexpr size_t lds = decay_lds_f32<DP>(true);
+    GRK_CHECK_HIP(ensure_dynamic_lds((const void*)k_decay_f32<T, V, DP, true>, lds));
+    k_decay_f32<T, V, DP, true><<<grid, DP * 4, lds, s>>>(p);
+    GRK_LAUNCH_CHECK();
+    const int64_t n = (int64_t)p.roles * p.batch * p.heads * DP * DP / 4;
+    k_decay_scan<DP><<<(unsigned)((n + 255) / 256), 256, 0, s>>>(p);
+    GRK_LAUNCH_CHECK();
+  }
+  constexpr size_t lds = decay_lds_f32<DP>(false);
+  GRK_CHECK_HIP(ensure_dynamic_lds((const void*)k_decay_f32<T, V, DP, false>, lds));
+  k_decay_f32<T, V, DP, false><<<grid, DP * 4, lds, s>>>(p);
+  GRK_LAUNCH_CHECK();
+  return GRK_OK;
+}
+
+static int decay_launch(const DecayParams& p, int dtype, hipStream_t s) {
+  // 8- or 16-byte loads of 4 columns: rows and heads start on them
+  bool vec = p.head_dim % 4 == 0;
+  const size_t b4 = 4 * dtype_size(dtype);
+  for (int r = 0; r < p.roles; ++r) {
+    const DecayRole& x = p.role[r];
+    vec = vec && ((uintptr_t)x.a | (uintptr_t)x.b | (uintptr_t)x.c) % b4 == 0 && (x.lda | x.ldb | x.ldc) % 4 == 0;
+  }
+  return for_dtype(dtype, [&](auto t) {
+    using T = decltype(t);
+    switch (decay_dp(p.head_dim)) {
+      case 16: return vec ? decay_run<T, 4, 16>(p, s) : decay_run<T, 1, 16>(p, s);
+      case 32: return vec ? decay_run<T, 4, 32>(p, s) : decay_run<T, 1, 32>(p, s);
+      case 64: return vec ? decay_run<T, 4, 64>(p, s) : decay_run<T, 1, 64>(p, s);
+      default: return vec ? decay_run<T, 4, 128>(p, s) : decay_run<T, 1, 128>(p, s);
+    }
+  });
+}
+
+}  // namespace grk
+
+using namespace grk;
+
+extern "C" size_t grk_decay_attn_workspace(const grk_decay_args* a, int backward) {
+  clear_error();
+  if (decay_check(a)) return 0;
+  DecayParams p;
+  decay_params(a, p);
+  p.roles = backward ? 3 : 1;
+  decay_segments(p);
+  return decay_ws(p);
+}
+
+extern "C" int grk_decay_attn_fwd(const grk_decay_args* a, const float* state_in, float* state_out, void* out,
+                                  int64_t ldo, void* ws, size_t ws_bytes, void* stream) {
+  clear_error();
+  int rc = decay_check(a);
+  if (rc) return rc;
+  if (a->batch == 0) return GRK_OK;
+  DecayParams p;
+  decay_params(a, p);
+  if (p.capacity == 0 && !state_out) return GRK_OK;
+  GRK_CHECK_ARG(a->log_decay, "log_decay required");
+  GRK_CHECK_ARG(!a->row_base || (a->seq_range && a->capacity >= 0), "row_base needs seq_range and capacity >= 0");
+  if (p.capacity > 0 &&
+      ((rc = decay_rows_ok(a->q, a->ldq, a, p.capacity, "q")) || (rc = decay_rows_ok(a->k, a->ldk, a, p.capacity, "k")) ||
+       (rc = decay_rows_ok(a->v, a->ldv, a, p.capacity, "v")) || (rc = decay_rows_ok(out, ldo, a, p.capacity, "out"))))
+    return rc;
+  p.roles = 1;
+  p.role[0] = DecayRole{a->q, a->ldq, a->k, a->ldk, a->v, a->ldv, out, ldo, 0};
+  p.state_in = state_in; p.state_out = state_out;
+  decay_segments(p);
+  GRK_CHECK_ARG(decay_ws(p) == 0 || (ws && ws_bytes >= decay_ws(p)), "workspace too small");
+  p.ws = (float*)ws;
+  return decay_launch(p, a->dtype, (hipStream_t)stream);
+}
+
+extern "C" int grk_decay_attn_bwd(const grk_decay_args* a, const void* dout, int64_t lddo, void* dq, int64_t lddq,
+                                  void* dk, int64_t lddk, void* dv, int64_t lddv, void* ws, size_t ws_bytes,
+                                  void* stream) {
+  clear_error();
+  int rc = decay_check(a);
+  if (rc) return rc;
+  DecayParams p;
+  decay_params(a, p);
+  if (a->batch == 0 || p.capacity == 0) return GRK_OK;
+  GRK_CHECK_ARG(a->log_decay, "log_decay required");
+  GRK_CHECK_ARG(!a->row_base || a->seq_range, "row_base needs seq_range");
+  if ((rc = decay_rows_ok(a->q, a->ldq, a, p.capacity, "q")) || (rc = decay_rows_ok(a->k, a->ldk, a, p.capacity, "k")) ||
+      (rc = decay_rows_ok(a->v, a->ldv, a, p.capacity, "v")) || (rc = decay_rows_ok(dout, lddo, a, p.capacity, "dout")) ||
+      (rc = decay_rows_ok(dq, lddq, a, p.capacity, "dq")) || (rc = decay_rows_ok(dk, lddk, a, p.capacity, "dk")) ||
+      (rc = decay_rows_ok(dv, lddv, a, p.capacity, "dv")))
+    return rc;
+  p.roles = 3;
+  p.role[0] = DecayRole{dout, lddo, a->v, a->ldv, a->k, a->ldk, dq, lddq, 0};
+  p.role[1] = DecayRole{a->v, a->ldv, dout, lddo, a->q, a->ldq, dk, lddk, 1};
+  p.role[2] = DecayRole{a->k, a->ldk, a->q, a->ldq, dout, lddo, dv, lddv, 1};
+  decay_segments(p);
+  GRK_CHECK_ARG(decay_ws(p) == 0 || (ws && ws_bytes >= decay_ws(p)), "workspace too small");
+  p.ws = (float*)ws;
+  return decay_launch(p, a->dtype, (hipStream_t)stream);
+}
+
+extern "C" size_t grk_decay_attn_step_workspace(int64_t n, int has_slots) {
+  return has_slots && n > kStepInline ? (size_t)n * 2 * sizeof(int32_t) : 0;
+}
+
+extern "C" int grk_decay_attn_step(const void* q, int64_t ldq, const void* k, int64_t ldk, const void* v, int64_t ldv,
+                                   int dtype, const float* log_decay, int64_t n, int heads, int head_dim, float scale,
+                                   float* state, int64_t num_slots, const void* slots, int itype, int32_t* err_flag,
+                                   void* out, int64_t ldo, void* ws, size_t ws_bytes, void* stream) {
+  clear_error();
+  GRK_CHECK_ARG(known_dtype(dtype), "dtype must be fp32, bf16 or fp16");
+  GRK_CHECK_ARG(itype == GRK_I32 || itype == GRK_I64, "slots must be int32 or int64");
+  GRK_CHECK_ARG(n >= 0 && heads > 0 && num_slots >= 0 && n < (1 << 24) &&
+                n * heads < (1 << 24), "n >= 0, heads > 0, num_slots >= 0 and n * heads < 2^24 required");
+  if (head_dim < 1 || head_dim > 128) {
+    set_error("head_dim must be in [1, 128]");
+    return GRK_EUNSUPPORTED;
+  }
+  if (n == 0) return GRK_OK;
+  const int64_t cols = (int64_t)heads * head_dim;
+  GRK_CHECK_ARG(q && k && v && log_decay && out && (state || num_slots == 0), "q / k / v / log_decay / state / out required");
+  GRK_CHECK_ARG(n == 1 || (ldq >= cols && ldk >= cols && ldv >= cols && ldo >= cols),
+                "row strides must be at least heads * head_dim");
+  GRK_CHECK_ARG(slots || num_slots >= n, "without slots event i takes state i: num_slots must be at least n");
+  const size_t need = grk_decay_attn_step_workspace(n, slots != nullptr);
+  GRK_CHECK_ARG(need == 0 || (ws && ws_bytes >= need), "workspace too small");
+  StepParams p;
+  memset(&p, 0, sizeof(p));
+  p.q = q; p.ldq = ldq; p.k = k; p.ldk = ldk; p.v = v; p.ldv = ldv; p.log_decay = log_decay; p.state = state;
+  p.num_slots = num_slots; p.slots = slots; p.slots64 = itype == GRK_I64; p.n = n; p.heads = heads; p.hd = head_dim;
+  p.scale = scale; p.err = err_flag; p.out = out; p.ldo = ldo; p.links = need ? (int32_t*)ws : nullptr;
+  hipStream_t s = (hipStream_t)stream;
+  if (need) {
+    k_step_links<<<(unsigned)((n + kStepThreads - 1) / kStepThreads), kStepThreads, 0, s>>>(p);
+    GRK_LAUNCH_CHECK();
+  }
+  const unsigned grid = (unsigned)(n * heads);
+  const bool vec = head_dim % 4 == 0 && (uintptr_t)state % 16 == 0;
+  for_dtype(dtype, [&](auto t) {
+    using T = decltype(t);
+    if (vec) k_decay_step<T, 4><<<grid, kStepThreads, 0, s>>>(p);
+    else k_decay_step<T, 1><<<grid, kStepThreads, 0, s>>>(p);
+    return 0;
+  });
+  GRK_LAUNCH_CHECK();
+  return GRK_OK;
+}

@@ -1004,6 +1004,112 @@ def hstu_core_fp8(pre, rab, ln_w, ln_b, key_valid, B, T, H, hd, inv_n, eps=1e-8,
                             seq_range)
 
 
+# ----------------------------------------------------------- decay block ----
+def _head_mat(x, dt=None):
+    """x as a [N, D] matrix the decay block's kernels read: dense rows at a row stride of
+    at least D (an expanded gradient is copied), of dtype dt."""
+    x = x.reshape(-1, x.shape[-1])
+    if dt is not None and x.dtype != dt:
+        x = x.to(dt)
+    ok = (x.shape[1] == 1 or x.stride(1) == 1) and (x.shape[0] <= 1 or x.stride(0) >= x.shape[1])
+    return x if ok else x.contiguous()
+
+
+class _RotaryFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, positions, freqs, heads, layout, scale):
+        ctx.save_for_backward(positions, freqs)
+        ctx.meta = (heads, layout, scale)
+        return K.rotary(_head_mat(x), positions, freqs, heads, layout, scale).view(x.shape)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, gy):
+        positions, freqs = ctx.saved_tensors
+        heads, layout, scale = ctx.meta
+        g = K.rotary(_head_mat(gy), positions, freqs, heads, layout, scale, inverse=True)
+        return g.view(gy.shape), None, None, None, None, None
+
+
+@_disable
+def rotary(x, positions, freqs, heads, layout='half', scale=1.0):
+    """Rotary positions of x [..., heads * head_dim] (kernels.rotary): positions one per row
+    (any shape of as many entries), freqs float64 [rotary_dim / 2].  The gradient is the
+    turn back; positions and freqs get none."""
+    if freqs.requires_grad:
+        raise L.GrkError('rotary: freqs get no gradient')
+    return _RotaryFn.apply(x, positions.reshape(-1).contiguous(), freqs, int(heads), layout, float(scale))
+
+
+class _DecayAttnFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, qkv, log_decay, key_valid, seq_range, row_base, batch, seq_len, scale):
+        x = _head_mat(qkv)
+        D = x.shape[1] // 3
+        o = K.decay_attn_fwd(x[:, :D], x[:, D:2 * D], x[:, 2 * D:], log_decay, batch, seq_len, scale, key_valid,
+                             seq_range, row_base)
+        ctx.save_for_backward(x, log_decay, key_valid, seq_range, row_base)
+        ctx.meta = (batch, seq_len, scale, qkv.shape)
+        return o.view(*qkv.shape[:-1], D)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, go):
+        x, log_decay, key_valid, seq_range, row_base = ctx.saved_tensors
+        batch, seq_len, scale, shape = ctx.meta
+        D = x.shape[1] // 3
+        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        K.decay_attn_bwd(_head_mat(go, x.dtype), x[:, :D], x[:, D:2 * D], x[:, 2 * D:], log_decay, batch, seq_len,
+                         scale, key_valid, seq_range, row_base, dx[:, :D], dx[:, D:2 * D], dx[:, 2 * D:])
+        return dx.view(shape), None, None, None, None, None, None, None
+
+
+@_disable
+def decay_attn(qkv, log_decay, batch, seq_len, scale=None, key_valid=None, seq_range=None, row_base=None):
+    """Linear attention with a decay for each head (kernels.decay_attn_fwd) of packed
+    q | k | v rows [..., 3 * heads * head_dim]; differentiable in qkv.  The decays are
+    given, not learned: log_decay (fp32 [heads]) gets no gradient."""
+    if log_decay.requires_grad:
+        raise L.GrkError('decay_attn: log_decay gets no gradient (the decays are given, not learned)')
+    if qkv.shape[-1] % 3:
+        raise L.GrkError('qkv must hold q | k | v side by side: [rows, 3 * heads * head_dim]')
+    return _DecayAttnFn.apply(qkv, log_decay, key_valid, seq_range, row_base, int(batch), int(seq_len),
+                              None if scale is None else float(scale))
+
+
+class _HeadNormFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, gate, heads, eps):
+        x2 = _head_mat(x)
+        g2 = _head_mat(gate, x.dtype) if gate is not None else None
+        w32 = weight.detach().float().contiguous() if weight is not None else None
+        b32 = bias.detach().float().contiguous() if bias is not None else None
+        y = K.head_norm_fwd(x2, w32, b32, heads, eps, g2)
+        ctx.save_for_backward(x2, w32, b32, g2)
+        ctx.meta = (heads, eps, x.shape, None if gate is None else gate.dtype,
+                    None if weight is None else weight.dtype, None if bias is None else bias.dtype)
+        return y.view(x.shape)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, gy):
+        x2, w32, b32, g2 = ctx.saved_tensors
+        heads, eps, shape, gdt, wdt, bdt = ctx.meta
+        dx, dg, dw, db = K.head_norm_bwd(_head_mat(gy, x2.dtype), x2, w32, b32, heads, eps, g2)
+        return (dx.view(shape), dw.to(wdt) if dw is not None else None, db.to(bdt) if db is not None else None,
+                dg.view(shape).to(gdt) if dg is not None else None, None, None)
+
+
+@_disable
+def head_norm(x, weight, bias, heads, eps=1e-5, gate=None):
+    """Layer norm of each head's columns of x [..., heads * head_dim], times SiLU(gate)
+    (kernels.head_norm_fwd); differentiable in x, weight, bias and gate.  weight / bias
+    [heads * head_dim] or None; the gate has x's shape."""
+    if gate is not None and gate.shape != x.shape:
+        raise L.GrkError('the gate must have the shape of x')
+    return _HeadNormFn.apply(x, weight, bias, gate, int(heads), float(eps))
+
+
 # ---------------------------------------------------------------- logits ----
 def _rows2d(x):
     x = x.reshape(-1, x.shape[-1])

@@ -7,6 +7,7 @@ built library.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 import math
 import os
@@ -1141,6 +1142,332 @@ def emb_combine_bwd(gy, a, b, scale, relu=True, dropout_p=0.0, seed=0, want=(Tru
                                         float(dropout_p), hs, _ptr(ds), p0, l0, p1, l1, p2, l2, L.stream_ptr(dev)),
             'grk_emb_combine_bwd')
     return tuple(outs)
+
+
+# -------------------------------------------------------------- decay block
+_ROW_DTYPES = (torch.float32, torch.bfloat16, torch.float16)
+_NO_DEVICE = contextlib.nullcontext()
+
+
+def _on_device(t):
+    """The tensor's device as the current one for a launch (no cost where it is already)."""
+    return _NO_DEVICE if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+
+
+def _same_device(ref, *ts):
+    _require_cuda(ref, *ts)
+    for t in ts:
+        if t is not None and t.device != ref.device:
+            raise L.GrkError(f'all operands must be on one device ({ref.device} and {t.device})')
+
+
+def _head_rows(t, name, rows, cols, dtype):
+    """(pointer, row stride) of a [rows, cols] row-major operand (a column view is fine)."""
+    if t.dtype != dtype or t.dtype not in _ROW_DTYPES:
+        raise L.GrkError(f'{name}: dtype {t.dtype}; the row operands share one of float32, bfloat16, float16')
+    if t.dim() != 2 or t.shape[0] != rows or t.shape[1] != cols:
+        raise L.GrkError(f'{name}: shape {tuple(t.shape)}, expected ({rows}, {cols})')
+    if rows and ((cols > 1 and t.stride(1) != 1) or (rows > 1 and t.stride(0) < cols)):
+        raise L.GrkError(f'{name}: rows must be dense, with a row stride of at least {cols} elements')
+    return t.data_ptr(), t.stride(0)
+
+
+def _overlap(a, b):
+    """Whether two row-major matrices of one dtype share an element (column views of one
+    buffer with one row stride are told apart; other interleavings count as shared)."""
+    if not a.numel() or not b.numel():
+        return False
+    es = a.element_size()
+
+    def end(t):
+        return t.data_ptr() + ((t.shape[0] - 1) * t.stride(0) + t.shape[1]) * es
+
+    if a.data_ptr() >= end(b) or b.data_ptr() >= end(a):
+        return False
+    ld, gap = a.stride(0), b.data_ptr() - a.data_ptr()
+    if ld != b.stride(0) or gap % es or ld <= 0:
+        return True
+    gap = gap // es % ld
+    return not (gap >= a.shape[1] and gap + b.shape[1] <= ld)
+
+
+def _fresh(out, name, *inputs):
+    for t in inputs:
+        if t is not None and _overlap(out, t):
+            raise L.GrkError(f'{name} must not overlap an input')
+
+
+def rotary_frequencies(rotary_dim, base=10000.0, scaling=None, device=None):
+    """(freqs, scale) of rotary positions: float64 [rotary_dim / 2] radians per position,
+    base^(-2 i / rotary_dim), and the factor on the rotated columns.
+
+    scaling (for windows longer than those a model was trained on):
+      None
+      {'kind': 'linear', 'factor': f}         every frequency / f
+      {'kind': 'base', 'factor': f}           base * f^(d / (d - 2)): the lowest frequency / f, the highest kept
+      {'kind': 'by_parts', 'factor': f, 'window': n, 'fast': 32, 'slow': 1}
+          frequencies with at least `fast` turns in a window of n positions kept, those with
+          at most `slow` turns / f, a linear blend of the two (over the turns' logarithm)
+          between; scale 0.1 ln f + 1
+    """
+    d = int(rotary_dim)
+    if d < 2 or d % 2:
+        raise ValueError('rotary_dim must be even and positive')
+    i = torch.arange(0, d, 2, dtype=torch.float64)
+    kind = (scaling or {}).get('kind')
+    if kind is not None and not float(scaling.get('factor', 0.0)) >= 1.0:
+        raise ValueError('scaling needs a factor of at least 1')
+    scale = 1.0
+    if kind is None and not scaling:
+        freqs = float(base) ** (-i / d)
+    elif kind == 'linear':
+        freqs = float(base) ** (-i / d) / float(scaling['factor'])
+    elif kind == 'base':
+        if d == 2:
+            raise ValueError("scaling 'base' needs rotary_dim > 2")
+        freqs = (float(base) * float(scaling['factor']) ** (d / (d - 2))) ** (-i / d)
+    elif kind == 'by_parts':
+        f, window = float(scaling['factor']), float(scaling['window'])
+        fast, slow = float(scaling.get('fast', 32.0)), float(scaling.get('slow', 1.0))
+        if not (window > 0 and fast > slow > 0):
+            raise ValueError("scaling 'by_parts' needs window > 0 and fast > slow > 0")
+        plain = float(base) ** (-i / d)
+        turns = window * plain / (2.0 * math.pi)
+        keep = ((torch.log(turns) - math.log(slow)) / (math.log(fast) - math.log(slow))).clamp(0.0, 1.0)
+        freqs = plain * keep + plain / f * (1.0 - keep)
+        scale = 0.1 * math.log(f) + 1.0
+    else:
+        raise ValueError(f"scaling kind {kind!r}: 'linear', 'base' or 'by_parts'")
+    return freqs.to(device) if device is not None else freqs, scale
+
+
+def rotary(x, positions, freqs, heads, layout='half', scale=1.0, inverse=False, out=None):
+    """Rotary positions of [N, heads * head_dim] rows (grk_rotary): the first
+    2 * len(freqs) columns of each head turned by positions * freqs.
+
+    positions int32 / int64 [N]; freqs float64 [r] (rotary_frequencies); layout 'half'
+    (columns i, i + r) or 'interleaved' (2 i, 2 i + 1).  inverse turns back.  out: x itself
+    (in place) or a matrix that shares nothing with it; a new one by default."""
+    _same_device(x, positions, freqs, out)
+    N, cols = x.shape if x.dim() == 2 else (-1, -1)
+    if x.dim() != 2 or heads <= 0 or cols % heads or cols == 0:
+        raise L.GrkError('x must be [N, heads * head_dim]')
+    if layout not in ('half', 'interleaved'):
+        raise L.GrkError("layout must be 'half' or 'interleaved'")
+    if positions.dtype not in (torch.int32, torch.int64) or positions.shape != (N,) or not positions.is_contiguous():
+        raise L.GrkError('positions must be a contiguous int32 / int64 [N] tensor')
+    if freqs.dtype != torch.float64 or freqs.dim() != 1 or not freqs.is_contiguous():
+        raise L.GrkError('freqs must be a contiguous float64 [rotary_dim / 2] tensor')
+    xp, xl = _head_rows(x, 'x', N, cols, x.dtype)
+    if out is None:
+        out = torch.empty(N, cols, dtype=x.dtype, device=x.device)
+    elif out.data_ptr() != x.data_ptr() or out.stride(0) != x.stride(0):
+        _fresh(out, 'out', x)
+    op, ol = _head_rows(out, 'out', N, cols, x.dtype)
+    with _on_device(x):
+        rc = L.lib().grk_rotary(xp, xl, op, ol, L.dtype_code(x.dtype), positions.data_ptr(),
+                                L.itype_code(positions.dtype), freqs.data_ptr(), N, heads, cols // heads,
+                                2 * freqs.shape[0], int(layout == 'interleaved'), float(scale), int(bool(inverse)),
+                                L.stream_ptr(x.device))
+    L.check(rc, 'grk_rotary')
+    return out
+
+
+def _decay_args(q, k, v, log_decay, batch, seq_len, scale, key_valid, seq_range, row_base):
+    _same_device(q, k, v, log_decay, key_valid, seq_range, row_base)
+    if log_decay.dtype != torch.float32 or log_decay.dim() != 1 or not log_decay.is_contiguous() \
+            or not log_decay.shape[0]:
+        raise L.GrkError('log_decay must be a contiguous float32 [heads] tensor')
+    H = log_decay.shape[0]
+    if q.dim() != 2 or q.shape[1] % H or not q.shape[1]:
+        raise L.GrkError('q must be [rows, heads * head_dim]')
+    rows, cols = q.shape
+    B, T = int(batch), int(seq_len)
+    if B < 0 or T < 0 or (row_base is None and rows != B * T):
+        raise L.GrkError(f'{rows} rows do not hold {B} sequences of {T}')
+    if key_valid is not None and (key_valid.dtype != torch.uint8 or key_valid.shape != (B, T)
+                                  or not key_valid.is_contiguous()):
+        raise L.GrkError('key_valid must be a contiguous uint8 [B, T] tensor')
+    if seq_range is not None and (seq_range.dtype != torch.int32 or seq_range.shape != (B, 3)
+                                  or not seq_range.is_contiguous()):
+        raise L.GrkError('seq_range must be a contiguous int32 [B, 3] tensor (kernels.seq_ranges)')
+    if row_base is not None and (seq_range is None or row_base.dtype != torch.int64 or row_base.shape != (B + 1,)
+                                 or not row_base.is_contiguous()):
+        raise L.GrkError('row_base must be a contiguous int64 [B + 1] tensor, with seq_range (jagged_layout)')
+    hd = cols // H
+    (qp, ql), (kp, kl), (vp, vl) = [_head_rows(t, n, rows, cols, q.dtype) for t, n in ((q, 'q'), (k, 'k'), (v, 'v'))]
+    scale = hd ** -0.5 if scale is None else float(scale)
+    return L.GrkDecayArgs(B, H, T, hd, L.dtype_code(q.dtype), scale, qp, kp, vp, ql, kl, vl, log_decay.data_ptr(),
+                          _ptr(key_valid), _ptr(seq_range), _ptr(row_base),
+                          None if row_base is None else row_base.data_ptr() + 8 * B, rows)
+
+
+def _decay_workspace(args, backward, device):
+    n = L.lib().grk_decay_attn_workspace(args, int(backward))
+    return (torch.empty(n, dtype=torch.uint8, device=device) if n else None), n
+
+
+def _state_ok(t, name, shape):
+    if t.dtype != torch.float32 or tuple(t.shape) != shape or not t.is_contiguous():
+        raise L.GrkError(f'{name} must be a contiguous float32 {shape} tensor')
+    return t
+
+
+def decay_attn_fwd(q, k, v, log_decay, batch, seq_len, scale=None, key_valid=None, seq_range=None, row_base=None,
+                   state=None, return_state=False, state_out=None, out=None):
+    """Linear attention with a decay for each head (grk_decay_attn_fwd):
+    S_t = g S_{t-1} + k_t v_t^T, o_t = scale q_t S_t, g = exp(min(log_decay[h], 0)).
+
+    q / k / v: [rows, heads * head_dim] of one dtype (column views of a projection are
+    fine), head_dim <= 128; rows = batch * seq_len, or the packed rows of jagged_layout
+    with row_base and seq_range.  Positions with key_valid 0, or before seq_range's start,
+    hold no event.  scale: head_dim^-0.5 by default.
+    state: the states before the first position, fp32 [B, heads, head_dim, head_dim];
+    return_state: also those behind the last one (into state_out, which may be state)."""
+    a = _decay_args(q, k, v, log_decay, batch, seq_len, scale, key_valid, seq_range, row_base)
+    _same_device(q, state, state_out, out)
+    shape = (a.batch, a.heads, a.head_dim, a.head_dim)
+    if state is not None:
+        _state_ok(state, 'state', shape)
+    if state_out is not None:
+        _state_ok(state_out, 'state_out', shape)
+    elif return_state:
+        state_out = torch.empty(shape, dtype=torch.float32, device=q.device)
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    else:
+        _fresh(out, 'out', q, k, v)
+    op, ol = _head_rows(out, 'out', q.shape[0], q.shape[1], q.dtype)
+    with _on_device(q):
+        ws, n = _decay_workspace(a, False, q.device)
+        rc = L.lib().grk_decay_attn_fwd(a, _ptr(state), _ptr(state_out), op, ol, _ptr(ws), n, L.stream_ptr(q.device))
+    L.check(rc, 'grk_decay_attn_fwd')
+    return (out, state_out) if return_state else out
+
+
+def decay_attn_bwd(dout, q, k, v, log_decay, batch, seq_len, scale=None, key_valid=None, seq_range=None,
+                   row_base=None, dq=None, dk=None, dv=None):
+    """Gradients (dq, dk, dv) of decay_attn_fwd without states (grk_decay_attn_bwd);
+    log_decay gets none.  dq / dk / dv: matrices to write (column views are fine)."""
+    a = _decay_args(q, k, v, log_decay, batch, seq_len, scale, key_valid, seq_range, row_base)
+    _same_device(q, dout, dq, dk, dv)
+    rows, cols = q.shape
+    gp, gl = _head_rows(dout, 'dout', rows, cols, q.dtype)
+    grads = [torch.empty(rows, cols, dtype=q.dtype, device=q.device) if t is None else t for t in (dq, dk, dv)]
+    ptrs = [_head_rows(t, n, rows, cols, q.dtype) for t, n in zip(grads, ('dq', 'dk', 'dv'))]
+    for i, t in enumerate(grads):
+        _fresh(t, ('dq', 'dk', 'dv')[i], dout, q, k, v, *grads[:i])
+    (p0, l0), (p1, l1), (p2, l2) = ptrs
+    with _on_device(q):
+        ws, n = _decay_workspace(a, True, q.device)
+        rc = L.lib().grk_decay_attn_bwd(a, gp, gl, p0, l0, p1, l1, p2, l2, _ptr(ws), n, L.stream_ptr(q.device))
+    L.check(rc, 'grk_decay_attn_bwd')
+    return tuple(grads)
+
+
+def decay_attn_step(q, k, v, log_decay, state, slots=None, scale=None, err_flag=None, out=None):
+    """One event of each of n users (grk_decay_attn_step): state[slot] <- g state[slot] +
+    k v^T in place, and scale q state[slot] as a new [n, heads * head_dim] (or into out).
+
+    state fp32 [slots, heads, head_dim, head_dim]; slots int32 / int64 [n] (None: event i
+    takes state i).  Events of one slot are taken in the order of their index.  A negative
+    slot holds no event (output row zero), one past the states as well, and sets err_flag
+    (int32 [1])."""
+    _same_device(q, k, v, log_decay, state, slots, err_flag, out)
+    if log_decay.dtype != torch.float32 or log_decay.dim() != 1 or not log_decay.is_contiguous() \
+            or not log_decay.shape[0]:
+        raise L.GrkError('log_decay must be a contiguous float32 [heads] tensor')
+    H = log_decay.shape[0]
+    if q.dim() != 2 or q.shape[1] % H or not q.shape[1]:
+        raise L.GrkError('q must be [n, heads * head_dim]')
+    n, cols = q.shape
+    hd = cols // H
+    if state.dim() != 4:
+        raise L.GrkError('state must be [slots, heads, head_dim, head_dim]')
+    _state_ok(state, 'state', (state.shape[0], H, hd, hd))
+    if slots is not None and (slots.dtype not in (torch.int32, torch.int64) or slots.shape != (n,)
+                              or not slots.is_contiguous()):
+        raise L.GrkError('slots must be a contiguous int32 / int64 [n] tensor')
+    if err_flag is not None and (err_flag.dtype != torch.int32 or err_flag.numel() < 1):
+        raise L.GrkError('err_flag must be an int32 [1] tensor')
+    (qp, ql), (kp, kl), (vp, vl) = [_head_rows(t, m, n, cols, q.dtype) for t, m in ((q, 'q'), (k, 'k'), (v, 'v'))]
+    if out is None:
+        out = torch.empty(n, cols, dtype=q.dtype, device=q.device)
+    else:
+        _fresh(out, 'out', q, k, v)
+    op, ol = _head_rows(out, 'out', n, cols, q.dtype)
+    with _on_device(q):
+        nb = L.lib().grk_decay_attn_step_workspace(n, int(slots is not None))
+        ws = torch.empty(nb, dtype=torch.uint8, device=q.device) if nb else None
+        rc = L.lib().grk_decay_attn_step(qp, ql, kp, kl, vp, vl, L.dtype_code(q.dtype), log_decay.data_ptr(), n, H,
+                                         hd, hd ** -0.5 if scale is None else float(scale), state.data_ptr(),
+                                         state.shape[0], _ptr(slots),
+                                         L.itype_code(slots.dtype) if slots is not None else L.GRK_I64,
+                                         _ptr(err_flag), op, ol, _ptr(ws), nb, L.stream_ptr(q.device))
+    L.check(rc, 'grk_decay_attn_step')
+    return out
+
+
+def _norm_operands(x, weight, bias, heads, gate):
+    _same_device(x, weight, bias, gate)
+    if x.dim() != 2 or heads <= 0 or x.shape[1] % heads or not x.shape[1]:
+        raise L.GrkError('x must be [N, heads * head_dim]')
+    N, cols = x.shape
+    for t, n in ((weight, 'weight'), (bias, 'bias')):
+        if t is not None and (t.dtype != torch.float32 or t.shape != (cols,) or not t.is_contiguous()):
+            raise L.GrkError(f'{n} must be a contiguous float32 [{cols}] tensor')
+    return (*_head_rows(x, 'x', N, cols, x.dtype),
+            *(_head_rows(gate, 'gate', N, cols, x.dtype) if gate is not None else (None, 0)))
+
+
+def head_norm_fwd(x, weight, bias, heads, eps=1e-5, gate=None, out=None):
+    """Layer norm of each head's columns, times SiLU(gate) (grk_head_norm_fwd): x / gate
+    [N, heads * head_dim] of one dtype, weight / bias fp32 [heads * head_dim] or None,
+    head_dim <= 2048; heads=1 is the layer norm of a row.  out may be x or gate."""
+    xp, xl, gp, gl = _norm_operands(x, weight, bias, heads, gate)
+    N, cols = x.shape
+    _same_device(x, out)
+    if out is None:
+        out = torch.empty(N, cols, dtype=x.dtype, device=x.device)
+    else:
+        _fresh(out, 'out', *[t for t in (x, gate) if t is not None and not (
+            t.data_ptr() == out.data_ptr() and t.stride(0) == out.stride(0))])
+    op, ol = _head_rows(out, 'out', N, cols, x.dtype)
+    with _on_device(x):
+        rc = L.lib().grk_head_norm_fwd(xp, xl, gp, gl, _ptr(weight), _ptr(bias), float(eps), N, heads, cols // heads,
+                                       L.dtype_code(x.dtype), op, ol, L.stream_ptr(x.device))
+    L.check(rc, 'grk_head_norm_fwd')
+    return out
+
+
+def head_norm_bwd(dy, x, weight, bias, heads, eps=1e-5, gate=None, dx=None, dgate=None):
+    """Gradients of head_norm_fwd: (dx, dgate or None, dweight or None, dbias or None);
+    dweight / dbias fp32, in a fixed order of addition."""
+    xp, xl, gp, gl = _norm_operands(x, weight, bias, heads, gate)
+    _same_device(x, dy, dx, dgate)
+    N, cols = x.shape
+    dev, dt = x.device, x.dtype
+    yp, yl = _head_rows(dy, 'dy', N, cols, dt)
+    dx = torch.empty(N, cols, dtype=dt, device=dev) if dx is None else dx
+    if gate is None:
+        dgate = None
+    elif dgate is None:
+        dgate = torch.empty(N, cols, dtype=dt, device=dev)
+    dw = torch.empty(cols, dtype=torch.float32, device=dev) if weight is not None else None
+    db = torch.empty(cols, dtype=torch.float32, device=dev) if bias is not None else None
+    dxp, dxl = _head_rows(dx, 'dx', N, cols, dt)
+    dgp, dgl = _head_rows(dgate, 'dgate', N, cols, dt) if dgate is not None else (None, 0)
+    _fresh(dx, 'dx', dy, x, gate)
+    if dgate is not None:
+        _fresh(dgate, 'dgate', dy, x, gate, dx)
+    with _on_device(x):
+        nb = L.lib().grk_head_norm_bwd_workspace(N, heads, cols // heads) if dw is not None or db is not None else 0
+        ws = torch.empty(nb, dtype=torch.uint8, device=dev) if nb else None
+        rc = L.lib().grk_head_norm_bwd(yp, yl, xp, xl, gp, gl, _ptr(weight), _ptr(bias), float(eps), N, heads,
+                                       cols // heads, L.dtype_code(dt), dxp, dxl, dgp, dgl, _ptr(dw), _ptr(db),
+                                       _ptr(ws), nb, L.stream_ptr(dev))
+    L.check(rc, 'grk_head_norm_bwd')
+    return dx, dgate, dw, db
 
 
 # -------------------------------------------------------------- pair logits
