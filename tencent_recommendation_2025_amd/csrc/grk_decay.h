@@ -127,4 +127,10 @@ __device__ __forceinline__ void mfma_keep(f32x4& acc, const A& a, const B& b) {
   asm("" : "+v"(acc) : "v"(a), "v"(b));
 }
 
+// host: the bf16 kernels (grk_decay_bf16.hip)
+bool decay_bf16_takes(const DecayParams& p);
+int decay_bf16_launch(const DecayParams& p, hipStream_t s);
+// the segments' scan (grk_decay.hip), for states padded to dp
+int decay_scan_launch(const DecayParams& p, int dp, hipStream_t s);
+
 }  // namespace grk

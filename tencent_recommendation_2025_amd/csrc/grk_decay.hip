@@ -347,6 +347,19 @@ __global__ void __launch_bounds__(kStepThreads) k_decay_step(StepParams p) {
 }
 
 // ------------------------------------------------------------------ launch --
+int decay_scan_launch(const DecayParams& p, int dp, hipStream_t s) {
+  const int64_t n = (int64_t)p.roles * p.batch * p.heads * dp * dp / 4;
+  const unsigned grid = (unsigned)((n + 255) / 256);
+  switch (dp) {
+    case 16: k_decay_scan<16><<<grid, 256, 0, s>>>(p); break;
+    case 32: k_decay_scan<32><<<grid, 256, 0, s>>>(p); break;
+    case 64: k_decay_scan<64><<<grid, 256, 0, s>>>(p); break;
+    default: k_decay_scan<128><<<grid, 256, 0, s>>>(p); break;
+  }
+  GRK_LAUNCH_CHECK();
+  return GRK_OK;
+}
+
 static int decay_dp(int hd) { return hd <= 16 ? 16 : hd <= 32 ? 32 : hd <= 64 ? 64 : 128; }
 
 // Segments: a workgroup walks a sequence alone where the (sequence, head) pairs already
@@ -366,7 +379,8 @@ static void decay_segments(DecayParams& p) {
 
 static size_t decay_ws(const DecayParams& p) {
   if (p.nseg <= 1) return 0;
-  const size_t dp = decay_dp(p.head_dim);
+  // (the bf16 kernels pad the narrowest heads to 32 columns)
+  const size_t dp = p.head_dim <= 16 ? 32 : decay_dp(p.head_dim);
   return (size_t)p.roles * p.batch * p.heads * p.nseg * dp * dp * sizeof(float);
 }
 
@@ -407,9 +421,8 @@ static int decay_run(const DecayParams& p, hipStream_t s) {
     GRK_CHECK_HIP(ensure_dynamic_lds((const void*)k_decay_f32<T, V, DP, true>, lds));
     k_decay_f32<T, V, DP, true><<<grid, DP * 4, lds, s>>>(p);
     GRK_LAUNCH_CHECK();
-    const int64_t n = (int64_t)p.roles * p.batch * p.heads * DP * DP / 4;
-    k_decay_scan<DP><<<(unsigned)((n + 255) / 256), 256, 0, s>>>(p);
-    GRK_LAUNCH_CHECK();
+    const int rc = decay_scan_launch(p, DP, s);
+    if (rc) return rc;
   }
   constexpr size_t lds = decay_lds_f32<DP>(false);
   GRK_CHECK_HIP(ensure_dynamic_lds((const void*)k_decay_f32<T, V, DP, false>, lds));
@@ -419,6 +432,7 @@ static int decay_run(const DecayParams& p, hipStream_t s) {
 }
 
 static int decay_launch(const DecayParams& p, int dtype, hipStream_t s) {
+  if (dtype == GRK_BF16 && decay_bf16_takes(p)) return decay_bf16_launch(p, s);
   // 8- or 16-byte loads of 4 columns: rows and heads start on them
   bool vec = p.head_dim % 4 == 0;
   const size_t b4 = 4 * dtype_size(dtype);
