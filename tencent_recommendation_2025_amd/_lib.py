@@ -262,6 +262,11 @@ def stream_ptr(device=None) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
+def raw_stream(index: int) -> int:
+    """stream_ptr of a device index, without the stream object."""
+    return torch._C._cuda_getCurrentRawStream(index)
+
+
 def dtype_code(t: torch.dtype) -> int:
     if t == torch.float32:
         return GRK_F32

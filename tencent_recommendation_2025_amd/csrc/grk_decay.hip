@@ -199,11 +199,19 @@ __global__ void __launch_bounds__(256) k_decay_scan(DecayParams p) {
         run[e] = g0 * p.state_in[(bh * p.head_dim + d0 + e) * p.head_dim + col];
   }
   f32x4* own = reinterpret_cast<f32x4*>(p.ws + rbh * p.nseg * DP * DP) + f;
-  for (int s = 0; s < p.nseg; ++s) {
-    const int left = len - s * p.seg_len, n = left < 0 ? 0 : (left < p.seg_len ? left : p.seg_len);
-    const f32x4 x = own[(int64_t)s * (DP * DP / 4)];
-    own[(int64_t)s * (DP * DP / 4)] = run;
-    run = run * decay_pow(lg, n) + x;
+  constexpr int U = 8;   // loads in flight: the recurrence itself is short
+  for (int s0 = 0; s0 < p.nseg; s0 += U) {
+    f32x4 x[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (s0 + u < p.nseg) x[u] = own[(int64_t)(s0 + u) * (DP * DP / 4)];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int s = s0 + u, left = len - s * p.seg_len, n = left < 0 ? 0 : (left < p.seg_len ? left : p.seg_len);
+      if (s >= p.nseg) break;
+      own[(int64_t)s * (DP * DP / 4)] = run;
+      run = run * decay_pow(lg, n) + x[u];
+    }
   }
   if (p.state_out) {
 #pragma unroll
@@ -244,28 +252,35 @@ __device__ __forceinline__ int64_t step_slot(const StepParams& p, int64_t i) {
 
 // Events of one slot are consecutive events of that user: the first one's workgroup
 // takes them all, in order.  links[i] = (an earlier event has this slot, the next event
-// that has it), by comparing every pair.
+// that has it), by comparing every pair: 8 threads an event, an eighth of the others each.
+constexpr int kLinkShare = 8;
 __global__ void __launch_bounds__(kStepThreads) k_step_links(StepParams p) {
   __shared__ int64_t tile[kStepThreads];
-  const int64_t i = (int64_t)blockIdx.x * kStepThreads + threadIdx.x;
+  const int64_t i = (int64_t)blockIdx.x * (kStepThreads / kLinkShare) + threadIdx.x / kLinkShare;
   const int64_t mine = i < p.n ? step_slot(p, i) : -1;
   int before = 0;
-  int64_t next = -1;
+  int next = 0x7fffffff;
   for (int64_t j0 = 0; j0 < p.n; j0 += kStepThreads) {
     __syncthreads();
-    tile[threadIdx.x] = j0 + threadIdx.x < p.n ? step_slot(p, j0 + threadIdx.x) : -1;
+    tile[threadIdx.x] = j0 + threadIdx.x < p.n ? step_slot(p, j0 + threadIdx.x) : -2;
     __syncthreads();
-    const int m = (int)(p.n - j0 < kStepThreads ? p.n - j0 : kStepThreads);
-    if (mine >= 0)
-      for (int t = 0; t < m; ++t)
-        if (tile[t] == mine) {
-          if (j0 + t < i) before = 1;
-          else if (j0 + t > i && next < 0) next = j0 + t;
-        }
+#pragma unroll 8
+    for (int t = threadIdx.x % kLinkShare; t < kStepThreads; t += kLinkShare) {
+      const int j = (int)j0 + t;
+      const bool same = tile[t] == mine;
+      before |= same && j < i;
+      next = same && j > i && j < next ? j : next;
+    }
   }
-  if (i < p.n) {
+#pragma unroll
+  for (int off = kLinkShare / 2; off > 0; off >>= 1) {
+    before |= __shfl_xor(before, off);
+    const int o = __shfl_xor(next, off);
+    next = o < next ? o : next;
+  }
+  if (i < p.n && threadIdx.x % kLinkShare == 0) {
     p.links[2 * i] = before;
-    p.links[2 * i + 1] = (int)next;
+    p.links[2 * i + 1] = next == 0x7fffffff ? -1 : next;
   }
 }
 
@@ -547,7 +562,8 @@ extern "C" int grk_decay_attn_step(const void* q, int64_t ldq, const void* k, in
   p.scale = scale; p.err = err_flag; p.out = out; p.ldo = ldo; p.links = need ? (int32_t*)ws : nullptr;
   hipStream_t s = (hipStream_t)stream;
   if (need) {
-    k_step_links<<<(unsigned)((n + kStepThreads - 1) / kStepThreads), kStepThreads, 0, s>>>(p);
+    constexpr int per = kStepThreads / kLinkShare;
+    k_step_links<<<(unsigned)((n + per - 1) / per), kStepThreads, 0, s>>>(p);
     GRK_LAUNCH_CHECK();
   }
   const unsigned grid = (unsigned)(n * heads);

@@ -1,8 +1,8 @@
 // Decayed linear attention of bf16 rows on the bf16 matrix instruction, for gfx950 (the
 // formulas: grk_decay.h; heads and rows made of 16-byte vectors).
 //
-// A workgroup walks a segment in chunks of 64 steps; wave w of DP / 16 owns columns
-// [16 w, 16 w + 16) of the state and of the output.  v_mfma_f32_16x16x32_bf16: lane
+// A workgroup walks a segment in chunks of 64 steps; each wave owns NE tiles of 16 columns
+// of the state and of the output.  v_mfma_f32_16x16x32_bf16: lane
 // l = 16 g + c holds A[c][8 g + s] and B[8 g + s][c], s < 8, and D[4 g + i][c], i < 4 -- A
 // and B fragments are laid out alike, so exchanging them transposes D.  What is stored
 // comes out transposed on purpose: P^T = K Q^T and O^T = V^T P^T + S^T Q^T leave 4
@@ -61,17 +61,18 @@ __device__ __forceinline__ bf16x8 pack8(const float* f) {
   return r;
 }
 
-// Rows of a chunk on their way from memory: thread t holds columns [8 (t % (DP / 8)), + 8) of rows
-// t / (DP / 8) and 32 more.  Masked steps are loaded too (their row exists) and zeroed by
+// Rows of a chunk on their way from memory: thread t holds columns [8 (t % (DP / 8)), + 8) of
+// row t / (DP / 8) and of every R-th after it, R = threads / (DP / 8).  Masked steps are loaded too (their row exists) and zeroed by
 // selection, so the loads do not wait for the mask.
-template <int DP>
+template <int DP, int NTH>
 struct DecayRows {
-  int64_t row[2];
-  bool live[2];
+  static constexpr int R = NTH / (DP / 8), N = kDecayChunk / R;
+  int64_t row[N];
+  bool live[N];
   __device__ __forceinline__ void at(const DecayParams& p, const DecayPlace& w, int rev, int64_t base, int t0) {
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const int t = t0 + (int)threadIdx.x / (DP / 8) + 32 * k;
+    for (int k = 0; k < N; ++k) {
+      const int t = t0 + (int)threadIdx.x / (DP / 8) + R * k;
       const int pos = rev ? p.seq_len - 1 - t : w.start + t;
       const int64_t r = base + pos;
       live[k] = t < w.t1 && r >= 0 && r < p.capacity;
@@ -81,13 +82,13 @@ struct DecayRows {
   }
   __device__ __forceinline__ void load(uint4* f, const void* src, int64_t ld, int64_t col) const {
 #pragma unroll
-    for (int k = 0; k < 2; ++k)
+    for (int k = 0; k < N; ++k)
       f[k] = *reinterpret_cast<const uint4*>(reinterpret_cast<const bf16_t*>(src) + row[k] * ld + col);
   }
   __device__ __forceinline__ void store(const uint4* f, char* dst, bool has) const {
 #pragma unroll
-    for (int k = 0; k < 2; ++k)
-      *reinterpret_cast<uint4*>(dst + lds_off<DP>((int)threadIdx.x / (DP / 8) + 32 * k, (int)threadIdx.x % (DP / 8) * 8)) =
+    for (int k = 0; k < N; ++k)
+      *reinterpret_cast<uint4*>(dst + lds_off<DP>((int)threadIdx.x / (DP / 8) + R * k, (int)threadIdx.x % (DP / 8) * 8)) =
           live[k] && has ? f[k] : make_uint4(0u, 0u, 0u, 0u);
   }
 };
@@ -95,9 +96,10 @@ struct DecayRows {
 // NS: bf16 parts of g^(n-1-j) v_j in the state's sum.  1 where the state only feeds bf16
 // outputs (it is rounded to bf16 as their operand anyway); 3 (all 24 bits of the fp32
 // value) where it is returned in fp32.
-template <int DP, int NS, bool STATE>
-__global__ void __launch_bounds__(DP * 4, 4) k_decay_bf16(DecayParams p) {
-  constexpr int C = kDecayChunk, NT = DP / 16, KS = DP / 32;
+template <int DP, int NE, int NS, bool STATE>
+__global__ void __launch_bounds__(DP * 4 / NE, NE == 1 ? 4 : 2) k_decay_bf16(DecayParams p) {
+  constexpr int C = kDecayChunk, NT = DP / 16, KS = DP / 32, NW = NT / NE, NTH = NW * 64;
+  using Rows = DecayRows<DP, NTH>;
   extern __shared__ __attribute__((aligned(16))) char lds[];
   char* sb = lds;
   char* sc = sb + C * DP * 2;
@@ -115,34 +117,38 @@ __global__ void __launch_bounds__(DP * 4, 4) k_decay_bf16(DecayParams p) {
   const int ccol = (int)threadIdx.x % (DP / 8) * 8;      // this thread's columns when rows are moved
   const bool has = ccol < p.head_dim;
   const int64_t mcol = hcol + (has ? ccol : 0);
-  f32x4 st[NT];
+  f32x4 st[NE][NT];
   float* frag = p.ws + (((int64_t)w.role * p.batch * p.heads + bh) * p.nseg + w.seg) * DP * DP;
   bool some = STATE || (p.nseg > 1 ? w.seg > 0 || p.state_in : p.state_in != nullptr);   // the state is not all 0
 #pragma unroll
-  for (int dt = 0; dt < NT; ++dt) {
-    st[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
-    if (!STATE && p.nseg > 1) {
-      st[dt] = *reinterpret_cast<const f32x4*>(frag + ((dt * NT + wave) * 64 + lane) * 4);
-    } else if (!STATE && p.state_in) {
-      const float f = decay_pow(w.lg, w.start);
+  for (int x = 0; x < NE; ++x) {
+    const int et = NE * wave + x;   // the wave's column tiles
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int d = 16 * dt + 4 * g + i, e = 16 * wave + c;
-        if (d < p.head_dim && e < p.head_dim) st[dt][i] = f * p.state_in[(bh * p.head_dim + d) * p.head_dim + e];
+    for (int dt = 0; dt < NT; ++dt) {
+      st[x][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+      if (!STATE && p.nseg > 1) {
+        st[x][dt] = *reinterpret_cast<const f32x4*>(frag + ((dt * NT + et) * 64 + lane) * 4);
+      } else if (!STATE && p.state_in) {
+        const float f = decay_pow(w.lg, w.start);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int d = 16 * dt + 4 * g + i, e = 16 * et + c;
+          if (d < p.head_dim && e < p.head_dim) st[x][dt][i] = f * p.state_in[(bh * p.head_dim + d) * p.head_dim + e];
+        }
       }
     }
   }
-  DecayRows<DP> rows;
-  uint4 fa[2], fb[2], fc[2];
+  Rows rows;
+  uint4 fa[Rows::N], fb[Rows::N], fc[Rows::N];
   if (w.t0 < w.t1) {
     rows.at(p, w, r.rev, base, w.t0);
     rows.load(fb, r.b, r.ldb, mcol);
     rows.load(fc, r.c, r.ldc, mcol);
     if (!STATE) rows.load(fa, r.a, r.lda, mcol);
   }
-  for (int n = threadIdx.x; n < kDecayPowers; n += DP * 4) pw[n - 16] = n < 16 ? 0.f : decay_pow(w.lg, n - 16);
+  for (int n = threadIdx.x; n < kDecayPowers; n += NTH) pw[n - 16] = n < 16 ? 0.f : decay_pow(w.lg, n - 16);
   if constexpr (!STATE) {
-    for (int n = threadIdx.x; n < C * C / 8; n += DP * 4) reinterpret_cast<uint4*>(sp)[n] = make_uint4(0u, 0u, 0u, 0u);
+    for (int n = threadIdx.x; n < C * C / 8; n += NTH) reinterpret_cast<uint4*>(sp)[n] = make_uint4(0u, 0u, 0u, 0u);
     decay_zero_rows<bf16_t>(p, w, r);
   }
   for (int t0 = w.t0; t0 < w.t1; t0 += C) {
@@ -155,7 +161,7 @@ __global__ void __launch_bounds__(DP * 4, 4) k_decay_bf16(DecayParams p) {
       rows.store(fa, sa, has);
       if (ccol == 0) {
 #pragma unroll
-        for (int k = 0; k < 2; ++k) slive[(int)threadIdx.x / (DP / 8) + 32 * k] = rows.live[k];
+        for (int k = 0; k < Rows::N; ++k) slive[(int)threadIdx.x / (DP / 8) + Rows::R * k] = rows.live[k];
       }
     }
     __syncthreads();
@@ -167,7 +173,7 @@ __global__ void __launch_bounds__(DP * 4, 4) k_decay_bf16(DecayParams p) {
     }
     if constexpr (!STATE) {
       // P^T, lower tiles; the tiles above the diagonal that a 32-deep step reads stay 0
-      for (int tile = wave; tile < 10; tile += NT) {
+      for (int tile = wave; tile < 10; tile += NW) {
         const int it = tile >= 6 ? 3 : tile >= 3 ? 2 : tile >= 1 ? 1 : 0, jt = tile - it * (it + 1) / 2;
         f32x4 x = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -181,35 +187,55 @@ __global__ void __launch_bounds__(DP * 4, 4) k_decay_bf16(DecayParams p) {
       }
       __syncthreads();
     }
-    bf16x8 vf[2];
+    bf16x8 vf[NE][2];
 #pragma unroll
-    for (int ks = 0; ks < 2; ++ks) vf[ks] = lds_col8<DP>(sc, 32 * ks, 16 * wave, lane);
+    for (int x = 0; x < NE; ++x)
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks) vf[x][ks] = lds_col8<DP>(sc, 32 * ks, 16 * (NE * wave + x), lane);
     if constexpr (!STATE) {
-      bf16x8 sf[KS];
+      bf16x8 sf[NE][KS];
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) {
-        const float f[8] = {st[2 * ks][0], st[2 * ks][1], st[2 * ks][2], st[2 * ks][3],
-                            st[2 * ks + 1][0], st[2 * ks + 1][1], st[2 * ks + 1][2], st[2 * ks + 1][3]};
-        sf[ks] = pack8(f);
-      }
+      for (int x = 0; x < NE; ++x)
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+          const f32x4 a = st[x][2 * ks], b = st[x][2 * ks + 1];
+          const float f[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+          sf[x][ks] = pack8(f);
+        }
 #pragma unroll
       for (int it = 0; it < C / 16; ++it) {
-        f32x4 x = {0.f, 0.f, 0.f, 0.f};
+        f32x4 o[NE];
+#pragma unroll
+        for (int x = 0; x < NE; ++x) o[x] = f32x4{0.f, 0.f, 0.f, 0.f};
         if (some) {
 #pragma unroll
-          for (int ks = 0; ks < KS; ++ks) mfma32(sf[ks], lds_row_pair<DP>(sa, 16 * it + c, 32 * ks, g), x);
-          x *= pw[16 * it + c + 1];
-        }
-        mfma32(vf[0], lds_row8<C>(sp, 16 * it + c, 8 * g), x);
-        if (it >= 2) mfma32(vf[1], lds_row8<C>(sp, 16 * it + c, 32 + 8 * g), x);
-        const int t = 16 * it + c, e = 16 * wave + 4 * g;
-        const int64_t row = base + (r.rev ? p.seq_len - 1 - (t0 + t) : w.start + t0 + t);
-        if (t < n && row >= 0 && row < p.capacity && e < p.head_dim) {
-          const float f = slive[t] ? p.scale : 0.f;
-          bf16x4 y;
+          for (int ks = 0; ks < KS; ++ks) {
+            const bf16x8 q = lds_row_pair<DP>(sa, 16 * it + c, 32 * ks, g);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) y[i] = (__bf16)(slive[t] ? f * x[i] : 0.f);
-          *reinterpret_cast<bf16x4*>(reinterpret_cast<bf16_t*>(r.out) + row * r.ldo + hcol + e) = y;
+            for (int x = 0; x < NE; ++x) mfma32(sf[x][ks], q, o[x]);
+          }
+#pragma unroll
+          for (int x = 0; x < NE; ++x) o[x] *= pw[16 * it + c + 1];
+        }
+#pragma unroll
+        for (int ks = 0; ks <= it / 2; ++ks) {
+          const bf16x8 y = lds_row8<C>(sp, 16 * it + c, 32 * ks + 8 * g);
+#pragma unroll
+          for (int x = 0; x < NE; ++x) mfma32(vf[x][ks], y, o[x]);
+        }
+        const int t = 16 * it + c;
+        const int64_t row = base + (r.rev ? p.seq_len - 1 - (t0 + t) : w.start + t0 + t);
+        if (t < n && row >= 0 && row < p.capacity) {
+          const bool live = slive[t];
+#pragma unroll
+          for (int x = 0; x < NE; ++x) {
+            const int e = 16 * (NE * wave + x) + 4 * g;
+            bf16x4 y;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) y[i] = (__bf16)(live ? p.scale * o[x][i] : 0.f);
+            if (e < p.head_dim)
+              *reinterpret_cast<bf16x4*>(reinterpret_cast<bf16_t*>(r.out) + row * r.ldo + hcol + e) = y;
+          }
         }
       }
     }
@@ -217,57 +243,66 @@ __global__ void __launch_bounds__(DP * 4, 4) k_decay_bf16(DecayParams p) {
     some = true;
     const float gn = pw[n];
 #pragma unroll
-    for (int dt = 0; dt < NT; ++dt) st[dt] *= gn;
+    for (int x = 0; x < NE; ++x)
+#pragma unroll
+      for (int dt = 0; dt < NT; ++dt) st[x][dt] *= gn;
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks) {
-      float f[8];
-      bf16x8 part[NS];
+      bf16x8 part[NE][NS];
 #pragma unroll
-      for (int s = 0; s < 8; ++s) {
-        const int j = 32 * ks + 8 * g + s;
-        f[s] = (float)vf[ks][s] * (j < n ? pw[n - 1 - j] : 0.f);
-      }
+      for (int x = 0; x < NE; ++x) {
+        float f[8];
 #pragma unroll
-      for (int q = 0; q < NS; ++q) {
-        part[q] = pack8(f);
+        for (int s = 0; s < 8; ++s) {
+          const int j = 32 * ks + 8 * g + s;
+          f[s] = (float)vf[x][ks][s] * (j < n ? pw[n - 1 - j] : 0.f);
+        }
 #pragma unroll
-        for (int s = 0; s < 8; ++s) f[s] -= (float)part[q][s];
+        for (int q = 0; q < NS; ++q) {
+          part[x][q] = pack8(f);
+#pragma unroll
+          for (int s = 0; s < 8; ++s) f[s] -= (float)part[x][q][s];
+        }
       }
 #pragma unroll
       for (int dt = 0; dt < NT; ++dt) {
         const bf16x8 k = lds_col8<DP>(sb, 32 * ks, 16 * dt, lane);
 #pragma unroll
-        for (int q = NS - 1; q >= 0; --q) mfma32(k, part[q], st[dt]);
+        for (int x = 0; x < NE; ++x)
+#pragma unroll
+          for (int q = NS - 1; q >= 0; --q) mfma32(k, part[x][q], st[x][dt]);
       }
     }
   }
-  if (STATE) {
 #pragma unroll
-    for (int dt = 0; dt < NT; ++dt)
-      *reinterpret_cast<f32x4*>(frag + ((dt * NT + wave) * 64 + lane) * 4) = st[dt];
-  } else if (p.nseg == 1 && p.state_out) {
+  for (int x = 0; x < NE; ++x)
 #pragma unroll
-    for (int dt = 0; dt < NT; ++dt)
+    for (int dt = 0; dt < NT; ++dt) {
+      const int et = NE * wave + x;
+      if (STATE) {
+        *reinterpret_cast<f32x4*>(frag + ((dt * NT + et) * 64 + lane) * 4) = st[x][dt];
+      } else if (p.nseg == 1 && p.state_out) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int d = 16 * dt + 4 * g + i, e = 16 * wave + c;
-        if (d < p.head_dim && e < p.head_dim) p.state_out[(bh * p.head_dim + d) * p.head_dim + e] = st[dt][i];
+        for (int i = 0; i < 4; ++i) {
+          const int d = 16 * dt + 4 * g + i, e = 16 * et + c;
+          if (d < p.head_dim && e < p.head_dim) p.state_out[(bh * p.head_dim + d) * p.head_dim + e] = st[x][dt][i];
+        }
       }
-  }
+    }
 }
 
-template <int DP>
+template <int DP, int NE>
 static int decay_bf16_run(const DecayParams& p, hipStream_t s) {
   const int64_t groups = (int64_t)p.batch * p.heads * p.nseg;
   const unsigned grid = (unsigned)((groups + 7) / 8 * 8 * p.roles);
   if (p.nseg > 1) {
     constexpr size_t lds = decay_lds_bf16<DP>(true);
     if (p.state_out) {
-      GRK_CHECK_HIP(ensure_dynamic_lds((const void*)k_decay_bf16<DP, 3, true>, lds));
-      k_decay_bf16<DP, 3, true><<<grid, DP * 4, lds, s>>>(p);
+      GRK_CHECK_HIP(ensure_dynamic_lds((const void*)k_decay_bf16<DP, NE, 3, true>, lds));
+      k_decay_bf16<DP, NE, 3, true><<<grid, DP * 4 / NE, lds, s>>>(p);
     } else {
-      GRK_CHECK_HIP(ensure_dynamic_lds((const void*)k_decay_bf16<DP, 1, true>, lds));
-      k_decay_bf16<DP, 1, true><<<grid, DP * 4, lds, s>>>(p);
+      GRK_CHECK_HIP(ensure_dynamic_lds((const void*)k_decay_bf16<DP, NE, 1, true>, lds));
+      k_decay_bf16<DP, NE, 1, true><<<grid, DP * 4 / NE, lds, s>>>(p);
     }
     GRK_LAUNCH_CHECK();
     const int rc = decay_scan_launch(p, DP, s);
@@ -275,11 +310,11 @@ static int decay_bf16_run(const DecayParams& p, hipStream_t s) {
   }
   constexpr size_t lds = decay_lds_bf16<DP>(false);
   if (p.nseg == 1 && p.state_out) {
-    GRK_CHECK_HIP(ensure_dynamic_lds((const void*)k_decay_bf16<DP, 3, false>, lds));
-    k_decay_bf16<DP, 3, false><<<grid, DP * 4, lds, s>>>(p);
+    GRK_CHECK_HIP(ensure_dynamic_lds((const void*)k_decay_bf16<DP, NE, 3, false>, lds));
+    k_decay_bf16<DP, NE, 3, false><<<grid, DP * 4 / NE, lds, s>>>(p);
   } else {
-    GRK_CHECK_HIP(ensure_dynamic_lds((const void*)k_decay_bf16<DP, 1, false>, lds));
-    k_decay_bf16<DP, 1, false><<<grid, DP * 4, lds, s>>>(p);
+    GRK_CHECK_HIP(ensure_dynamic_lds((const void*)k_decay_bf16<DP, NE, 1, false>, lds));
+    k_decay_bf16<DP, NE, 1, false><<<grid, DP * 4 / NE, lds, s>>>(p);
   }
   GRK_LAUNCH_CHECK();
   return GRK_OK;
@@ -297,9 +332,9 @@ bool decay_bf16_takes(const DecayParams& p) {
 }
 
 int decay_bf16_launch(const DecayParams& p, hipStream_t s) {
-  if (p.head_dim <= 32) return decay_bf16_run<32>(p, s);
-  if (p.head_dim <= 64) return decay_bf16_run<64>(p, s);
-  return decay_bf16_run<128>(p, s);
+  if (p.head_dim <= 32) return decay_bf16_run<32, 1>(p, s);
+  if (p.head_dim <= 64) return decay_bf16_run<64, 1>(p, s);
+  return decay_bf16_run<128, 2>(p, s);
 }
 
 }  // namespace grk

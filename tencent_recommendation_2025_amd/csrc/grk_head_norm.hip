@@ -19,7 +19,8 @@
 namespace grk {
 
 constexpr int kHnThreads = 256;
-constexpr int kHnBwdBlocks = 512;      // row blocks of a backward at most: two on each CU
+constexpr int kHnFwdBlocks = 2048;     // workgroups of a forward at most: a full card, each walking its rows
+constexpr int kHnBwdBlocks = 1024;     // row blocks of a backward at most: 4 workgroups on each CU
 constexpr int kHnMaxDim = 2048;
 
 struct HNParams {
@@ -29,6 +30,7 @@ struct HNParams {
   float eps;
   int64_t rows; int heads, dim;
   int head_tile, rows_per_iter;             // heads and rows of a workgroup's tile
+  int vec_affine;                           // weight and bias start on 16 bytes
   void* y; int64_t ldy;
   // backward
   const void* dy; int64_t lddy;
@@ -120,14 +122,23 @@ __device__ __forceinline__ float hn_normalise(float* x, int dim, int lane, float
 }
 
 template <int V, int LPG, int VPL>
-__device__ __forceinline__ void hn_affine(const float* src, int head, int dim, int lane, float none, float* f) {
+__device__ __forceinline__ void hn_affine(const float* src, bool vec, int head, int dim, int lane, float none,
+                                          float* f) {
 #pragma unroll
-  for (int j = 0; j < VPL; ++j)
+  for (int j = 0; j < VPL; ++j) {
+    const int c = (lane + LPG * j) * V;
 #pragma unroll
-    for (int e = 0; e < V; ++e) {
-      const int c = (lane + LPG * j) * V + e;
-      f[j * V + e] = src && c < dim ? src[(int64_t)head * dim + c] : none;
+    for (int e = 0; e < V; ++e) f[j * V + e] = none;
+    if (!src || c >= dim) continue;
+    const float* s = src + (int64_t)head * dim + c;
+    if (V >= 4 && vec) {
+#pragma unroll
+      for (int e = 0; e + 3 < V; e += 4) vload<float, 4>(s + e, f + j * V + e);
+    } else {
+#pragma unroll
+      for (int e = 0; e < V; ++e) f[j * V + e] = s[e];
     }
+  }
 }
 
 template <typename T, int V, int LPG, int VPL>
@@ -136,8 +147,8 @@ __global__ void __launch_bounds__(kHnThreads) k_hn_fwd(HNParams p) {
   const HNPlace t = hn_place<LPG>(p);
   if (!t.on) return;   // whole groups of LPG lanes leave together
   float w[E], b[E];
-  hn_affine<V, LPG, VPL>(p.weight, t.head, p.dim, t.lane, 1.f, w);
-  hn_affine<V, LPG, VPL>(p.bias, t.head, p.dim, t.lane, 0.f, b);
+  hn_affine<V, LPG, VPL>(p.weight, p.vec_affine, t.head, p.dim, t.lane, 1.f, w);
+  hn_affine<V, LPG, VPL>(p.bias, p.vec_affine, t.head, p.dim, t.lane, 0.f, b);
   for (int64_t row = (int64_t)blockIdx.x * p.rows_per_iter + t.row; row < p.rows;
        row += (int64_t)gridDim.x * p.rows_per_iter) {
     float z[E], u[E];
@@ -162,8 +173,8 @@ __global__ void __launch_bounds__(kHnThreads) k_hn_bwd(HNParams p) {
 #pragma unroll
   for (int i = 0; i < E; ++i) dw[i] = db[i] = 0.f;
   if (t.on) {
-    hn_affine<V, LPG, VPL>(p.weight, t.head, p.dim, t.lane, 1.f, w);
-    hn_affine<V, LPG, VPL>(p.bias, t.head, p.dim, t.lane, 0.f, b);
+    hn_affine<V, LPG, VPL>(p.weight, p.vec_affine, t.head, p.dim, t.lane, 1.f, w);
+    hn_affine<V, LPG, VPL>(p.bias, p.vec_affine, t.head, p.dim, t.lane, 0.f, b);
     const float inv = 1.f / (float)p.dim;
     for (int64_t row = (int64_t)blockIdx.x * p.rows_per_iter + t.row; row < p.rows;
          row += (int64_t)gridDim.x * p.rows_per_iter) {
@@ -228,16 +239,19 @@ __global__ void __launch_bounds__(kHnThreads) k_hn_bwd(HNParams p) {
   }
 }
 
-// out[i] = sum over the row blocks' partials, 4 groups of blocks in a fixed order.
-constexpr int kHnColGroups = 4;
+// out[i] = sum over the row blocks' partials: 16 threads a column, each every 16th block
+// in order, their sums in order.
+constexpr int kHnColGroups = 16;
 __global__ void __launch_bounds__(64 * kHnColGroups) k_hn_colsum(const float* partial, int nblocks, int64_t cols,
                                                                   float* dw, float* db) {
   __shared__ float part[kHnColGroups][64];
   const int cl = threadIdx.x & 63, g = threadIdx.x >> 6;
   const int64_t i = (int64_t)blockIdx.x * 64 + cl;
   float s = 0.f;
-  if (i < 2 * cols)
+  if (i < 2 * cols) {
+#pragma unroll 8
     for (int b = g; b < nblocks; b += kHnColGroups) s += partial[(int64_t)b * 2 * cols + i];
+  }
   part[g][cl] = s;
   __syncthreads();
   if (g == 0 && i < 2 * cols) {
@@ -267,6 +281,7 @@ static HNShape hn_shape(int dim, int dtype, bool vec) {
 }
 
 static void hn_tile(const HNShape& s, HNParams& p) {
+  p.vec_affine = ((uintptr_t)p.weight | (uintptr_t)p.bias) % 16 == 0;
   const int groups = kHnThreads / s.lpg;
   p.head_tile = p.heads < groups ? p.heads : groups;
   p.rows_per_iter = groups / p.head_tile;
@@ -333,7 +348,8 @@ extern "C" int grk_head_norm_fwd(const void* x, int64_t ldx, const void* gate, i
   const HNShape c = hn_shape(head_dim, dtype, vec);
   hn_tile(c, p);
   const int64_t iters = (rows + p.rows_per_iter - 1) / p.rows_per_iter;
-  const int64_t most = (1 << 22) / ((heads + p.head_tile - 1) / p.head_tile);   // workgroups of one launch
+  const int gy = (heads + p.head_tile - 1) / p.head_tile;
+  const int64_t most = gy < kHnFwdBlocks ? kHnFwdBlocks / gy : 1;
   const unsigned gx = (unsigned)(iters < most ? iters : most);
   rc = for_dtype(dtype, [&](auto t) { return hn_run<decltype(t)>(p, c, false, gx, (hipStream_t)stream); });
   if (rc) return rc;

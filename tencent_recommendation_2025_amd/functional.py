@@ -1008,11 +1008,22 @@ def hstu_core_fp8(pre, rab, ln_w, ln_b, key_valid, B, T, H, hd, inv_n, eps=1e-8,
 def _head_mat(x, dt=None):
     """x as a [N, D] matrix the decay block's kernels read: dense rows at a row stride of
     at least D (an expanded gradient is copied), of dtype dt."""
-    x = x.reshape(-1, x.shape[-1])
+    if x.dim() != 2:
+        x = x.reshape(-1, x.shape[-1])
     if dt is not None and x.dtype != dt:
         x = x.to(dt)
-    ok = (x.shape[1] == 1 or x.stride(1) == 1) and (x.shape[0] <= 1 or x.stride(0) >= x.shape[1])
-    return x if ok else x.contiguous()
+    ld, one = x.stride()
+    N, D = x.shape
+    return x if (one == 1 or D == 1) and (ld >= D or N <= 1) else x.contiguous()
+
+
+def _once(backward):
+    """once_differentiable, without its cost where no graph of the gradient is asked for."""
+    guarded = torch.autograd.function.once_differentiable(backward)
+
+    def run(ctx, *grads):
+        return guarded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+    return run
 
 
 class _RotaryFn(torch.autograd.Function):
@@ -1023,7 +1034,7 @@ class _RotaryFn(torch.autograd.Function):
         return K.rotary(_head_mat(x), positions, freqs, heads, layout, scale).view(x.shape)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once
     def backward(ctx, gy):
         positions, freqs = ctx.saved_tensors
         heads, layout, scale = ctx.meta
@@ -1045,22 +1056,18 @@ class _DecayAttnFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, qkv, log_decay, key_valid, seq_range, row_base, batch, seq_len, scale):
         x = _head_mat(qkv)
-        D = x.shape[1] // 3
-        o = K.decay_attn_fwd(x[:, :D], x[:, D:2 * D], x[:, 2 * D:], log_decay, batch, seq_len, scale, key_valid,
-                             seq_range, row_base)
+        o = K.decay_attn_packed_fwd(x, log_decay, batch, seq_len, scale, key_valid, seq_range, row_base)
         ctx.save_for_backward(x, log_decay, key_valid, seq_range, row_base)
         ctx.meta = (batch, seq_len, scale, qkv.shape)
-        return o.view(*qkv.shape[:-1], D)
+        return o.view(*qkv.shape[:-1], o.shape[1])
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once
     def backward(ctx, go):
         x, log_decay, key_valid, seq_range, row_base = ctx.saved_tensors
         batch, seq_len, scale, shape = ctx.meta
-        D = x.shape[1] // 3
-        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        K.decay_attn_bwd(_head_mat(go, x.dtype), x[:, :D], x[:, D:2 * D], x[:, 2 * D:], log_decay, batch, seq_len,
-                         scale, key_valid, seq_range, row_base, dx[:, :D], dx[:, D:2 * D], dx[:, 2 * D:])
+        dx = K.decay_attn_packed_bwd(_head_mat(go, x.dtype), x, log_decay, batch, seq_len, scale, key_valid,
+                                     seq_range, row_base)
         return dx.view(shape), None, None, None, None, None, None, None
 
 
@@ -1077,13 +1084,16 @@ def decay_attn(qkv, log_decay, batch, seq_len, scale=None, key_valid=None, seq_r
                               None if scale is None else float(scale))
 
 
+def _fp32_vec(t):
+    return t if t is None or (t.dtype == torch.float32 and t.is_contiguous()) else t.float().contiguous()
+
+
 class _HeadNormFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, gate, heads, eps):
         x2 = _head_mat(x)
         g2 = _head_mat(gate, x.dtype) if gate is not None else None
-        w32 = weight.detach().float().contiguous() if weight is not None else None
-        b32 = bias.detach().float().contiguous() if bias is not None else None
+        w32, b32 = _fp32_vec(weight), _fp32_vec(bias)
         y = K.head_norm_fwd(x2, w32, b32, heads, eps, g2)
         ctx.save_for_backward(x2, w32, b32, g2)
         ctx.meta = (heads, eps, x.shape, None if gate is None else gate.dtype,
@@ -1091,13 +1101,19 @@ class _HeadNormFn(torch.autograd.Function):
         return y.view(x.shape)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once
     def backward(ctx, gy):
         x2, w32, b32, g2 = ctx.saved_tensors
         heads, eps, shape, gdt, wdt, bdt = ctx.meta
         dx, dg, dw, db = K.head_norm_bwd(_head_mat(gy, x2.dtype), x2, w32, b32, heads, eps, g2)
-        return (dx.view(shape), dw.to(wdt) if dw is not None else None, db.to(bdt) if db is not None else None,
-                dg.view(shape).to(gdt) if dg is not None else None, None, None)
+        if dw is not None and wdt != torch.float32:
+            dw = dw.to(wdt)
+        if db is not None and bdt != torch.float32:
+            db = db.to(bdt)
+        if dg is not None:
+            dg = dg.view(shape)
+            dg = dg if dg.dtype == gdt else dg.to(gdt)
+        return dx.view(shape), dw, db, dg, None, None
 
 
 @_disable

@@ -1145,31 +1145,46 @@ def emb_combine_bwd(gy, a, b, scale, relu=True, dropout_p=0.0, seed=0, want=(Tru
 
 
 # -------------------------------------------------------------- decay block
-_ROW_DTYPES = (torch.float32, torch.bfloat16, torch.float16)
+# An eager training step runs these wrappers on two threads in turn (autograd's backward
+# has its own) with cold caches: what they check costs more than the launch, so each
+# operand is looked at once and a refusal is worded only after it has failed.
+_ROW_DTYPES = {torch.float32: L.GRK_F32, torch.bfloat16: L.GRK_BF16, torch.float16: L.GRK_F16}
 _NO_DEVICE = contextlib.nullcontext()
 
 
-def _on_device(t):
-    """The tensor's device as the current one for a launch (no cost where it is already)."""
-    return _NO_DEVICE if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+def _on_device(index):
+    """That device as the current one for a launch (no cost where it is already)."""
+    return _NO_DEVICE if index == torch.cuda.current_device() else torch.cuda.device(index)
 
 
 def _same_device(ref, *ts):
-    _require_cuda(ref, *ts)
+    """The device index that all operands share."""
+    dev = ref.device
+    if dev.type != 'cuda':
+        raise L.GrkError('grk kernels need device (HIP) tensors; there is no CPU path')
     for t in ts:
-        if t is not None and t.device != ref.device:
-            raise L.GrkError(f'all operands must be on one device ({ref.device} and {t.device})')
+        if t is not None and t.device != dev:
+            raise L.GrkError(f'all operands must be on one device ({dev} and {t.device})')
+    return dev.index
 
 
 def _head_rows(t, name, rows, cols, dtype):
     """(pointer, row stride) of a [rows, cols] row-major operand (a column view is fine)."""
-    if t.dtype != dtype or t.dtype not in _ROW_DTYPES:
-        raise L.GrkError(f'{name}: dtype {t.dtype}; the row operands share one of float32, bfloat16, float16')
-    if t.dim() != 2 or t.shape[0] != rows or t.shape[1] != cols:
-        raise L.GrkError(f'{name}: shape {tuple(t.shape)}, expected ({rows}, {cols})')
-    if rows and ((cols > 1 and t.stride(1) != 1) or (rows > 1 and t.stride(0) < cols)):
+    if t.dtype == dtype and t.shape == (rows, cols):
+        ld, one = t.stride()
+        if (one == 1 or cols <= 1 or rows == 0) and (ld >= cols or rows <= 1):
+            return t.data_ptr(), ld
         raise L.GrkError(f'{name}: rows must be dense, with a row stride of at least {cols} elements')
-    return t.data_ptr(), t.stride(0)
+    if t.dtype != dtype:
+        raise L.GrkError(f'{name}: dtype {t.dtype}, expected {dtype}')
+    raise L.GrkError(f'{name}: shape {tuple(t.shape)}, expected ({rows}, {cols})')
+
+
+def _row_code(dtype):
+    code = _ROW_DTYPES.get(dtype)
+    if code is None:
+        raise L.GrkError(f'dtype {dtype}: rows are float32, bfloat16 or float16')
+    return code
 
 
 def _overlap(a, b):
@@ -1248,7 +1263,7 @@ def rotary(x, positions, freqs, heads, layout='half', scale=1.0, inverse=False, 
     positions int32 / int64 [N]; freqs float64 [r] (rotary_frequencies); layout 'half'
     (columns i, i + r) or 'interleaved' (2 i, 2 i + 1).  inverse turns back.  out: x itself
     (in place) or a matrix that shares nothing with it; a new one by default."""
-    _same_device(x, positions, freqs, out)
+    dev = _same_device(x, positions, freqs, out)
     N, cols = x.shape if x.dim() == 2 else (-1, -1)
     if x.dim() != 2 or heads <= 0 or cols % heads or cols == 0:
         raise L.GrkError('x must be [N, heads * head_dim]')
@@ -1258,30 +1273,32 @@ def rotary(x, positions, freqs, heads, layout='half', scale=1.0, inverse=False, 
         raise L.GrkError('positions must be a contiguous int32 / int64 [N] tensor')
     if freqs.dtype != torch.float64 or freqs.dim() != 1 or not freqs.is_contiguous():
         raise L.GrkError('freqs must be a contiguous float64 [rotary_dim / 2] tensor')
-    xp, xl = _head_rows(x, 'x', N, cols, x.dtype)
+    dt = x.dtype
+    code = _row_code(dt)
+    xp, xl = _head_rows(x, 'x', N, cols, dt)
     if out is None:
-        out = torch.empty(N, cols, dtype=x.dtype, device=x.device)
-    elif out.data_ptr() != x.data_ptr() or out.stride(0) != x.stride(0):
-        _fresh(out, 'out', x)
-    op, ol = _head_rows(out, 'out', N, cols, x.dtype)
-    with _on_device(x):
-        rc = L.lib().grk_rotary(xp, xl, op, ol, L.dtype_code(x.dtype), positions.data_ptr(),
-                                L.itype_code(positions.dtype), freqs.data_ptr(), N, heads, cols // heads,
-                                2 * freqs.shape[0], int(layout == 'interleaved'), float(scale), int(bool(inverse)),
-                                L.stream_ptr(x.device))
+        out = torch.empty((N, cols), dtype=dt, device=x.device)
+        op, ol = out.data_ptr(), cols
+    else:
+        op, ol = _head_rows(out, 'out', N, cols, dt)
+        if op != xp or ol != xl:
+            _fresh(out, 'out', x)
+    with _on_device(dev):
+        rc = L.lib().grk_rotary(xp, xl, op, ol, code, positions.data_ptr(), L.itype_code(positions.dtype),
+                                freqs.data_ptr(), N, heads, cols // heads, 2 * freqs.shape[0],
+                                layout == 'interleaved', scale, bool(inverse), L.raw_stream(dev))
     L.check(rc, 'grk_rotary')
     return out
 
 
-def _decay_args(q, k, v, log_decay, batch, seq_len, scale, key_valid, seq_range, row_base):
-    _same_device(q, k, v, log_decay, key_valid, seq_range, row_base)
+def _decay_layout(log_decay, rows, cols, batch, seq_len, key_valid, seq_range, row_base):
+    """Checks what the sequences are made of; (batch, seq_len, heads, head_dim)."""
     if log_decay.dtype != torch.float32 or log_decay.dim() != 1 or not log_decay.is_contiguous() \
             or not log_decay.shape[0]:
         raise L.GrkError('log_decay must be a contiguous float32 [heads] tensor')
     H = log_decay.shape[0]
-    if q.dim() != 2 or q.shape[1] % H or not q.shape[1]:
+    if cols % H or not cols:
         raise L.GrkError('q must be [rows, heads * head_dim]')
-    rows, cols = q.shape
     B, T = int(batch), int(seq_len)
     if B < 0 or T < 0 or (row_base is None and rows != B * T):
         raise L.GrkError(f'{rows} rows do not hold {B} sequences of {T}')
@@ -1294,17 +1311,78 @@ def _decay_args(q, k, v, log_decay, batch, seq_len, scale, key_valid, seq_range,
     if row_base is not None and (seq_range is None or row_base.dtype != torch.int64 or row_base.shape != (B + 1,)
                                  or not row_base.is_contiguous()):
         raise L.GrkError('row_base must be a contiguous int64 [B + 1] tensor, with seq_range (jagged_layout)')
-    hd = cols // H
-    (qp, ql), (kp, kl), (vp, vl) = [_head_rows(t, n, rows, cols, q.dtype) for t, n in ((q, 'q'), (k, 'k'), (v, 'v'))]
-    scale = hd ** -0.5 if scale is None else float(scale)
-    return L.GrkDecayArgs(B, H, T, hd, L.dtype_code(q.dtype), scale, qp, kp, vp, ql, kl, vl, log_decay.data_ptr(),
-                          _ptr(key_valid), _ptr(seq_range), _ptr(row_base),
-                          None if row_base is None else row_base.data_ptr() + 8 * B, rows)
+    return B, T, H, cols // H
+
+
+def _decay_struct(layout, code, scale, q, k, v, log_decay, key_valid, seq_range, row_base, rows):
+    """grk_decay_args of (pointer, row stride) operands."""
+    B, T, H, hd = layout
+    base = None if row_base is None else row_base.data_ptr()
+    return L.GrkDecayArgs(B, H, T, hd, code, hd ** -0.5 if scale is None else scale, q[0], k[0], v[0], q[1], k[1],
+                          v[1], log_decay.data_ptr(), _ptr(key_valid), _ptr(seq_range), base,
+                          None if base is None else base + 8 * B, rows)
+
+
+def _decay_args(q, k, v, log_decay, batch, seq_len, scale, key_valid, seq_range, row_base):
+    _same_device(q, k, v, log_decay, key_valid, seq_range, row_base)
+    if q.dim() != 2:
+        raise L.GrkError('q must be [rows, heads * head_dim]')
+    rows, cols = q.shape
+    dt = q.dtype
+    code = _row_code(dt)
+    layout = _decay_layout(log_decay, rows, cols, batch, seq_len, key_valid, seq_range, row_base)
+    return _decay_struct(layout, code, scale, *[_head_rows(t, n, rows, cols, dt) for t, n in
+                                                ((q, 'q'), (k, 'k'), (v, 'v'))], log_decay, key_valid, seq_range,
+                         row_base, rows)
 
 
 def _decay_workspace(args, backward, device):
-    n = L.lib().grk_decay_attn_workspace(args, int(backward))
+    n = L.lib().grk_decay_attn_workspace(args, backward)
     return (torch.empty(n, dtype=torch.uint8, device=device) if n else None), n
+
+
+def decay_attn_packed_fwd(qkv, log_decay, batch, seq_len, scale=None, key_valid=None, seq_range=None, row_base=None):
+    """decay_attn_fwd of the rows q | k | v side by side, [rows, 3 * heads * head_dim]."""
+    dev = _same_device(qkv, log_decay, key_valid, seq_range, row_base)
+    rows, cols = qkv.shape if qkv.dim() == 2 else (-1, -1)
+    if cols < 0 or cols % 3:
+        raise L.GrkError('qkv must hold q | k | v side by side: [rows, 3 * heads * head_dim]')
+    dt, D = qkv.dtype, cols // 3
+    layout = _decay_layout(log_decay, rows, D, batch, seq_len, key_valid, seq_range, row_base)
+    x, ld = _head_rows(qkv, 'qkv', rows, cols, dt)
+    a = _decay_struct(layout, _row_code(dt), scale, *_thirds(x, ld, D, dt), log_decay, key_valid, seq_range, row_base,
+                      rows)
+    out = torch.empty((rows, D), dtype=dt, device=qkv.device)
+    with _on_device(dev):
+        ws, n = _decay_workspace(a, 0, qkv.device)
+        rc = L.lib().grk_decay_attn_fwd(a, None, None, out.data_ptr(), D, _ptr(ws), n, L.raw_stream(dev))
+    L.check(rc, 'grk_decay_attn_fwd')
+    return out
+
+
+def decay_attn_packed_bwd(dout, qkv, log_decay, batch, seq_len, scale=None, key_valid=None, seq_range=None,
+                          row_base=None):
+    """Gradient of decay_attn_packed_fwd: dq | dk | dv side by side."""
+    dev = _same_device(qkv, dout, log_decay, key_valid, seq_range, row_base)
+    rows, cols = qkv.shape
+    dt, D = qkv.dtype, cols // 3
+    layout = _decay_layout(log_decay, rows, D, batch, seq_len, key_valid, seq_range, row_base)
+    x, ld = _head_rows(qkv, 'qkv', rows, cols, dt)
+    a = _decay_struct(layout, _row_code(dt), scale, *_thirds(x, ld, D, dt), log_decay, key_valid, seq_range, row_base,
+                      rows)
+    gp, gl = _head_rows(dout, 'dout', rows, D, dt)
+    dx = torch.empty((rows, cols), dtype=dt, device=qkv.device)
+    (p0, _), (p1, _), (p2, _) = _thirds(dx.data_ptr(), cols, D, dt)
+    with _on_device(dev):
+        ws, n = _decay_workspace(a, 1, qkv.device)
+        rc = L.lib().grk_decay_attn_bwd(a, gp, gl, p0, cols, p1, cols, p2, cols, _ptr(ws), n, L.raw_stream(dev))
+    L.check(rc, 'grk_decay_attn_bwd')
+    return dx
+
+
+def _thirds(ptr, ld, cols, dtype):
+    step = cols * dtype.itemsize
+    return (ptr, ld), (ptr + step, ld), (ptr + 2 * step, ld)
 
 
 def _state_ok(t, name, shape):
@@ -1325,7 +1403,7 @@ def decay_attn_fwd(q, k, v, log_decay, batch, seq_len, scale=None, key_valid=Non
     state: the states before the first position, fp32 [B, heads, head_dim, head_dim];
     return_state: also those behind the last one (into state_out, which may be state)."""
     a = _decay_args(q, k, v, log_decay, batch, seq_len, scale, key_valid, seq_range, row_base)
-    _same_device(q, state, state_out, out)
+    dev = _same_device(q, state, state_out, out)
     shape = (a.batch, a.heads, a.head_dim, a.head_dim)
     if state is not None:
         _state_ok(state, 'state', shape)
@@ -1338,9 +1416,9 @@ def decay_attn_fwd(q, k, v, log_decay, batch, seq_len, scale=None, key_valid=Non
     else:
         _fresh(out, 'out', q, k, v)
     op, ol = _head_rows(out, 'out', q.shape[0], q.shape[1], q.dtype)
-    with _on_device(q):
-        ws, n = _decay_workspace(a, False, q.device)
-        rc = L.lib().grk_decay_attn_fwd(a, _ptr(state), _ptr(state_out), op, ol, _ptr(ws), n, L.stream_ptr(q.device))
+    with _on_device(dev):
+        ws, n = _decay_workspace(a, 0, q.device)
+        rc = L.lib().grk_decay_attn_fwd(a, _ptr(state), _ptr(state_out), op, ol, _ptr(ws), n, L.raw_stream(dev))
     L.check(rc, 'grk_decay_attn_fwd')
     return (out, state_out) if return_state else out
 
@@ -1350,7 +1428,7 @@ def decay_attn_bwd(dout, q, k, v, log_decay, batch, seq_len, scale=None, key_val
     """Gradients (dq, dk, dv) of decay_attn_fwd without states (grk_decay_attn_bwd);
     log_decay gets none.  dq / dk / dv: matrices to write (column views are fine)."""
     a = _decay_args(q, k, v, log_decay, batch, seq_len, scale, key_valid, seq_range, row_base)
-    _same_device(q, dout, dq, dk, dv)
+    dev = _same_device(q, dout, dq, dk, dv)
     rows, cols = q.shape
     gp, gl = _head_rows(dout, 'dout', rows, cols, q.dtype)
     grads = [torch.empty(rows, cols, dtype=q.dtype, device=q.device) if t is None else t for t in (dq, dk, dv)]
@@ -1358,9 +1436,9 @@ def decay_attn_bwd(dout, q, k, v, log_decay, batch, seq_len, scale=None, key_val
     for i, t in enumerate(grads):
         _fresh(t, ('dq', 'dk', 'dv')[i], dout, q, k, v, *grads[:i])
     (p0, l0), (p1, l1), (p2, l2) = ptrs
-    with _on_device(q):
-        ws, n = _decay_workspace(a, True, q.device)
-        rc = L.lib().grk_decay_attn_bwd(a, gp, gl, p0, l0, p1, l1, p2, l2, _ptr(ws), n, L.stream_ptr(q.device))
+    with _on_device(dev):
+        ws, n = _decay_workspace(a, 1, q.device)
+        rc = L.lib().grk_decay_attn_bwd(a, gp, gl, p0, l0, p1, l1, p2, l2, _ptr(ws), n, L.raw_stream(dev))
     L.check(rc, 'grk_decay_attn_bwd')
     return tuple(grads)
 
@@ -1373,7 +1451,7 @@ def decay_attn_step(q, k, v, log_decay, state, slots=None, scale=None, err_flag=
     takes state i).  Events of one slot are taken in the order of their index.  A negative
     slot holds no event (output row zero), one past the states as well, and sets err_flag
     (int32 [1])."""
-    _same_device(q, k, v, log_decay, state, slots, err_flag, out)
+    dev = _same_device(q, k, v, log_decay, state, slots, err_flag, out)
     if log_decay.dtype != torch.float32 or log_decay.dim() != 1 or not log_decay.is_contiguous() \
             or not log_decay.shape[0]:
         raise L.GrkError('log_decay must be a contiguous float32 [heads] tensor')
@@ -1390,26 +1468,27 @@ def decay_attn_step(q, k, v, log_decay, state, slots=None, scale=None, err_flag=
         raise L.GrkError('slots must be a contiguous int32 / int64 [n] tensor')
     if err_flag is not None and (err_flag.dtype != torch.int32 or err_flag.numel() < 1):
         raise L.GrkError('err_flag must be an int32 [1] tensor')
-    (qp, ql), (kp, kl), (vp, vl) = [_head_rows(t, m, n, cols, q.dtype) for t, m in ((q, 'q'), (k, 'k'), (v, 'v'))]
+    dt = q.dtype
+    code = _row_code(dt)
+    (qp, ql), (kp, kl), (vp, vl) = [_head_rows(t, m, n, cols, dt) for t, m in ((q, 'q'), (k, 'k'), (v, 'v'))]
     if out is None:
-        out = torch.empty(n, cols, dtype=q.dtype, device=q.device)
+        out = torch.empty((n, cols), dtype=dt, device=q.device)
     else:
         _fresh(out, 'out', q, k, v)
-    op, ol = _head_rows(out, 'out', n, cols, q.dtype)
-    with _on_device(q):
-        nb = L.lib().grk_decay_attn_step_workspace(n, int(slots is not None))
+    op, ol = _head_rows(out, 'out', n, cols, dt)
+    lib = L.lib()
+    with _on_device(dev):
+        nb = lib.grk_decay_attn_step_workspace(n, slots is not None)
         ws = torch.empty(nb, dtype=torch.uint8, device=q.device) if nb else None
-        rc = L.lib().grk_decay_attn_step(qp, ql, kp, kl, vp, vl, L.dtype_code(q.dtype), log_decay.data_ptr(), n, H,
-                                         hd, hd ** -0.5 if scale is None else float(scale), state.data_ptr(),
-                                         state.shape[0], _ptr(slots),
-                                         L.itype_code(slots.dtype) if slots is not None else L.GRK_I64,
-                                         _ptr(err_flag), op, ol, _ptr(ws), nb, L.stream_ptr(q.device))
+        rc = lib.grk_decay_attn_step(qp, ql, kp, kl, vp, vl, code, log_decay.data_ptr(), n, H, hd,
+                                     hd ** -0.5 if scale is None else scale, state.data_ptr(), state.shape[0],
+                                     _ptr(slots), L.itype_code(slots.dtype) if slots is not None else L.GRK_I64,
+                                     _ptr(err_flag), op, ol, _ptr(ws), nb, L.raw_stream(dev))
     L.check(rc, 'grk_decay_attn_step')
     return out
 
 
 def _norm_operands(x, weight, bias, heads, gate):
-    _same_device(x, weight, bias, gate)
     if x.dim() != 2 or heads <= 0 or x.shape[1] % heads or not x.shape[1]:
         raise L.GrkError('x must be [N, heads * head_dim]')
     N, cols = x.shape
@@ -1424,18 +1503,20 @@ def head_norm_fwd(x, weight, bias, heads, eps=1e-5, gate=None, out=None):
     """Layer norm of each head's columns, times SiLU(gate) (grk_head_norm_fwd): x / gate
     [N, heads * head_dim] of one dtype, weight / bias fp32 [heads * head_dim] or None,
     head_dim <= 2048; heads=1 is the layer norm of a row.  out may be x or gate."""
+    dev = _same_device(x, weight, bias, gate, out)
     xp, xl, gp, gl = _norm_operands(x, weight, bias, heads, gate)
     N, cols = x.shape
-    _same_device(x, out)
+    dt = x.dtype
+    code = _row_code(dt)
     if out is None:
-        out = torch.empty(N, cols, dtype=x.dtype, device=x.device)
+        out = torch.empty((N, cols), dtype=dt, device=x.device)
+        op, ol = out.data_ptr(), cols
     else:
-        _fresh(out, 'out', *[t for t in (x, gate) if t is not None and not (
-            t.data_ptr() == out.data_ptr() and t.stride(0) == out.stride(0))])
-    op, ol = _head_rows(out, 'out', N, cols, x.dtype)
-    with _on_device(x):
-        rc = L.lib().grk_head_norm_fwd(xp, xl, gp, gl, _ptr(weight), _ptr(bias), float(eps), N, heads, cols // heads,
-                                       L.dtype_code(x.dtype), op, ol, L.stream_ptr(x.device))
+        op, ol = _head_rows(out, 'out', N, cols, dt)
+        _fresh(out, 'out', *[t for t, p, ld in ((x, xp, xl), (gate, gp, gl)) if t is not None and (p, ld) != (op, ol)])
+    with _on_device(dev):
+        rc = L.lib().grk_head_norm_fwd(xp, xl, gp, gl, _ptr(weight), _ptr(bias), eps, N, heads, cols // heads, code,
+                                       op, ol, L.raw_stream(dev))
     L.check(rc, 'grk_head_norm_fwd')
     return out
 
@@ -1443,29 +1524,33 @@ def head_norm_fwd(x, weight, bias, heads, eps=1e-5, gate=None, out=None):
 def head_norm_bwd(dy, x, weight, bias, heads, eps=1e-5, gate=None, dx=None, dgate=None):
     """Gradients of head_norm_fwd: (dx, dgate or None, dweight or None, dbias or None);
     dweight / dbias fp32, in a fixed order of addition."""
+    device = x.device
+    dev = _same_device(x, dy, weight, bias, gate, dx, dgate)
     xp, xl, gp, gl = _norm_operands(x, weight, bias, heads, gate)
-    _same_device(x, dy, dx, dgate)
     N, cols = x.shape
-    dev, dt = x.device, x.dtype
+    dt = x.dtype
+    code = _row_code(dt)
     yp, yl = _head_rows(dy, 'dy', N, cols, dt)
-    dx = torch.empty(N, cols, dtype=dt, device=dev) if dx is None else dx
+    if dx is None:
+        dx = torch.empty((N, cols), dtype=dt, device=device)
+    else:
+        _fresh(dx, 'dx', dy, x, gate)
     if gate is None:
         dgate = None
     elif dgate is None:
-        dgate = torch.empty(N, cols, dtype=dt, device=dev)
-    dw = torch.empty(cols, dtype=torch.float32, device=dev) if weight is not None else None
-    db = torch.empty(cols, dtype=torch.float32, device=dev) if bias is not None else None
+        dgate = torch.empty((N, cols), dtype=dt, device=device)
+    else:
+        _fresh(dgate, 'dgate', dy, x, gate, dx)
+    dw = torch.empty(cols, dtype=torch.float32, device=device) if weight is not None else None
+    db = torch.empty(cols, dtype=torch.float32, device=device) if bias is not None else None
     dxp, dxl = _head_rows(dx, 'dx', N, cols, dt)
     dgp, dgl = _head_rows(dgate, 'dgate', N, cols, dt) if dgate is not None else (None, 0)
-    _fresh(dx, 'dx', dy, x, gate)
-    if dgate is not None:
-        _fresh(dgate, 'dgate', dy, x, gate, dx)
-    with _on_device(x):
-        nb = L.lib().grk_head_norm_bwd_workspace(N, heads, cols // heads) if dw is not None or db is not None else 0
-        ws = torch.empty(nb, dtype=torch.uint8, device=dev) if nb else None
-        rc = L.lib().grk_head_norm_bwd(yp, yl, xp, xl, gp, gl, _ptr(weight), _ptr(bias), float(eps), N, heads,
-                                       cols // heads, L.dtype_code(dt), dxp, dxl, dgp, dgl, _ptr(dw), _ptr(db),
-                                       _ptr(ws), nb, L.stream_ptr(dev))
+    lib = L.lib()
+    with _on_device(dev):
+        nb = lib.grk_head_norm_bwd_workspace(N, heads, cols // heads) if dw is not None or db is not None else 0
+        ws = torch.empty(nb, dtype=torch.uint8, device=device) if nb else None
+        rc = lib.grk_head_norm_bwd(yp, yl, xp, xl, gp, gl, _ptr(weight), _ptr(bias), eps, N, heads, cols // heads,
+                                   code, dxp, dxl, dgp, dgl, _ptr(dw), _ptr(db), _ptr(ws), nb, L.raw_stream(dev))
     L.check(rc, 'grk_head_norm_bwd')
     return dx, dgate, dw, db
 
