@@ -1126,6 +1126,86 @@ def head_norm(x, weight, bias, heads, eps=1e-5, gate=None):
     return _HeadNormFn.apply(x, weight, bias, gate, int(heads), float(eps))
 
 
+class _RotaryQKFn(torch.autograd.Function):
+    @staticmethod
+    def _turn(x, positions, freqs, heads, layout, scale, inverse):
+        n = x.shape[1] // 3 * 2
+        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        K.rotary(x[:, :n], positions, freqs, 2 * heads, layout, scale, inverse, out=out[:, :n])
+        out[:, n:].copy_(x[:, n:])
+        return out
+
+    @staticmethod
+    def forward(ctx, qkv, positions, freqs, heads, layout, scale):
+        ctx.save_for_backward(positions, freqs)
+        ctx.meta = (heads, layout, scale)
+        return _RotaryQKFn._turn(_head_mat(qkv), positions, freqs, heads, layout, scale, False).view(qkv.shape)
+
+    @staticmethod
+    @_once
+    def backward(ctx, g):
+        return (_RotaryQKFn._turn(_head_mat(g), *ctx.saved_tensors, *ctx.meta, True).view(g.shape),
+                None, None, None, None, None)
+
+
+@_disable
+def rotary_qk(qkv, positions, freqs, heads, layout='half', scale=1.0):
+    """q | k | v rows [..., 3 * heads * head_dim] with q and k turned by their positions
+    (kernels.rotary) and v as it is."""
+    return _RotaryQKFn.apply(qkv, positions, freqs, int(heads), layout, float(scale))
+
+
+class _DecayCoreFn(torch.autograd.Function):
+    """The decay block between its projections, on the [N, 4 D] (u | v | q | k) rows: q and k
+    turned, attention, norm of each head times SiLU(u).  The gradients of u, v, q and k are
+    written side by side; q and k's are turned back where they lie."""
+
+    @staticmethod
+    def forward(ctx, pre, log_decay, w, b, eps, rot, layout):
+        positions, freqs, style, scale = rot if rot is not None else (None, None, None, None)
+        batch, seq_len, key_valid, seq_range, row_base = layout
+        x = _head_mat(pre)
+        D = x.shape[1] // 4
+        H = log_decay.shape[0]
+        qk = x[:, 2 * D:]
+        if rot is not None:
+            qk = K.rotary(qk, positions, freqs, 2 * H, style, scale)
+        o = K.decay_attn_fwd(qk[:, :D], qk[:, D:], x[:, D:2 * D], log_decay, batch, seq_len, None, key_valid,
+                             seq_range, row_base)
+        w32, b32 = _fp32_vec(w), _fp32_vec(b)
+        y = K.head_norm_fwd(o, w32, b32, H, eps, gate=x[:, :D])
+        ctx.save_for_backward(x, qk if rot is not None else None, o, log_decay, w32, b32, positions, freqs, key_valid,
+                              seq_range, row_base)
+        ctx.meta = (eps, style, scale, batch, seq_len, w.dtype, b.dtype, pre.shape)
+        return y
+
+    @staticmethod
+    @_once
+    def backward(ctx, gy):
+        x, qk, o, log_decay, w32, b32, positions, freqs, key_valid, seq_range, row_base = ctx.saved_tensors
+        eps, style, scale, batch, seq_len, wdt, bdt, shape = ctx.meta
+        D = x.shape[1] // 4
+        H = log_decay.shape[0]
+        qk = x[:, 2 * D:] if qk is None else qk
+        dx = torch.empty((x.shape[0], 4 * D), dtype=x.dtype, device=x.device)
+        do, _, dw, db = K.head_norm_bwd(_head_mat(gy, x.dtype), o, w32, b32, H, eps, gate=x[:, :D], dgate=dx[:, :D])
+        K.decay_attn_bwd(do, qk[:, :D], qk[:, D:], x[:, D:2 * D], log_decay, batch, seq_len, None, key_valid,
+                         seq_range, row_base, dx[:, 2 * D:3 * D], dx[:, 3 * D:], dx[:, D:2 * D])
+        if positions is not None:
+            K.rotary(dx[:, 2 * D:], positions, freqs, 2 * H, style, scale, inverse=True, out=dx[:, 2 * D:])
+        return dx.view(shape), None, dw.to(wdt), db.to(bdt), None, None, None
+
+
+@_disable
+def decay_core(pre, log_decay, weight, bias, batch, seq_len, key_valid=None, seq_range=None, row_base=None, eps=1e-5,
+               rot=None):
+    """norm(decay_attn(rotary(q), rotary(k), v)) * SiLU(u) of [N, 4 D] (u | v | q | k) rows,
+    [N, D] out: the decay block between its projections.  rot: (positions [N], freqs,
+    layout, scale) of kernels.rotary, or None."""
+    return _DecayCoreFn.apply(pre, log_decay, weight, bias, float(eps), rot,
+                              (int(batch), int(seq_len), key_valid, seq_range, row_base))
+
+
 # ---------------------------------------------------------------- logits ----
 def _rows2d(x):
     x = x.reshape(-1, x.shape[-1])

@@ -7,12 +7,17 @@ seq_feature, pos_feature, neg_feature) -> (pos_logits, neg_logits)``,
 ``predict``, ``save_item_emb``, the sub-module contract
 ``attention_layers[i](q, k, v, attn_mask=[B,T,T]) -> (out, None)`` and every
 state_dict key (``model/BaseLine/model.py:81-433``,
-``model/BaseLineO1/model.py:167-555``).  ``args`` may carry three optional
+``model/BaseLineO1/model.py:167-555``).  ``args`` may carry optional
 fields the reference does not have:
 
 * ``variant``: "baseline" (Conv1d FFN, default) | "o1" (PackedSwiGLUFFN);
 * ``block``:   "softmax" (reference attention, default) | "hstu" (north-star
-  HSTU layer; no FFN, pre-norm residual);
+  HSTU layer; no FFN, pre-norm residual) | "decay" (linear attention with a
+  decay for each head; no FFN, pre-norm residual);
+* ``rotary``:  True, or a dict (class Rotary): positions by rotation of q and k
+  (softmax and decay blocks) instead of the position table;
+* ``decay_windows``: the shortest and the longest head's window in events
+  (decay block; default (8, 256));
 * ``hstu_num_buckets``: relative-position buckets (default maxlen + 1).
 
 Device work: all table lookups of a feat2emb call are ONE fused gather
@@ -37,6 +42,30 @@ from . import kernels as K
 from .dataset import MM_SHAPE, save_emb, tensorize
 
 
+class Rotary:
+    """What ``args.rotary`` says: True (all of the head in the half layout, base 10000), or
+    a dict of ``dim`` (rotated columns of a head), ``base``, ``layout`` ('half' |
+    'interleaved') and ``scaling`` (kernels.rotary_frequencies)."""
+
+    def __init__(self, spec, head_dim):
+        spec = {} if spec is True else dict(spec)
+        self.layout = spec.pop('layout', 'half')
+        dim = int(spec.pop('dim', head_dim // 2 * 2))
+        if not 2 <= dim <= head_dim or self.layout not in ('half', 'interleaved'):
+            raise ValueError(f'rotary: dim {dim} of a head of {head_dim}, layout {self.layout!r}')
+        self._freqs, self.scale = K.rotary_frequencies(dim, spec.pop('base', 10000.0), spec.pop('scaling', None))
+        if spec:
+            raise ValueError(f'rotary: unknown {sorted(spec)}')
+        self._on = {}   # device -> float64 frequencies (no buffer: a module's casts leave them 64 bits)
+
+    def at(self, positions):
+        """(positions, freqs, layout, scale) on the positions' device."""
+        dev = positions.device
+        if dev not in self._on:
+            self._on[dev] = self._freqs.to(dev)
+        return positions, self._on[dev], self.layout, self.scale
+
+
 class FlashMultiHeadAttention(torch.nn.Module):
     """Softmax MHA (model/BaseLine/model.py:10-62) on grk_attention_fwd/bwd.
 
@@ -45,20 +74,23 @@ class FlashMultiHeadAttention(torch.nn.Module):
     directly, with the mask given as causal + per-key validity instead of a
     materialised [B,T,T] tensor."""
 
-    def __init__(self, hidden_units, num_heads, dropout_rate):
+    def __init__(self, hidden_units, num_heads, dropout_rate, rotary=None):
         super().__init__()
         assert hidden_units % num_heads == 0, 'hidden_units must be divisible by num_heads'
         self.hidden_units, self.num_heads = hidden_units, num_heads
         self.head_dim = hidden_units // num_heads
+        self.rotary = Rotary(rotary, self.head_dim) if rotary else None
         self.dropout_rate = dropout_rate
         self.q_linear = torch.nn.Linear(hidden_units, hidden_units)
         self.k_linear = torch.nn.Linear(hidden_units, hidden_units)
         self.v_linear = torch.nn.Linear(hidden_units, hidden_units)
         self.out_linear = torch.nn.Linear(hidden_units, hidden_units)
 
-    def forward(self, query, key, value, attn_mask=None, key_valid=None, seq_range=None, row_base=None):
+    def forward(self, query, key, value, attn_mask=None, key_valid=None, seq_range=None, row_base=None,
+                positions=None):
         """row_base (with key_valid [B, T] and seq_range): query / key / value hold the
-        jagged rows of the batch (jagged.py) as [1, rows, D]."""
+        jagged rows of the batch (jagged.py) as [1, rows, D].  positions (rotary): one per
+        row; those of a [B, T] batch by default."""
         B, T, D = query.shape
         if row_base is not None:
             B, T = key_valid.shape
@@ -71,6 +103,9 @@ class FlashMultiHeadAttention(torch.nn.Module):
             qkv = _linear(query, w, b)
         else:
             qkv = torch.cat([self.q_linear(query), self.k_linear(key), self.v_linear(value)], -1)
+        if self.rotary is not None:
+            rot = self.rotary.at(_row_positions(B, T, qkv.device) if positions is None else positions)
+            qkv = G.rotary_qk(qkv, *rot[:2], self.num_heads, *rot[2:])
         p = self.dropout_rate if self.training else 0.0
         seed = dropout_seed(qkv.device) if p > 0 else 0
         o = G.softmax_mha(qkv.reshape(N, 3 * D), key_valid, B, T, self.num_heads, self.head_dim, p, seed,
@@ -132,6 +167,20 @@ def _valid_bytes(token_type):
     dtype view)."""
     kv = (token_type != 0).contiguous()
     return kv.to(torch.uint8) if torch.compiler.is_compiling() else kv.view(torch.uint8)
+
+
+_ROW_POSITIONS = {}
+
+
+def _row_positions(B, T, device):
+    """Cached int32 [B * T]: the position of each row of a [B, T] batch."""
+    key = (int(B), int(T), str(device))
+    p = _ROW_POSITIONS.get(key)
+    if p is None:
+        if len(_ROW_POSITIONS) > 64:
+            _ROW_POSITIONS.clear()
+        p = _ROW_POSITIONS[key] = torch.arange(T, dtype=torch.int32).repeat(B).to(device)
+    return p
 
 
 _UNIT_ROWS = {}
@@ -216,6 +265,124 @@ class HSTUAttention(torch.nn.Module):
         return _linear(y.view(query.shape), self.out_linear.weight, self.out_linear.bias), None
 
 
+class HeadNorm(torch.nn.Module):
+    """Weight and bias of a layer norm over each head's columns (kernels.head_norm_fwd)."""
+
+    def __init__(self, hidden_units, num_heads, eps=1e-5):
+        super().__init__()
+        self.num_heads, self.eps = num_heads, eps
+        self.weight = torch.nn.Parameter(torch.ones(hidden_units))
+        self.bias = torch.nn.Parameter(torch.zeros(hidden_units))
+
+
+class DecayAttention(torch.nn.Module):
+    """Linear attention with a decay for each head (no reference):
+
+        u, v, q, k = split(uvqk(x));  S_t = g S_{t-1} + k_t v_t^T;  o_t = q_t S_t / sqrt(head_dim)
+        y = out_linear(dropout(norm_h(o) * SiLU(u)))
+
+    with q and k turned by their positions (rotary) and each head's columns normalised by
+    themselves (a long window's sums are larger than a short one's).  The decays g are
+    given, not learned: windows 1 / (1 - g) from decay_windows[0] to [1] events, evenly
+    spaced in their logarithm (buffer log_decay).  A sequence's state is all that a next
+    event needs: ``read`` returns it, ``step`` takes single events on it."""
+
+    def __init__(self, hidden_units, num_heads, dropout_rate, windows=(8.0, 256.0), rotary=None):
+        super().__init__()
+        assert hidden_units % num_heads == 0, 'hidden_units must be divisible by num_heads'
+        lo, hi = (float(w) for w in windows)
+        if not 1.0 <= lo <= hi:
+            raise ValueError('decay_windows: 1 <= shortest <= longest')
+        self.hidden_units, self.num_heads = hidden_units, num_heads
+        self.head_dim = hidden_units // num_heads
+        if self.head_dim > 128:
+            raise NotImplementedError('decay attention takes head_dim <= 128')
+        self.dropout_rate = dropout_rate
+        self.rotary = Rotary(rotary, self.head_dim) if rotary else None
+        self.uvqk = torch.nn.Linear(hidden_units, 4 * hidden_units)
+        win = torch.exp(torch.linspace(np.log(lo), np.log(hi), num_heads, dtype=torch.float64))
+        self.register_buffer('log_decay', torch.log1p(-1.0 / win).float())
+        self.attn_norm = HeadNorm(hidden_units, num_heads)
+        self.out_linear = torch.nn.Linear(hidden_units, hidden_units)
+
+    def forward(self, query, key=None, value=None, attn_mask=None, key_valid=None, seq_range=None, row_base=None,
+                positions=None):
+        """row_base (with key_valid [B, T] and seq_range): query holds the jagged rows of
+        the batch (jagged.py) as [1, rows, D].  positions (rotary): one per row; those of a
+        [B, T] batch by default."""
+        B, T, D = query.shape
+        if row_base is not None:
+            B, T = key_valid.shape
+        elif key_valid is None:
+            key_valid = key_valid_from_mask(attn_mask, B, T)
+        pre = _linear(query, self.uvqk.weight, self.uvqk.bias).reshape(-1, 4 * D)
+        rot = None
+        if self.rotary is not None:
+            rot = self.rotary.at(_row_positions(B, T, pre.device) if positions is None else positions)
+        y = G.decay_core(pre, self.log_decay.float(), self.attn_norm.weight, self.attn_norm.bias, B, T, key_valid,
+                         seq_range, row_base, self.attn_norm.eps, rot)
+        if self.training and self.dropout_rate > 0:
+            y = F.dropout(y, self.dropout_rate)
+        return _linear(y.view(query.shape), self.out_linear.weight, self.out_linear.bias), None
+
+    def _serve(self, x, positions, attend):
+        """The layer on [N, D] rows without gradients; attend(q, k, v) is its attention."""
+        D = self.hidden_units
+        pre = _linear(x, self.uvqk.weight, self.uvqk.bias)
+        qk = pre[:, 2 * D:]
+        if self.rotary is not None:
+            rot = self.rotary.at(positions)
+            K.rotary(qk, *rot[:2], 2 * self.num_heads, *rot[2:], out=qk)
+        o = attend(qk[:, :D], qk[:, D:], pre[:, D:2 * D])
+        y = K.head_norm_fwd(o, self.attn_norm.weight.float(), self.attn_norm.bias.float(), self.num_heads,
+                            self.attn_norm.eps, gate=pre[:, :D], out=o)
+        return _linear(y, self.out_linear.weight, self.out_linear.bias)
+
+    def read(self, query, key_valid, seq_range, positions):
+        """(the layer's output [B, T, D], the states behind the last position)."""
+        B, T, D = query.shape
+        lg, state = self.log_decay.float(), []
+
+        def attend(q, k, v):
+            o, s = K.decay_attn_fwd(q, k, v, lg, B, T, None, key_valid, seq_range, return_state=True)
+            state.append(s)
+            return o
+
+        return self._serve(query.reshape(-1, D), positions, attend).view(B, T, D), state[0]
+
+    def step(self, x, positions, state, slots, err_flag=None):
+        """One event of each row's user [n, D] on the states of their slots, in place."""
+        lg = self.log_decay.float()
+        return self._serve(x, positions, lambda q, k, v: K.decay_attn_step(q, k, v, lg, state, slots,
+                                                                           err_flag=err_flag))
+
+
+class DecayStream:
+    """What BaselineModel.stream_begin keeps of its users: of each layer the states
+    (fp32 [slots, heads, head_dim, head_dim]), the position of each user's next event and a
+    device flag set by a slot outside the stream (``check`` reads it)."""
+
+    def __init__(self, states, position):
+        self.states, self.position = states, position
+        self.err = torch.zeros(1, dtype=torch.int32, device=position.device)
+
+    def place(self, slots, other):
+        """The users of another stream (stream_begin's, in its order) into these slots."""
+        for mine, theirs in zip(self.states, other.states):
+            mine[slots] = theirs
+        self.position[slots] = other.position
+
+    def clear(self, slots):
+        """These slots as users without a history."""
+        for s in self.states:
+            s[slots] = 0
+        self.position[slots] = 0
+
+    def check(self):
+        if int(self.err.item()):
+            raise ValueError(f'stream_step: a slot outside the {self.position.numel()} of the stream')
+
+
 class PointWiseFeedForward(torch.nn.Module):
     """Conv1d(k=1)-ReLU FFN (model/BaseLine/model.py:65-78)."""
 
@@ -268,6 +435,9 @@ class BaselineModel(torch.nn.Module):
         self.maxlen = args.maxlen
         self.variant = getattr(args, 'variant', 'baseline')
         self.block = getattr(args, 'block', 'softmax')
+        self.rotary = getattr(args, 'rotary', None) or None
+        if self.rotary and self.block == 'hstu':
+            raise NotImplementedError('rotary positions: the softmax and decay blocks (HSTU layers have their own bias)')
         d = args.hidden_units
         self.hidden_units = d
         # feature tables with more rows than this are looked up directly into the
@@ -314,7 +484,12 @@ class BaselineModel(torch.nn.Module):
                                                            getattr(args, 'hstu_time_buckets', 0) or 0,
                                                            fp8=bool(getattr(args, 'hstu_fp8', False))))
                 continue
-            self.attention_layers.append(FlashMultiHeadAttention(d, args.num_heads, args.dropout_rate))
+            if self.block == 'decay':
+                self.attention_layers.append(DecayAttention(d, args.num_heads, args.dropout_rate,
+                                                            getattr(args, 'decay_windows', None) or (8.0, 256.0),
+                                                            self.rotary))
+                continue
+            self.attention_layers.append(FlashMultiHeadAttention(d, args.num_heads, args.dropout_rate, self.rotary))
             self.forward_layernorms.append(torch.nn.LayerNorm(d, eps=1e-8))
             if self.variant == 'o1':
                 self.forward_layers.append(PackedSwiGLUFFN(d, dropout_rate=args.dropout_rate))
@@ -696,17 +871,20 @@ class BaselineModel(torch.nn.Module):
             y = torch.addmm(p, a, w.t()) if p is not None else a @ w.t()
             return torch.relu(y) if relu else y
 
-        if combine is not None and include_user and with_pos and _grk_gemm_ok(blocks[0]):
+        if combine is not None and include_user and _grk_gemm_ok(blocks[0]):
             # log2feats' first-block input in one pass: the dnn ReLUs, the sum, the
             # sqrt(d) scale, the position rows and the dropout (grk_emb_combine)
             scale, p = combine
             xi = dnn('item', wi, bool(item_p), relu=False)
             xu = dnn('user', wu, bool(user_p), relu=False)
             seed = dropout_seed(dev) if p > 0 else 0
-            return G.emb_combine(xi, xu, blocks.pop(0), scale, True, p, seed).view(B, T, d), None
+            pos = blocks.pop(0) if with_pos else None
+            return G.emb_combine(xi, xu, pos, scale, True, p, seed).view(B, T, d), None
         x = dnn('item', wi, bool(item_p))
         if include_user:
             x = x + dnn('user', wu, bool(user_p))
+        if combine is not None and not with_pos:
+            return self.emb_dropout(x * combine[0]).view(B, T, d), None
         pos_rows = blocks.pop(0) if with_pos else None
         return x.view(B, T, d), pos_rows
 
@@ -774,19 +952,37 @@ class BaselineModel(torch.nn.Module):
         B, T = log_seqs.shape
         scale = self.item_emb.embedding_dim ** 0.5
         p = self.emb_dropout.p if self.training else 0.0
-        seqs, pos_rows = self._embed(log_seqs, seq_feature, mask=mask, include_user=True, with_pos=True,
+        seqs, pos_rows = self._embed(log_seqs, seq_feature, mask=mask, include_user=True, with_pos=not self.rotary,
                                      pos_idx=pos_idx if jagged is not None else None, combine=(scale, p))
         if pos_rows is not None:
             seqs = seqs * scale + pos_rows.view(B, T, -1)
             seqs = self.emb_dropout(seqs)
         if jagged is not None:
             kw = dict(key_valid=jagged.key_valid, seq_range=jagged.seq_range, row_base=jagged.row_base)
+            if self.rotary:
+                kw['positions'] = jagged.row_map % jagged.T   # (the rows behind the last sequence: any)
         else:
             key_valid = _valid_bytes(mask.to(dev, non_blocking=True))
             kw = dict(key_valid=key_valid, seq_range=torch.ops.grk.seq_ranges(key_valid))  # one launch serves every layer
         if timestamps is not None and self.block == 'hstu':
             kw['timestamps'] = timestamps.to(dev, torch.int64, non_blocking=True).contiguous()
-        if self.block == 'hstu' and _grk_gemm_ok(seqs) and self.hidden_units % 8 == 0:
+        if self.block in ('hstu', 'decay'):
+            return self._prenorm_blocks(seqs, lambda i, x: self.attention_layers[i](x, **kw)[0])
+        for i in range(len(self.attention_layers)):
+            if self.norm_first:
+                x = self.attention_layernorms[i](seqs)
+                seqs = seqs + self.attention_layers[i](x, x, x, **kw)[0]
+                seqs = seqs + self.forward_layers[i](self.forward_layernorms[i](seqs))
+            else:
+                y, _ = self.attention_layers[i](seqs, seqs, seqs, **kw)
+                seqs = self.attention_layernorms[i](seqs + y)
+                seqs = self.forward_layernorms[i](seqs + self.forward_layers[i](seqs))
+        return self.last_layernorm(seqs)
+
+    def _prenorm_blocks(self, seqs, layer):
+        """The HSTU / decay block stack: seqs + layer(i, norm_i(seqs)) for each layer, then
+        the last norm."""
+        if _grk_gemm_ok(seqs) and self.hidden_units % 8 == 0:
             # bf16 residual stream: each residual add is fused into the next LayerNorm
             # (grk_add_norm), the last one into last_layernorm (fp32 output, as autocast's)
             y = None
@@ -796,24 +992,87 @@ class BaselineModel(torch.nn.Module):
                     x = G.add_norm(seqs, None, ln.weight, ln.bias, ln.eps)
                 else:
                     seqs, x = G.add_norm(seqs, y, ln.weight, ln.bias, ln.eps)
-                y, _ = self.attention_layers[i](x, **kw)
+                y = layer(i, x)
             ln = self.last_layernorm
             if y is None:
                 return G.add_norm(seqs, None, ln.weight, ln.bias, ln.eps, x_dtype=torch.float32)
             return G.add_norm(seqs, y, ln.weight, ln.bias, ln.eps, x_dtype=torch.float32)[1]
         for i in range(len(self.attention_layers)):
-            if self.block == 'hstu':
-                y, _ = self.attention_layers[i](self.attention_layernorms[i](seqs), **kw)
-                seqs = seqs + y
-            elif self.norm_first:
-                x = self.attention_layernorms[i](seqs)
-                seqs = seqs + self.attention_layers[i](x, x, x, **kw)[0]
-                seqs = seqs + self.forward_layers[i](self.forward_layernorms[i](seqs))
-            else:
-                y, _ = self.attention_layers[i](seqs, seqs, seqs, **kw)
-                seqs = self.attention_layernorms[i](seqs + y)
-                seqs = self.forward_layernorms[i](seqs + self.forward_layers[i](seqs))
+            seqs = seqs + layer(i, self.attention_layernorms[i](seqs))
         return self.last_layernorm(seqs)
+
+    # ------------------------------------------ single events on kept states --
+    def _stream_rows(self, seq, seq_feature, mask):
+        return self._embed(seq, seq_feature, mask=mask, include_user=True, with_pos=False,
+                           combine=(self.item_emb.embedding_dim ** 0.5, 0.0))[0]
+
+    @torch.no_grad()
+    def stream_begin(self, log_seqs, seq_feature, mask, slots=None):
+        """Read B users' events [B, T] (left-padded, as predict takes them) into kept states:
+        (predict's features [B, D], a DecayStream of ``slots`` users, by default B, with
+        these in slots 0 .. B - 1).  A decay model with rotary positions, in eval mode."""
+        if self.block != 'decay' or not self.rotary:
+            raise NotImplementedError('streams need the decay block with rotary positions (a position table ends)')
+        if self.training:
+            raise RuntimeError('stream_begin: call eval() first')
+        dev = self._device()
+        B, T = log_seqs.shape
+        n = B if slots is None else int(slots)
+        if n < B:
+            raise ValueError(f'{n} slots for {B} users')
+        self.flush_tables()
+        with self._inference_autocast():
+            seqs = self._stream_rows(log_seqs, seq_feature, mask)
+            key_valid = _valid_bytes(mask.to(dev))
+            rng, pos, states = K.seq_ranges(key_valid), _row_positions(B, T, dev), []
+
+            def layer(i, x):
+                y, s = self.attention_layers[i].read(x, key_valid, rng, pos)
+                if n > B:
+                    s = torch.cat([s, s.new_zeros(n - B, *s.shape[1:])])
+                states.append(s)
+                return y
+
+            feats = self._prenorm_blocks(seqs, layer)[:, -1, :]
+        position = torch.zeros(n, dtype=torch.int64, device=dev)
+        position[:B] = T
+        return feats, DecayStream(states, position)
+
+    @torch.no_grad()
+    def stream_step(self, stream, ids, feature, token_type, slots=None):
+        """One new event of each of n users: ids / token_type [n], feature the dict (or list of
+        dicts) of their features as [n, 1] sequences, slots int64 [n] the users' (None: the
+        stream's in order).  Returns the features [n, D] behind the events, what predict
+        gives for the longer history.  Events of one slot in a call are that user's next
+        events in order; a negative slot holds no event."""
+        if self.training:
+            raise RuntimeError('stream_step: call eval() first')
+        dev = self._device()
+        ids, token_type = ids.reshape(-1, 1), token_type.reshape(-1, 1)
+        n = ids.shape[0]
+        if slots is None:
+            if n != stream.position.numel():
+                raise ValueError(f'{n} events for the {stream.position.numel()} users of the stream: slots needed')
+            pos = stream.position.clone()
+            stream.position += 1
+        else:
+            slots = slots.to(dev, torch.int64).contiguous()
+            if slots.shape != (n,):
+                raise ValueError(f'{n} events, slots of shape {tuple(slots.shape)}')
+            inside = (slots >= 0) & (slots < stream.position.numel())
+            at = torch.where(inside, slots, 0)
+            earlier = torch.tril(slots[:, None] == slots[None, :], -1).sum(1)
+            pos = stream.position[at] + earlier
+            stream.position.index_add_(0, at, inside.to(torch.int64))
+        self.flush_tables()
+        with self._inference_autocast():
+            seqs = self._stream_rows(ids, feature, token_type)
+
+            def layer(i, x):
+                y = self.attention_layers[i].step(x.reshape(n, -1), pos, stream.states[i], slots, stream.err)
+                return y.view(x.shape)
+
+            return self._prenorm_blocks(seqs, layer)[:, -1, :]
 
     # -------------------------------------------------- model/BaseLine/model.py:352-384
     def forward(self, user_item, pos_seqs, neg_seqs, mask, next_mask, next_action_type, seq_feature, pos_feature,
@@ -1012,6 +1271,6 @@ def init_reference_(model, seed=None, live_norms=False):
                 t.weight[0].zero_()
         if live_norms:
             for mm in model.modules():
-                if isinstance(mm, torch.nn.LayerNorm):
+                if isinstance(mm, (torch.nn.LayerNorm, HeadNorm)):
                     mm.weight.fill_(1.0)
     return model

@@ -1,0 +1,285 @@
+"""The decay block and rotary positions in BaselineModel: the layer against a plain 64-bit
+composition, jagged rows against padded ones, the trainer (eager, graph, jagged), single
+events on kept states against predict on the longer history.
+
+Tolerances.  fp32 layers: GEMMs and kernels in fp32, sums of at most 4 * 64 + 128 terms and
+a norm that divides by a spread: 2^-24 times 2000.  A model is a few such layers: the same
+per layer, normwise.  bf16 models run the same rounding points on both sides; where the
+order of events differs (chunks against single steps) every layer re-rounds: u = 2^-8 per
+rounding, about 8 roundings a layer, two layers, unit gains: 16 u."""
+import zlib
+
+import pytest
+import torch
+import torch.nn.functional as F
+
+pytestmark = pytest.mark.gpu
+DEV = 'cuda'
+
+
+def gen(*key):
+    return torch.Generator(device=DEV).manual_seed(zlib.crc32(repr(key).encode()))
+
+
+def nrel(a, b):
+    a, b = a.detach(), b.detach()
+    return float((a.double() - b.double()).norm() / b.double().norm().clamp(min=1e-30))
+
+
+def make(block='decay', rotary=True, hidden=64, heads=2, maxlen=40, layers=2, seed=0, B=4, **over):
+    from tencent_recommendation_2025_amd import synthetic as S
+    from tencent_recommendation_2025_amd.model import BaselineModel, init_reference_
+    cfg = S.SyntheticConfig(batch_size=B, maxlen=maxlen, num_items=500, num_users=80, min_len=8)
+    stats, types = S.feature_schema(cfg)
+    m = BaselineModel(cfg.num_users, cfg.num_items, stats, types,
+                      S.make_args(hidden_units=hidden, maxlen=maxlen, num_blocks=layers, num_heads=heads, block=block,
+                                  rotary=rotary, **over)).to(DEV)
+    init_reference_(m, seed=seed, live_norms=True)
+    batch = S.make_batch(cfg, torch.Generator(device=DEV).manual_seed(seed + 1), torch.device(DEV))
+    return m, batch, cfg
+
+
+# ---------------------------------------------------------------- the layer ----
+def plain_layer(layer, x, valid):
+    """DecayAttention.forward in 64 bits from the formulas."""
+    B, T, D = x.shape
+    H, hd = layer.num_heads, layer.head_dim
+    P = {n: p.detach().double().requires_grad_(True) for n, p in layer.named_parameters()}
+    u, v, q, k = F.linear(x, P['uvqk.weight'], P['uvqk.bias']).split(D, -1)
+    if layer.rotary is not None:
+        pos, freqs, style, scale = layer.rotary.at(torch.arange(T, device=DEV))
+        ang = pos.double()[:, None] * freqs
+        c, s = torch.cos(ang)[:, None] * scale, torch.sin(ang)[:, None] * scale
+        r = freqs.numel()
+
+        def turn(z):
+            z = z.view(B, T, H, hd)
+            if style == 'half':
+                a, b = z[..., :r], z[..., r:2 * r]
+                return torch.cat([a * c - b * s, b * c + a * s, z[..., 2 * r:]], -1)
+            a, b = z[..., 0:2 * r:2], z[..., 1:2 * r:2]
+            return torch.cat([torch.stack([a * c - b * s, b * c + a * s], -1).flatten(-2), z[..., 2 * r:]], -1)
+        q, k = turn(q), turn(k)
+    m = valid[..., None, None]
+    q, k, v = (torch.where(m, z.reshape(B, T, H, hd), 0.0).transpose(1, 2) for z in (q, k, v))
+    t = torch.arange(T, device=DEV)
+    lag = t[:, None] - t[None, :]
+    A = (q @ k.transpose(-1, -2)) * hd ** -0.5
+    A = A * torch.exp(layer.log_decay.double()[:, None, None] * lag.clamp(min=0)) * (lag >= 0)
+    o = (A @ v).transpose(1, 2)
+    o = o - o.mean(-1, keepdim=True)
+    o = (o / torch.sqrt((o * o).mean(-1, keepdim=True) + layer.attn_norm.eps)).reshape(B, T, D)
+    y = (o * P['attn_norm.weight'] + P['attn_norm.bias']) * u * torch.sigmoid(u)
+    return F.linear(y, P['out_linear.weight'], P['out_linear.bias']), P
+
+
+@pytest.mark.parametrize('rotary', [None, True, {'dim': 16, 'layout': 'interleaved',
+                                                'scaling': {'kind': 'by_parts', 'factor': 4, 'window': 64}}])
+def test_layer_matches_the_formulas(rotary):
+    from tencent_recommendation_2025_amd.model import DecayAttention
+    torch.manual_seed(3)
+    layer = DecayAttention(96, 3, 0.0, rotary=rotary).to(DEV)
+    with torch.no_grad():
+        layer.attn_norm.weight.add_(0.2 * torch.randn(96, device=DEV))
+        layer.attn_norm.bias.add_(0.2 * torch.randn(96, device=DEV))
+    g = gen('layer')
+    x = torch.randn(2, 130, 96, device=DEV, generator=g, requires_grad=True)
+    valid = torch.arange(130, device=DEV) >= torch.tensor([[30], [0]], device=DEV)
+    dy = torch.randn(2, 130, 96, device=DEV, generator=g)
+    y, none = layer(x, key_valid=valid.to(torch.uint8))
+    assert none is None
+    names = [n for n, _ in layer.named_parameters()]
+    got = torch.autograd.grad(y, [x, *layer.parameters()], dy)
+    x64 = x.detach().double().requires_grad_(True)
+    ry, P = plain_layer(layer, x64, valid)
+    want = torch.autograd.grad(ry, [x64, *[P[n] for n in names]], dy.double())
+    tol = 2000 * 2.0 ** -24
+    assert nrel(y, ry) < tol
+    for n, a, b in zip(['x', *names], got, want):
+        assert nrel(a, b) < 4 * tol, n
+    # the reference's mask argument and its refusal
+    mask = torch.tril(torch.ones(130, 130, dtype=torch.bool, device=DEV)) & valid[:, None, :]
+    assert torch.equal(layer(x, attn_mask=mask)[0], y)
+    with pytest.raises(NotImplementedError):
+        layer(x, attn_mask=~mask)
+
+
+def test_layer_in_bf16_and_fp16_autocast():
+    from tencent_recommendation_2025_amd.model import DecayAttention
+    torch.manual_seed(4)
+    layer = DecayAttention(128, 2, 0.0, rotary=True).to(DEV)
+    g = gen('amp')
+    x = torch.randn(3, 201, 128, device=DEV, generator=g)
+    kv = torch.ones(3, 201, dtype=torch.uint8, device=DEV)
+    want, _ = plain_layer(layer, x.double(), kv.bool())
+    for dt, u in ((torch.bfloat16, 2.0 ** -8), (torch.float16, 2.0 ** -11)):
+        with torch.autocast('cuda', dtype=dt):
+            xx = x.clone().requires_grad_(True)
+            y, _ = layer(xx, key_valid=kv)
+        assert y.dtype == dt and nrel(y, want) < 8 * u
+        y.float().square().sum().backward()
+        assert bool(torch.isfinite(xx.grad).all()) and all(bool(torch.isfinite(p.grad).all()) for p in layer.parameters())
+        layer.zero_grad()
+
+
+def test_softmax_attention_with_rotary():
+    """q and k turned before the softmax kernels: scores depend on the distance, so shifting
+    all positions changes nothing; against plain attention on turned rows."""
+    from tencent_recommendation_2025_amd.model import FlashMultiHeadAttention
+    torch.manual_seed(5)
+    att = FlashMultiHeadAttention(64, 2, 0.0, rotary={'base': 500.0}).to(DEV).eval()
+    g = gen('softmax')
+    x = torch.randn(2, 50, 64, device=DEV, generator=g, requires_grad=True)
+    kv = torch.ones(2, 50, dtype=torch.uint8, device=DEV)
+    y, _ = att(x, x, x, key_valid=kv)
+    pos = torch.arange(50, dtype=torch.int64, device=DEV).repeat(2)
+    y2, _ = att(x, x, x, key_valid=kv, positions=pos + 12345)
+    assert nrel(y2, y) < 2000 * 2.0 ** -24
+    q, k, v = (lin(x).double().view(2, 50, 2, 32).transpose(1, 2) for lin in (att.q_linear, att.k_linear, att.v_linear))
+    _, freqs, _, _ = att.rotary.at(pos)
+    z = torch.polar(torch.ones(50, 16, dtype=torch.float64, device=DEV), torch.arange(50, device=DEV)[:, None] * freqs)
+
+    def turn(t):
+        r = torch.complex(t[..., :16], t[..., 16:]) * z
+        return torch.cat([r.real, r.imag], -1)
+    s = turn(q) @ turn(k).transpose(-1, -2) / 32 ** 0.5
+    s = s.masked_fill(torch.triu(torch.ones(50, 50, dtype=torch.bool, device=DEV), 1), float('-inf'))
+    o = (torch.softmax(s, -1) @ v).transpose(1, 2).reshape(2, 50, 64)
+    want = F.linear(o, att.out_linear.weight.double(), att.out_linear.bias.double())
+    # the softmax kernels' fp32 mode splits its operands into two bf16 parts (2^-16 each)
+    assert nrel(y, want) < 2.0 ** -12
+    dy = torch.randn(2, 50, 64, device=DEV, generator=g)
+    assert nrel(torch.autograd.grad(y, x, dy)[0], torch.autograd.grad(want, x, dy.double())[0]) < 2.0 ** -12
+
+
+# ---------------------------------------------------------------- the model ----
+@pytest.mark.parametrize('block', ['decay', 'softmax'])
+def test_model_trains_and_leaves_the_position_table(block):
+    m, batch, _ = make(block)
+    m.train()
+    pos_logits, neg_logits = m(*batch[:9])
+    ntt = batch[4] == 1
+    loss = F.softplus(-pos_logits[ntt]).mean() + F.softplus(neg_logits[ntt]).mean()
+    loss.backward()
+    assert bool(torch.isfinite(loss))
+    assert m.pos_emb.weight.grad is None          # rotary: the table takes no part
+    for n, p in m.named_parameters():
+        if n.startswith('attention_layers') and p.dim() >= 2:
+            assert p.grad is not None and float(p.grad.abs().max()) > 0, n
+    assert ('attention_layers.0.log_decay' in m.state_dict()) == (block == 'decay')
+
+
+@pytest.mark.parametrize('block,rotary', [('decay', True), ('decay', None), ('softmax', True)])
+def test_trainer_graph_and_jagged_rows(block, rotary):
+    """The fused trainer: a captured step equals the eager one bit by bit over several
+    batches, and jagged rows follow the padded layout's losses."""
+    from tencent_recommendation_2025_amd import jagged as J
+    from tencent_recommendation_2025_amd import synthetic as S
+    from tencent_recommendation_2025_amd.optim import FusedAdamW
+    from tencent_recommendation_2025_amd.train import Trainer
+    losses = {}
+    for mode in ('eager', 'graph', 'jagged'):
+        m, _, cfg = make(block, rotary, hidden=128)
+        kw = dict(graph=True) if mode == 'graph' else dict(jagged=True, jagged_quantum=64) if mode == 'jagged' else {}
+        tr = Trainer(m, FusedAdamW(m, lr=1e-3), loss='bce', **kw)
+        g = torch.Generator(device=DEV).manual_seed(11)
+        out = []
+        for _ in range(7):
+            b = S.make_batch(cfg, g, torch.device(DEV))
+            out.append(tr.step(b, **({'rows': J.span_rows(b[3])} if mode == 'jagged' else {})).clone())
+            torch.cuda.synchronize()
+        losses[mode] = torch.stack(out)
+        assert bool(torch.isfinite(losses[mode]).all())
+    assert torch.equal(losses['graph'], losses['eager'])
+    # 7 steps of a bf16 model whose GEMMs see other row counts: 16 u
+    assert nrel(losses['jagged'], losses['eager']) < 16 * 2.0 ** -8
+
+
+def to_rows(feat, sl):
+    return {k: v[:, sl] for k, v in feat.items()}
+
+
+@pytest.mark.parametrize('fused', [False, True])
+def test_stream_follows_predict(fused):
+    """Histories read up to a point and then event by event give predict's features of the
+    longer history (fp32 tables, and the fused trainer's bf16 tables)."""
+    m, batch, cfg = make(hidden=64, layers=2, B=5)
+    if fused:
+        from tencent_recommendation_2025_amd.optim import FusedAdamW
+        FusedAdamW(m, lr=1e-3)
+    m.eval()
+    seq, tt, feat = batch[0], batch[3], batch[6]
+    T, m_steps = seq.shape[1], 6
+    cut = T - m_steps
+    head = slice(0, cut)
+    first, stream = m.stream_begin(seq[:, head], to_rows(feat, head), tt[:, head], slots=8)
+    tol = 16 * 2.0 ** -8 if fused else 2 * 2000 * 2.0 ** -24
+    with torch.no_grad():
+        assert nrel(first, m.predict(seq[:, head], to_rows(feat, head), tt[:, head])) < tol
+        order = torch.tensor([3, 0, 4, 1, 2], device=DEV)
+        for t in range(cut, T):
+            s = slice(t, t + 1)
+            got = m.stream_step(stream, seq[order, t], {k: v[order, s] for k, v in feat.items()}, tt[order, t],
+                                slots=order)
+            want = m.predict(seq[:, :t + 1], to_rows(feat, slice(0, t + 1)), tt[:, :t + 1])
+            assert nrel(got, want[order]) < tol, t
+    assert stream.position.tolist() == [T] * 5 + [0] * 3
+    stream.check()
+
+
+def test_stream_events_of_one_user_in_one_call_and_free_slots():
+    m, batch, cfg = make(B=3)
+    m.eval()
+    seq, tt, feat = batch[0], batch[3], batch[6]
+    T = seq.shape[1]
+    head = slice(0, T - 2)
+    _, one = m.stream_begin(seq[:, head], to_rows(feat, head), tt[:, head])
+    for t in (T - 2, T - 1):
+        last = m.stream_step(one, seq[:, t], to_rows(feat, slice(t, t + 1)), tt[:, t])
+    # both events of every user, and an empty event, in one call
+    _, both = m.stream_begin(seq[:, head], to_rows(feat, head), tt[:, head], slots=5)
+    idx = torch.tensor([0, 1, 2, 0, 1, 2, 0], device=DEV)
+    at = torch.tensor([T - 2] * 3 + [T - 1] * 4, device=DEV)
+    slots = torch.tensor([0, 1, 2, 0, 1, 2, -1], device=DEV)
+    got = m.stream_step(both, seq[idx, at], {k: v[idx, at][:, None] for k, v in feat.items()}, tt[idx, at], slots)
+    tol = 2 * 2000 * 2.0 ** -24
+    assert nrel(got[3:6], last) < tol
+    for a, b in zip(both.states, one.states):
+        assert nrel(a[:3], b) < tol and bool((a[3:] == 0).all())
+    assert both.position.tolist() == [T, T, T, 0, 0]
+    # a user moved to another slot goes on there; a cleared slot starts anew
+    both.place(torch.tensor([4, 3, 1], device=DEV), one)
+    both.clear(torch.tensor([0], device=DEV))
+    assert both.position.tolist() == [0, T, T, T, T] and bool((both.states[0][0] == 0).all())
+    assert torch.equal(both.states[1][4], one.states[1][0])
+    m.stream_step(both, seq[:1, 0], to_rows({k: v[:1] for k, v in feat.items()}, slice(0, 1)), tt[:1, 0],
+                  slots=torch.tensor([5], device=DEV))
+    with pytest.raises(ValueError):
+        both.check()
+
+
+def test_stream_and_block_refusals():
+    m, batch, _ = make(B=2)
+    a = (batch[0], batch[6], batch[3])
+    with pytest.raises(RuntimeError):
+        m.stream_begin(*a)
+    m.eval()
+    with pytest.raises(ValueError):
+        m.stream_begin(*a, slots=1)
+    _, s = m.stream_begin(*a, slots=3)
+    with pytest.raises(ValueError):
+        m.stream_step(s, batch[0][:, 0], to_rows(batch[6], slice(0, 1)), batch[3][:, 0])
+    with pytest.raises(ValueError):
+        m.stream_step(s, batch[0][:, 0], to_rows(batch[6], slice(0, 1)), batch[3][:, 0], slots=torch.zeros(3, device=DEV))
+    for kw in (dict(block='softmax', rotary=True), dict(block='decay', rotary=None)):
+        n, b, _ = make(**kw)
+        n.eval()
+        with pytest.raises(NotImplementedError):
+            n.stream_begin(b[0], b[6], b[3])
+    with pytest.raises(NotImplementedError):
+        make(block='hstu', rotary=True)
+    with pytest.raises(NotImplementedError):
+        make(hidden=512, heads=2)
+    for bad in ({'dim': 200}, {'layout': 'pairs'}, {'theta': 3}):
+        with pytest.raises(ValueError):
+            make(rotary=bad)
