@@ -15,17 +15,27 @@
 // quarter of the time the chunk's 32 KB take from HBM on one CU of 256, so the kernel is
 // bound by memory and by what hides its latency: the next chunk is loaded to registers
 // while this one is computed, and 4 workgroups share a CU.
+//
+// LDS rows are 16 bytes longer than the head: 16 rows' 16-byte pieces fall on all 64 banks
+// at once, every address is a lane's base plus a constant, and a transposing read that
+// takes every second row (4 rows 8 banks apart) has no conflicts either.  So the
+// contraction over the 64 steps takes each 8 of them in the order 0 2 4 6 1 3 5 7 ("slots"):
+// P and the weights of the state's sum are laid down in that order.
 #include "grk_decay.h"
 #include "grk_mfma.h"
 
 namespace grk {
 
-// Powers of g in LDS: pw[n] = g^n for 0 <= n <= 64 and 0 for -16 < n < 0 (above the diagonal).
-constexpr int kDecayPowers = 16 + kDecayChunk + 1;
+// Tables in LDS: scale g^n for 0 <= n <= 64, 0 for -16 < n < 0 (above the diagonal); the
+// state's weights g^(63 - j) by slot; one word a step that holds an event.
+constexpr int kDecayPowers = 16 + kDecayChunk + 4;
+
+template <int DP> constexpr int decay_stride() { return DP * 2 + 16; }   // bytes of an LDS row
+constexpr int kDecayPStride = decay_stride<kDecayChunk>();
 
 template <int DP> constexpr size_t decay_lds_bf16(bool state_only) {
-  return (size_t)(state_only ? 2 : 3) * kDecayChunk * DP * 2 + (state_only ? 0 : kDecayChunk * kDecayChunk * 2) +
-         kDecayChunk * 4 + (kDecayPowers + 3) / 4 * 16;
+  return (size_t)(state_only ? 2 : 3) * kDecayChunk * decay_stride<DP>() +
+         (state_only ? 0 : kDecayChunk * kDecayPStride) + (kDecayPowers + 2 * kDecayChunk) * 4;
 }
 
 __device__ __forceinline__ void mfma32(bf16x8 a, bf16x8 b, f32x4& c) {
@@ -33,24 +43,30 @@ __device__ __forceinline__ void mfma32(bf16x8 a, bf16x8 b, f32x4& c) {
   mfma_keep(c, a, b);
 }
 
-// Fragment of M^T: element s of lane (c, g) = M[row0 + 8 g + s][col0 + c].  A 16-lane group
-// of the transposing read takes 4 rows of 16 columns, lane i of it the row i / 4 from
-// column 4 (i % 4) on, and receives column i of the 4 rows.
-template <int HD>
-__device__ __forceinline__ bf16x8 lds_col8(const char* base, int row0, int col0, int lane) {
-  const int i = lane & 15, row = row0 + 8 * (lane >> 4) + (i >> 2), col = col0 + 4 * (i & 3);
+__device__ __forceinline__ bf16x8 lds_b128(const char* p) {
+  return __builtin_bit_cast(bf16x8, *reinterpret_cast<const uint4*>(p));
+}
+
+// Fragment of M^T in slot order from a lane's base (decay_col_base): rows 8 g + 0 2 4 6 and
+// + 1 3 5 7 of column c.  A 16-lane group of the transposing read takes 4 rows of 16
+// columns, lane i of it row i / 4 from column 4 (i % 4) on, and receives column i.
+template <int ST>
+__device__ __forceinline__ int decay_col_base(int lane) {
+  const int i = lane & 15;
+  return (8 * (lane >> 4) + 2 * (i >> 2)) * ST + 8 * (i & 3);
+}
+template <int ST>
+__device__ __forceinline__ bf16x8 lds_col8s(const char* p) {
   typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
-  const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(base + lds_off<HD>(row, col)));
-  const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(base + lds_off<HD>(row + 4, col)));
+  const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)p);
+  const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p + ST));
   const bf16x4 l = __builtin_bit_cast(bf16x4, lo), h = __builtin_bit_cast(bf16x4, hi);
   return bf16x8{l[0], l[1], l[2], l[3], h[0], h[1], h[2], h[3]};
 }
 
-// Fragment of the rows in the state's order: M[row][col0 + 4 g + s], M[row][col0 + 16 + 4 g + s].
-template <int HD>
-__device__ __forceinline__ bf16x8 lds_row_pair(const char* base, int row, int col0, int g) {
-  const uint2 a = *reinterpret_cast<const uint2*>(base + lds_off<HD>(row, col0 + 4 * g));
-  const uint2 b = *reinterpret_cast<const uint2*>(base + lds_off<HD>(row, col0 + 16 + 4 * g));
+// Fragment of a row in the state's order: columns 4 g + s and 16 + 4 g + s from p = column 4 g.
+__device__ __forceinline__ bf16x8 lds_row_pair(const char* p) {
+  const uint2 a = *reinterpret_cast<const uint2*>(p), b = *reinterpret_cast<const uint2*>(p + 32);
   return __builtin_bit_cast(bf16x8, make_uint4(a.x, a.y, b.x, b.y));
 }
 
@@ -62,34 +78,40 @@ __device__ __forceinline__ bf16x8 pack8(const float* f) {
 }
 
 // Rows of a chunk on their way from memory: thread t holds columns [8 (t % (DP / 8)), + 8) of
-// row t / (DP / 8) and of every R-th after it, R = threads / (DP / 8).  Masked steps are loaded too (their row exists) and zeroed by
+// row t / (DP / 8) and of every R-th after it, R = threads / (DP / 8).  The chunk's lowest
+// row is a uniform pointer, a lane's offset from it 32 bits (the host admits row strides
+// below 2^24 elements).  Masked steps are loaded too (their row exists) and zeroed by
 // selection, so the loads do not wait for the mask.
 template <int DP, int NTH>
 struct DecayRows {
   static constexpr int R = NTH / (DP / 8), N = kDecayChunk / R;
-  int64_t row[N];
-  bool live[N];
-  __device__ __forceinline__ void at(const DecayParams& p, const DecayPlace& w, int rev, int64_t base, int t0) {
+  unsigned at[N];    // the row's place above the chunk's lowest
+  bool live[N];      // it holds an event
+  int64_t low;       // the chunk's lowest row
+  __device__ __forceinline__ void chunk(const DecayParams& p, const DecayPlace& w, int rev, int64_t base, bool masked,
+                                        int t0) {
+    const int n = w.t1 - t0 < kDecayChunk ? w.t1 - t0 : kDecayChunk;
+    const int pos0 = rev ? p.seq_len - t0 - n : w.start + t0;
+    low = base + pos0;
 #pragma unroll
     for (int k = 0; k < N; ++k) {
-      const int t = t0 + (int)threadIdx.x / (DP / 8) + R * k;
-      const int pos = rev ? p.seq_len - 1 - t : w.start + t;
-      const int64_t r = base + pos;
-      live[k] = t < w.t1 && r >= 0 && r < p.capacity;
-      row[k] = live[k] ? r : 0;
-      if (p.key_valid && live[k]) live[k] = p.key_valid[(int64_t)w.b * p.seq_len + pos] != 0;
+      const int t = (int)threadIdx.x / (DP / 8) + R * k, s = t < n ? t : n - 1;
+      at[k] = rev ? n - 1 - s : s;
+      live[k] = t < n;
+      if (masked) live[k] = live[k] && p.key_valid[(int64_t)w.b * p.seq_len + pos0 + at[k]] != 0;
     }
   }
-  __device__ __forceinline__ void load(uint4* f, const void* src, int64_t ld, int64_t col) const {
+  __device__ __forceinline__ void load(uint4* f, const void* src, int64_t ld, int64_t col, int ccol) const {
+    const char* q = reinterpret_cast<const char*>(src) + (low * ld + col) * 2;
 #pragma unroll
     for (int k = 0; k < N; ++k)
-      f[k] = *reinterpret_cast<const uint4*>(reinterpret_cast<const bf16_t*>(src) + row[k] * ld + col);
+      f[k] = *reinterpret_cast<const uint4*>(q + (at[k] * (unsigned)ld + (unsigned)ccol) * 2u);
   }
   __device__ __forceinline__ void store(const uint4* f, char* dst, bool has) const {
 #pragma unroll
     for (int k = 0; k < N; ++k)
-      *reinterpret_cast<uint4*>(dst + lds_off<DP>((int)threadIdx.x / (DP / 8) + R * k, (int)threadIdx.x % (DP / 8) * 8)) =
-          live[k] && has ? f[k] : make_uint4(0u, 0u, 0u, 0u);
+      *reinterpret_cast<uint4*>(dst + ((int)threadIdx.x / (DP / 8) + R * k) * decay_stride<DP>() +
+                                (int)threadIdx.x % (DP / 8) * 16) = live[k] && has ? f[k] : make_uint4(0u, 0u, 0u, 0u);
   }
 };
 
@@ -99,24 +121,29 @@ struct DecayRows {
 template <int DP, int NE, int NS, bool STATE>
 __global__ void __launch_bounds__(DP * 4 / NE, NE == 1 ? 4 : 2) k_decay_bf16(DecayParams p) {
   constexpr int C = kDecayChunk, NT = DP / 16, KS = DP / 32, NW = NT / NE, NTH = NW * 64;
+  constexpr int ST = decay_stride<DP>(), PS = kDecayPStride;
   using Rows = DecayRows<DP, NTH>;
   extern __shared__ __attribute__((aligned(16))) char lds[];
   char* sb = lds;
-  char* sc = sb + C * DP * 2;
-  char* sa = sc + C * DP * 2;
-  char* sp = sa + (STATE ? 0 : C * DP * 2);
-  float* pw = reinterpret_cast<float*>(sp + (STATE ? 0 : C * C * 2)) + 16;
-  int* slive = reinterpret_cast<int*>(pw - 16 + (kDecayPowers + 3) / 4 * 4);
-  const DecayPlace w = decay_place(p);
+  char* sc = sb + C * ST;
+  char* sa = sc + C * ST;
+  char* sp = sa + (STATE ? 0 : C * ST);
+  float* pw = reinterpret_cast<float*>(sp + (STATE ? 0 : C * PS)) + 16;
+  float* wv = pw - 16 + kDecayPowers;
+  int* slive = reinterpret_cast<int*>(wv + C);
+  DecayPlace w = decay_place(p);
   if (!w.on) return;
   const DecayRole r = p.role[w.role];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int g = lane >> 4, c = lane & 15;
   const int64_t bh = (int64_t)w.b * p.heads + w.h, hcol = (int64_t)w.h * p.head_dim;
   const int64_t base = p.row_base ? p.row_base[w.b] : (int64_t)w.b * p.seq_len;
+  if (base + w.start < 0 || base + p.seq_len > p.capacity) w.t1 = w.t0;   // rows that do not exist: no step
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int g = lane >> 4, c = lane & 15;
+  // (a range that grk_seq_ranges calls contiguous leaves nothing to mask)
+  const bool masked = p.key_valid && !(p.seq_range && p.seq_range[3 * (int64_t)w.b + 1] == 1);
   const int ccol = (int)threadIdx.x % (DP / 8) * 8;      // this thread's columns when rows are moved
   const bool has = ccol < p.head_dim;
-  const int64_t mcol = hcol + (has ? ccol : 0);
+  const int mcol = has ? ccol : 0;
   f32x4 st[NE][NT];
   float* frag = p.ws + (((int64_t)w.role * p.batch * p.heads + bh) * p.nseg + w.seg) * DP * DP;
   bool some = STATE || (p.nseg > 1 ? w.seg > 0 || p.state_in : p.state_in != nullptr);   // the state is not all 0
@@ -141,16 +168,26 @@ __global__ void __launch_bounds__(DP * 4 / NE, NE == 1 ? 4 : 2) k_decay_bf16(Dec
   Rows rows;
   uint4 fa[Rows::N], fb[Rows::N], fc[Rows::N];
   if (w.t0 < w.t1) {
-    rows.at(p, w, r.rev, base, w.t0);
-    rows.load(fb, r.b, r.ldb, mcol);
-    rows.load(fc, r.c, r.ldc, mcol);
-    if (!STATE) rows.load(fa, r.a, r.lda, mcol);
+    rows.chunk(p, w, r.rev, base, masked, w.t0);
+    rows.load(fb, r.b, r.ldb, hcol, mcol);
+    rows.load(fc, r.c, r.ldc, hcol, mcol);
+    if (!STATE) rows.load(fa, r.a, r.lda, hcol, mcol);
   }
-  for (int n = threadIdx.x; n < kDecayPowers; n += NTH) pw[n - 16] = n < 16 ? 0.f : decay_pow(w.lg, n - 16);
+  if (!STATE)
+    for (int n = threadIdx.x; n <= 16 + C; n += NTH) pw[n - 16] = n < 16 ? 0.f : p.scale * decay_pow(w.lg, n - 16);
+  auto weights = [&](int n) {   // of a chunk of n steps, by slot
+    for (int k = threadIdx.x; k < C; k += NTH) {
+      const int q = k & 7, j = k - q + (q < 4 ? 2 * q : 2 * q - 7);
+      wv[k] = j < n ? decay_pow(w.lg, n - 1 - j) : 0.f;
+    }
+  };
+  weights(C);
+  const float gc = decay_pow(w.lg, C);
   if constexpr (!STATE) {
-    for (int n = threadIdx.x; n < C * C / 8; n += NTH) reinterpret_cast<uint4*>(sp)[n] = make_uint4(0u, 0u, 0u, 0u);
+    for (int n = threadIdx.x; n < C * PS / 16; n += NTH) reinterpret_cast<uint4*>(sp)[n] = make_uint4(0u, 0u, 0u, 0u);
     decay_zero_rows<bf16_t>(p, w, r);
   }
+  const int row_b = c * ST + 16 * g, col_b = decay_col_base<ST>(lane);   // this lane's LDS bases
   for (int t0 = w.t0; t0 < w.t1; t0 += C) {
     const int n = w.t1 - t0 < C ? w.t1 - t0 : C;
     const bool last = t0 + C >= w.t1;
@@ -164,26 +201,30 @@ __global__ void __launch_bounds__(DP * 4 / NE, NE == 1 ? 4 : 2) k_decay_bf16(Dec
         for (int k = 0; k < Rows::N; ++k) slive[(int)threadIdx.x / (DP / 8) + Rows::R * k] = rows.live[k];
       }
     }
+    const int64_t low = rows.low;
     __syncthreads();
     if (!last) {
-      rows.at(p, w, r.rev, base, t0 + C);
-      rows.load(fb, r.b, r.ldb, mcol);
-      rows.load(fc, r.c, r.ldc, mcol);
-      if (!STATE) rows.load(fa, r.a, r.lda, mcol);
+      rows.chunk(p, w, r.rev, base, masked, t0 + C);
+      rows.load(fb, r.b, r.ldb, hcol, mcol);
+      rows.load(fc, r.c, r.ldc, hcol, mcol);
+      if (!STATE) rows.load(fa, r.a, r.lda, hcol, mcol);
     }
     if constexpr (!STATE) {
       // P^T, lower tiles; the tiles above the diagonal that a 32-deep step reads stay 0
       for (int tile = wave; tile < 10; tile += NW) {
         const int it = tile >= 6 ? 3 : tile >= 3 ? 2 : tile >= 1 ? 1 : 0, jt = tile - it * (it + 1) / 2;
+        const char* q = sa + 16 * it * ST + row_b;
+        const char* k = sb + 16 * jt * ST + row_b;
         f32x4 x = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks)
-          mfma32(lds_row8<DP>(sb, 16 * jt + c, 32 * ks + 8 * g), lds_row8<DP>(sa, 16 * it + c, 32 * ks + 8 * g), x);
+        for (int ks = 0; ks < KS; ++ks) mfma32(lds_b128(k + 64 * ks), lds_b128(q + 64 * ks), x);
         const float* lag = pw + 16 * (it - jt) + c - 4 * g;
-        bf16x4 y;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) y[i] = (__bf16)(x[i] * lag[-i]);
-        *reinterpret_cast<bf16x4*>(sp + lds_off<C>(16 * it + c, 16 * jt + 4 * g)) = y;
+        const bf16x4 y = {(__bf16)(x[0] * lag[0]), (__bf16)(x[2] * lag[-2]), (__bf16)(x[1] * lag[-1]),
+                          (__bf16)(x[3] * lag[-3])};
+        const uint2 z = __builtin_bit_cast(uint2, y);   // steps 0 2 | 1 3 of four
+        char* dst = sp + (16 * it + c) * PS + (2 * jt + (g >> 1)) * 16 + 4 * (g & 1);
+        *reinterpret_cast<unsigned*>(dst) = z.x;
+        *reinterpret_cast<unsigned*>(dst + 8) = z.y;
       }
       __syncthreads();
     }
@@ -191,7 +232,7 @@ __global__ void __launch_bounds__(DP * 4 / NE, NE == 1 ? 4 : 2) k_decay_bf16(Dec
 #pragma unroll
     for (int x = 0; x < NE; ++x)
 #pragma unroll
-      for (int ks = 0; ks < 2; ++ks) vf[x][ks] = lds_col8<DP>(sc, 32 * ks, 16 * (NE * wave + x), lane);
+      for (int ks = 0; ks < 2; ++ks) vf[x][ks] = lds_col8s<ST>(sc + col_b + 32 * ks * ST + 32 * (NE * wave + x));
     if constexpr (!STATE) {
       bf16x8 sf[NE][KS];
 #pragma unroll
@@ -202,6 +243,7 @@ __global__ void __launch_bounds__(DP * 4 / NE, NE == 1 ? 4 : 2) k_decay_bf16(Dec
           const float f[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
           sf[x][ks] = pack8(f);
         }
+      char* out = reinterpret_cast<char*>(r.out) + (low * r.ldo + hcol) * 2;
 #pragma unroll
       for (int it = 0; it < C / 16; ++it) {
         f32x4 o[NE];
@@ -210,38 +252,42 @@ __global__ void __launch_bounds__(DP * 4 / NE, NE == 1 ? 4 : 2) k_decay_bf16(Dec
         if (some) {
 #pragma unroll
           for (int ks = 0; ks < KS; ++ks) {
-            const bf16x8 q = lds_row_pair<DP>(sa, 16 * it + c, 32 * ks, g);
+            const bf16x8 q = lds_row_pair(sa + c * ST + 8 * g + 16 * it * ST + 64 * ks);
 #pragma unroll
             for (int x = 0; x < NE; ++x) mfma32(sf[x][ks], q, o[x]);
           }
+          const float rise = pw[16 * it + c + 1];
 #pragma unroll
-          for (int x = 0; x < NE; ++x) o[x] *= pw[16 * it + c + 1];
+          for (int x = 0; x < NE; ++x) o[x] *= rise;
         }
 #pragma unroll
         for (int ks = 0; ks <= it / 2; ++ks) {
-          const bf16x8 y = lds_row8<C>(sp, 16 * it + c, 32 * ks + 8 * g);
+          const bf16x8 y = lds_b128(sp + c * PS + 16 * g + 16 * it * PS + 64 * ks);
 #pragma unroll
           for (int x = 0; x < NE; ++x) mfma32(vf[x][ks], y, o[x]);
         }
         const int t = 16 * it + c;
-        const int64_t row = base + (r.rev ? p.seq_len - 1 - (t0 + t) : w.start + t0 + t);
-        if (t < n && row >= 0 && row < p.capacity) {
+        if (t < n) {
           const bool live = slive[t];
+          const unsigned at = (unsigned)(r.rev ? n - 1 - t : t) * (unsigned)r.ldo;
 #pragma unroll
           for (int x = 0; x < NE; ++x) {
             const int e = 16 * (NE * wave + x) + 4 * g;
-            bf16x4 y;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) y[i] = (__bf16)(live ? p.scale * o[x][i] : 0.f);
-            if (e < p.head_dim)
-              *reinterpret_cast<bf16x4*>(reinterpret_cast<bf16_t*>(r.out) + row * r.ldo + hcol + e) = y;
+            const bf16x4 y = {(__bf16)o[x][0], (__bf16)o[x][1], (__bf16)o[x][2], (__bf16)o[x][3]};
+            const uint2 z = live ? __builtin_bit_cast(uint2, y) : make_uint2(0u, 0u);
+            if (e < p.head_dim) *reinterpret_cast<uint2*>(out + (at + (unsigned)e) * 2u) = z;
           }
         }
       }
     }
     if (!STATE && last && !(p.nseg == 1 && p.state_out)) break;   // nothing reads the state any more
     some = true;
-    const float gn = pw[n];
+    float gn = gc;
+    if (n < C) {   // the last chunk only
+      weights(n);
+      __syncthreads();
+      gn = decay_pow(w.lg, n);
+    }
 #pragma unroll
     for (int x = 0; x < NE; ++x)
 #pragma unroll
@@ -249,14 +295,13 @@ __global__ void __launch_bounds__(DP * 4 / NE, NE == 1 ? 4 : 2) k_decay_bf16(Dec
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks) {
       bf16x8 part[NE][NS];
+      const f32x4 w0 = *reinterpret_cast<const f32x4*>(wv + 32 * ks + 8 * g);
+      const f32x4 w1 = *reinterpret_cast<const f32x4*>(wv + 32 * ks + 8 * g + 4);
 #pragma unroll
       for (int x = 0; x < NE; ++x) {
         float f[8];
 #pragma unroll
-        for (int s = 0; s < 8; ++s) {
-          const int j = 32 * ks + 8 * g + s;
-          f[s] = (float)vf[x][ks][s] * (j < n ? pw[n - 1 - j] : 0.f);
-        }
+        for (int s = 0; s < 8; ++s) f[s] = (float)vf[x][ks][s] * (s < 4 ? w0[s & 3] : w1[s & 3]);
 #pragma unroll
         for (int q = 0; q < NS; ++q) {
           part[x][q] = pack8(f);
@@ -266,7 +311,7 @@ __global__ void __launch_bounds__(DP * 4 / NE, NE == 1 ? 4 : 2) k_decay_bf16(Dec
       }
 #pragma unroll
       for (int dt = 0; dt < NT; ++dt) {
-        const bf16x8 k = lds_col8<DP>(sb, 32 * ks, 16 * dt, lane);
+        const bf16x8 k = lds_col8s<ST>(sb + col_b + 32 * ks * ST + 32 * dt);
 #pragma unroll
         for (int x = 0; x < NE; ++x)
 #pragma unroll
@@ -320,13 +365,14 @@ static int decay_bf16_run(const DecayParams& p, hipStream_t s) {
   return GRK_OK;
 }
 
-// Whole 16-byte vectors: rows, strides and heads start on them (8 bytes for the output).
+// Whole 16-byte vectors: rows, strides and heads start on them (8 bytes for the output);
+// 64 rows' offsets fit 32 bits.
 bool decay_bf16_takes(const DecayParams& p) {
   bool ok = p.head_dim % 8 == 0;
   for (int i = 0; i < p.roles; ++i) {
     const DecayRole& r = p.role[i];
     ok = ok && ((uintptr_t)r.a | (uintptr_t)r.b | (uintptr_t)r.c) % 16 == 0 && (r.lda | r.ldb | r.ldc) % 8 == 0 &&
-         (uintptr_t)r.out % 8 == 0 && r.ldo % 4 == 0;
+         (uintptr_t)r.out % 8 == 0 && r.ldo % 4 == 0 && (r.lda | r.ldb | r.ldc | r.ldo) < (1 << 24);
   }
   return ok;
 }

@@ -558,10 +558,18 @@ def test_offsets_past_32_bits(K):
     pos, (freqs, _) = torch.arange(n, device=DEV), K.rotary_frequencies(64, device=DEV)
     assert torch.equal(K.rotary(x, pos, freqs, 2), K.rotary(c, pos, freqs, 2))
     assert torch.equal(K.head_norm_fwd(x, None, None, 2), K.head_norm_fwd(c, None, None, 2))
-    lg = decays(2)
-    assert torch.equal(K.decay_attn_fwd(x, x, x, lg, 1, n), K.decay_attn_fwd(c, c, c, lg, 1, n))
-    for a, b in zip(K.decay_attn_bwd(x, x, x, x, lg, 1, n), K.decay_attn_bwd(c, c, c, c, lg, 1, n)):
-        assert torch.equal(a, b)
+    # attention: strides of 2^24 and more take the general kernel, shorter ones the bf16 kernel
+    for ld, n in ((ld, n), (2 ** 23 + 8, 300)):
+        buf = torch.empty(ld * n, device=DEV, dtype=torch.bfloat16)
+        x = buf.as_strided((n, 128), (ld, 1))
+        x.copy_(randn(g, n, 128, dt=torch.bfloat16))
+        lg, one = decays(2), x.reshape(1, n, 2, 64)
+        want = decay_ref(one, one, one, lg, torch.ones(1, n, dtype=torch.bool, device=DEV), 0.125, one)
+        close(K.decay_attn_fwd(x, x, x, lg, 1, n), want[0], decay_tol(torch.bfloat16))
+        for a, b in zip(K.decay_attn_bwd(x, x, x, x, lg, 1, n), want[2:]):
+            close(a, b, decay_tol(torch.bfloat16))
+        out = torch.empty(ld * n, device=DEV, dtype=torch.bfloat16).as_strided((n, 128), (ld, 1))
+        close(K.decay_attn_fwd(x, x, x, lg, 1, n, out=out), want[0], decay_tol(torch.bfloat16))
 
 
 # ------------------------------------------------- graphs, streams, a run of them --
