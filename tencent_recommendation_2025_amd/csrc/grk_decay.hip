@@ -378,10 +378,13 @@ int decay_scan_launch(const DecayParams& p, int dp, hipStream_t s) {
 static int decay_dp(int hd) { return hd <= 16 ? 16 : hd <= 32 ? 32 : hd <= 64 ? 64 : 128; }
 
 // Segments: a workgroup walks a sequence alone where the (sequence, head) pairs already
-// fill the card; else the sequence is cut, at least 4 chunks to a segment.
+// fill half the workgroups that run at once (4 a CU; 2 with heads wider than 64); else the
+// sequence is cut into as many segments as fill them, of at least 4 chunks.  (A cut costs a
+// second read of two operands and the traffic of its states: one round of longer
+// segments beat two of shorter ones.)
 static void decay_segments(DecayParams& p) {
-  const int64_t units = (int64_t)p.roles * p.batch * p.heads;
-  int64_t nseg = units >= 512 ? 1 : 1024 / (units > 0 ? units : 1);
+  const int64_t units = (int64_t)p.roles * p.batch * p.heads, slots = p.head_dim > 64 ? 512 : 1024;
+  int64_t nseg = 2 * units >= slots ? 1 : slots / (units > 0 ? units : 1);
   const int64_t most = p.seq_len / (4 * kDecayChunk);
   if (nseg > most) nseg = most;
   if (nseg < 1) nseg = 1;

@@ -145,7 +145,7 @@ __global__ void __launch_bounds__(DP * 4 / NE, NE == 1 ? 4 : 2) k_decay_bf16(Dec
   const bool has = ccol < p.head_dim;
   const int mcol = has ? ccol : 0;
   f32x4 st[NE][NT];
-  float* frag = p.ws + (((int64_t)w.role * p.batch * p.heads + bh) * p.nseg + w.seg) * DP * DP;
+  float* frag = p.ws + (((int64_t)(w.role < 2 ? w.role : 1) * p.batch * p.heads + bh) * p.nseg + w.seg) * DP * DP;
   bool some = STATE || (p.nseg > 1 ? w.seg > 0 || p.state_in : p.state_in != nullptr);   // the state is not all 0
 #pragma unroll
   for (int x = 0; x < NE; ++x) {
@@ -154,7 +154,12 @@ __global__ void __launch_bounds__(DP * 4 / NE, NE == 1 ? 4 : 2) k_decay_bf16(Dec
     for (int dt = 0; dt < NT; ++dt) {
       st[x][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
       if (!STATE && p.nseg > 1) {
-        st[x][dt] = *reinterpret_cast<const f32x4*>(frag + ((dt * NT + et) * 64 + lane) * 4);
+        if (w.role < 2) {
+          st[x][dt] = *reinterpret_cast<const f32x4*>(frag + ((dt * NT + et) * 64 + lane) * 4);
+        } else {   // the transpose of role 1's state, element by element
+#pragma unroll
+          for (int i = 0; i < 4; ++i) st[x][dt][i] = frag[((et * NT + dt) * 64 + (c >> 2) * 16 + 4 * g + i) * 4 + (c & 3)];
+        }
       } else if (!STATE && p.state_in) {
         const float f = decay_pow(w.lg, w.start);
 #pragma unroll
@@ -188,10 +193,12 @@ __global__ void __launch_bounds__(DP * 4 / NE, NE == 1 ? 4 : 2) k_decay_bf16(Dec
     decay_zero_rows<bf16_t>(p, w, r);
   }
   const int row_b = c * ST + 16 * g, col_b = decay_col_base<ST>(lane);   // this lane's LDS bases
+  // A chunk: its rows to LDS | P, what the output takes from the state, the state's step |
+  // the output.  Two barriers: behind the second one only P is read, so the next chunk's
+  // rows may be laid down at once.
   for (int t0 = w.t0; t0 < w.t1; t0 += C) {
     const int n = w.t1 - t0 < C ? w.t1 - t0 : C;
     const bool last = t0 + C >= w.t1;
-    __syncthreads();
     rows.store(fb, sb, has);
     rows.store(fc, sc, has);
     if constexpr (!STATE) {
@@ -226,96 +233,107 @@ __global__ void __launch_bounds__(DP * 4 / NE, NE == 1 ? 4 : 2) k_decay_bf16(Dec
         *reinterpret_cast<unsigned*>(dst) = z.x;
         *reinterpret_cast<unsigned*>(dst + 8) = z.y;
       }
-      __syncthreads();
     }
     bf16x8 vf[NE][2];
 #pragma unroll
     for (int x = 0; x < NE; ++x)
 #pragma unroll
       for (int ks = 0; ks < 2; ++ks) vf[x][ks] = lds_col8s<ST>(sc + col_b + 32 * ks * ST + 32 * (NE * wave + x));
+    f32x4 o[C / 16][NE];
+    bool live[C / 16];
     if constexpr (!STATE) {
-      bf16x8 sf[NE][KS];
-#pragma unroll
-      for (int x = 0; x < NE; ++x)
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-          const f32x4 a = st[x][2 * ks], b = st[x][2 * ks + 1];
-          const float f[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
-          sf[x][ks] = pack8(f);
-        }
-      char* out = reinterpret_cast<char*>(r.out) + (low * r.ldo + hcol) * 2;
 #pragma unroll
       for (int it = 0; it < C / 16; ++it) {
-        f32x4 o[NE];
+        live[it] = slive[16 * it + c];
 #pragma unroll
-        for (int x = 0; x < NE; ++x) o[x] = f32x4{0.f, 0.f, 0.f, 0.f};
-        if (some) {
+        for (int x = 0; x < NE; ++x) o[it][x] = f32x4{0.f, 0.f, 0.f, 0.f};
+      }
+      if (some) {
+        bf16x8 sf[NE][KS];
+#pragma unroll
+        for (int x = 0; x < NE; ++x)
+#pragma unroll
+          for (int ks = 0; ks < KS; ++ks) {
+            const f32x4 a = st[x][2 * ks], b = st[x][2 * ks + 1];
+            const float f[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+            sf[x][ks] = pack8(f);
+          }
+#pragma unroll
+        for (int it = 0; it < C / 16; ++it) {
 #pragma unroll
           for (int ks = 0; ks < KS; ++ks) {
             const bf16x8 q = lds_row_pair(sa + c * ST + 8 * g + 16 * it * ST + 64 * ks);
 #pragma unroll
-            for (int x = 0; x < NE; ++x) mfma32(sf[x][ks], q, o[x]);
+            for (int x = 0; x < NE; ++x) mfma32(sf[x][ks], q, o[it][x]);
           }
           const float rise = pw[16 * it + c + 1];
 #pragma unroll
-          for (int x = 0; x < NE; ++x) o[x] *= rise;
+          for (int x = 0; x < NE; ++x) o[it][x] *= rise;
         }
+      }
+    }
+    if (STATE || !last || (p.nseg == 1 && p.state_out)) {   // (nothing reads the state behind the last chunk else)
+      some = true;
+      float gn = gc;
+      if (n < C) {   // the last chunk only
+        weights(n);
+        __syncthreads();
+        gn = decay_pow(w.lg, n);
+      }
+#pragma unroll
+      for (int x = 0; x < NE; ++x)
+#pragma unroll
+        for (int dt = 0; dt < NT; ++dt) st[x][dt] *= gn;
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks) {
+        bf16x8 part[NE][NS];
+        const f32x4 w0 = *reinterpret_cast<const f32x4*>(wv + 32 * ks + 8 * g);
+        const f32x4 w1 = *reinterpret_cast<const f32x4*>(wv + 32 * ks + 8 * g + 4);
+#pragma unroll
+        for (int x = 0; x < NE; ++x) {
+          float f[8];
+#pragma unroll
+          for (int s = 0; s < 8; ++s) f[s] = (float)vf[x][ks][s] * (s < 4 ? w0[s & 3] : w1[s & 3]);
+#pragma unroll
+          for (int q = 0; q < NS; ++q) {
+            part[x][q] = pack8(f);
+#pragma unroll
+            for (int s = 0; s < 8; ++s) f[s] -= (float)part[x][q][s];
+          }
+        }
+#pragma unroll
+        for (int dt = 0; dt < NT; ++dt) {
+          const bf16x8 k = lds_col8s<ST>(sb + col_b + 32 * ks * ST + 32 * dt);
+#pragma unroll
+          for (int x = 0; x < NE; ++x)
+#pragma unroll
+            for (int q = NS - 1; q >= 0; --q) mfma32(k, part[x][q], st[x][dt]);
+        }
+      }
+    }
+    __syncthreads();
+    if constexpr (!STATE) {
+      char* out = reinterpret_cast<char*>(r.out) + (low * r.ldo + hcol) * 2;
+#pragma unroll
+      for (int it = 0; it < C / 16; ++it) {
 #pragma unroll
         for (int ks = 0; ks <= it / 2; ++ks) {
           const bf16x8 y = lds_b128(sp + c * PS + 16 * g + 16 * it * PS + 64 * ks);
 #pragma unroll
-          for (int x = 0; x < NE; ++x) mfma32(vf[x][ks], y, o[x]);
+          for (int x = 0; x < NE; ++x) mfma32(vf[x][ks], y, o[it][x]);
         }
         const int t = 16 * it + c;
         if (t < n) {
-          const bool live = slive[t];
           const unsigned at = (unsigned)(r.rev ? n - 1 - t : t) * (unsigned)r.ldo;
 #pragma unroll
           for (int x = 0; x < NE; ++x) {
             const int e = 16 * (NE * wave + x) + 4 * g;
-            const bf16x4 y = {(__bf16)o[x][0], (__bf16)o[x][1], (__bf16)o[x][2], (__bf16)o[x][3]};
-            const uint2 z = live ? __builtin_bit_cast(uint2, y) : make_uint2(0u, 0u);
+            const f32x4 v = o[it][x];
+            const bf16x4 y = {(__bf16)v[0], (__bf16)v[1], (__bf16)v[2], (__bf16)v[3]};
+            const uint2 z = live[it] ? __builtin_bit_cast(uint2, y) : make_uint2(0u, 0u);
             if (e < p.head_dim) *reinterpret_cast<uint2*>(out + (at + (unsigned)e) * 2u) = z;
           }
         }
-      }
-    }
-    if (!STATE && last && !(p.nseg == 1 && p.state_out)) break;   // nothing reads the state any more
-    some = true;
-    float gn = gc;
-    if (n < C) {   // the last chunk only
-      weights(n);
-      __syncthreads();
-      gn = decay_pow(w.lg, n);
-    }
-#pragma unroll
-    for (int x = 0; x < NE; ++x)
-#pragma unroll
-      for (int dt = 0; dt < NT; ++dt) st[x][dt] *= gn;
-#pragma unroll
-    for (int ks = 0; ks < 2; ++ks) {
-      bf16x8 part[NE][NS];
-      const f32x4 w0 = *reinterpret_cast<const f32x4*>(wv + 32 * ks + 8 * g);
-      const f32x4 w1 = *reinterpret_cast<const f32x4*>(wv + 32 * ks + 8 * g + 4);
-#pragma unroll
-      for (int x = 0; x < NE; ++x) {
-        float f[8];
-#pragma unroll
-        for (int s = 0; s < 8; ++s) f[s] = (float)vf[x][ks][s] * (s < 4 ? w0[s & 3] : w1[s & 3]);
-#pragma unroll
-        for (int q = 0; q < NS; ++q) {
-          part[x][q] = pack8(f);
-#pragma unroll
-          for (int s = 0; s < 8; ++s) f[s] -= (float)part[x][q][s];
-        }
-      }
-#pragma unroll
-      for (int dt = 0; dt < NT; ++dt) {
-        const bf16x8 k = lds_col8s<ST>(sb + col_b + 32 * ks * ST + 32 * dt);
-#pragma unroll
-        for (int x = 0; x < NE; ++x)
-#pragma unroll
-          for (int q = NS - 1; q >= 0; --q) mfma32(k, part[x][q], st[x][dt]);
       }
     }
   }
@@ -336,21 +354,26 @@ __global__ void __launch_bounds__(DP * 4 / NE, NE == 1 ? 4 : 2) k_decay_bf16(Dec
     }
 }
 
+// Segment states are those of roles 0 and 1: role 2 (K, Q, dO) sums q dO^T where role 1
+// (V, dO, Q) sums dO q^T.
 template <int DP, int NE>
 static int decay_bf16_run(const DecayParams& p, hipStream_t s) {
-  const int64_t groups = (int64_t)p.batch * p.heads * p.nseg;
-  const unsigned grid = (unsigned)((groups + 7) / 8 * 8 * p.roles);
+  const int64_t groups = ((int64_t)p.batch * p.heads * p.nseg + 7) / 8 * 8;
+  const unsigned grid = (unsigned)(groups * p.roles);
   if (p.nseg > 1) {
+    DecayParams q = p;
+    q.roles = p.roles < 2 ? p.roles : 2;
+    const unsigned sgrid = (unsigned)(groups * q.roles);
     constexpr size_t lds = decay_lds_bf16<DP>(true);
     if (p.state_out) {
       GRK_CHECK_HIP(ensure_dynamic_lds((const void*)k_decay_bf16<DP, NE, 3, true>, lds));
-      k_decay_bf16<DP, NE, 3, true><<<grid, DP * 4 / NE, lds, s>>>(p);
+      k_decay_bf16<DP, NE, 3, true><<<sgrid, DP * 4 / NE, lds, s>>>(q);
     } else {
       GRK_CHECK_HIP(ensure_dynamic_lds((const void*)k_decay_bf16<DP, NE, 1, true>, lds));
-      k_decay_bf16<DP, NE, 1, true><<<grid, DP * 4 / NE, lds, s>>>(p);
+      k_decay_bf16<DP, NE, 1, true><<<sgrid, DP * 4 / NE, lds, s>>>(q);
     }
     GRK_LAUNCH_CHECK();
-    const int rc = decay_scan_launch(p, DP, s);
+    const int rc = decay_scan_launch(q, DP, s);
     if (rc) return rc;
   }
   constexpr size_t lds = decay_lds_bf16<DP>(false);
