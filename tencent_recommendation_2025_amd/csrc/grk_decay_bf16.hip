@@ -77,8 +77,18 @@ __device__ __forceinline__ bf16x8 pack8(const float* f) {
   return r;
 }
 
+// The row of the chunk that DP / 8 threads hold first: 16 neighbouring lanes write one row
+// of 128 columns, or rows 8 (4) apart whose 16-byte pieces fall on different banks.
+template <int DP>
+__device__ __forceinline__ int decay_first_row() {
+  const int q = (int)threadIdx.x / (DP / 8);
+  if constexpr (DP == 128) return q;
+  if constexpr (DP == 64) return (q & 1) * 8 + (q >> 1 & 7) + (q & ~15);
+  return (q & 3) * 4 + (q >> 2 & 3) + (q & ~15);
+}
+
 // Rows of a chunk on their way from memory: thread t holds columns [8 (t % (DP / 8)), + 8) of
-// row t / (DP / 8) and of every R-th after it, R = threads / (DP / 8).  The chunk's lowest
+// its first row and of every R-th after it, R = threads / (DP / 8).  The chunk's lowest
 // row is a uniform pointer, a lane's offset from it 32 bits (the host admits row strides
 // below 2^24 elements).  Masked steps are loaded too (their row exists) and zeroed by
 // selection, so the loads do not wait for the mask.
@@ -95,7 +105,7 @@ struct DecayRows {
     low = base + pos0;
 #pragma unroll
     for (int k = 0; k < N; ++k) {
-      const int t = (int)threadIdx.x / (DP / 8) + R * k, s = t < n ? t : n - 1;
+      const int t = decay_first_row<DP>() + R * k, s = t < n ? t : n - 1;
       at[k] = rev ? n - 1 - s : s;
       live[k] = t < n;
       if (masked) live[k] = live[k] && p.key_valid[(int64_t)w.b * p.seq_len + pos0 + at[k]] != 0;
@@ -110,7 +120,7 @@ struct DecayRows {
   __device__ __forceinline__ void store(const uint4* f, char* dst, bool has) const {
 #pragma unroll
     for (int k = 0; k < N; ++k)
-      *reinterpret_cast<uint4*>(dst + ((int)threadIdx.x / (DP / 8) + R * k) * decay_stride<DP>() +
+      *reinterpret_cast<uint4*>(dst + (decay_first_row<DP>() + R * k) * decay_stride<DP>() +
                                 (int)threadIdx.x % (DP / 8) * 16) = live[k] && has ? f[k] : make_uint4(0u, 0u, 0u, 0u);
   }
 };
@@ -205,7 +215,7 @@ __global__ void __launch_bounds__(DP * 4 / NE, NE == 1 ? 4 : 2) k_decay_bf16(Dec
       rows.store(fa, sa, has);
       if (ccol == 0) {
 #pragma unroll
-        for (int k = 0; k < Rows::N; ++k) slive[(int)threadIdx.x / (DP / 8) + Rows::R * k] = rows.live[k];
+        for (int k = 0; k < Rows::N; ++k) slive[decay_first_row<DP>() + Rows::R * k] = rows.live[k];
       }
     }
     const int64_t low = rows.low;

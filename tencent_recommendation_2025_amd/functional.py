@@ -8,6 +8,7 @@ kernels require device tensors.
 """
 from __future__ import annotations
 
+import functools
 import os
 import weakref
 
@@ -1026,12 +1027,22 @@ def _once(backward):
     return run
 
 
+def _uncompiled(fn):
+    """fn outside of compiled graphs (as _disable, whose wrapper costs every eager call too)."""
+    apart = _disable(fn)
+
+    def run(*args, **kw):
+        return apart(*args, **kw) if torch.compiler.is_compiling() else fn(*args, **kw)
+    return functools.wraps(fn)(run)
+
+
 class _RotaryFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, positions, freqs, heads, layout, scale):
         ctx.save_for_backward(positions, freqs)
         ctx.meta = (heads, layout, scale)
-        return K.rotary(_head_mat(x), positions, freqs, heads, layout, scale).view(x.shape)
+        y = K.rotary(_head_mat(x), positions, freqs, heads, layout, scale)
+        return y if x.dim() == 2 else y.view(x.shape)
 
     @staticmethod
     @_once
@@ -1039,49 +1050,46 @@ class _RotaryFn(torch.autograd.Function):
         positions, freqs = ctx.saved_tensors
         heads, layout, scale = ctx.meta
         g = K.rotary(_head_mat(gy), positions, freqs, heads, layout, scale, inverse=True)
-        return g.view(gy.shape), None, None, None, None, None
+        return (g if gy.dim() == 2 else g.view(gy.shape)), None, None, None, None, None
 
 
-@_disable
+@_uncompiled
 def rotary(x, positions, freqs, heads, layout='half', scale=1.0):
     """Rotary positions of x [..., heads * head_dim] (kernels.rotary): positions one per row
     (any shape of as many entries), freqs float64 [rotary_dim / 2].  The gradient is the
     turn back; positions and freqs get none."""
     if freqs.requires_grad:
         raise L.GrkError('rotary: freqs get no gradient')
-    return _RotaryFn.apply(x, positions.reshape(-1).contiguous(), freqs, int(heads), layout, float(scale))
+    if positions.dim() != 1 or not positions.is_contiguous():
+        positions = positions.reshape(-1).contiguous()
+    return _RotaryFn.apply(x, positions, freqs, heads, layout, scale)
 
 
 class _DecayAttnFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, qkv, log_decay, key_valid, seq_range, row_base, batch, seq_len, scale):
         x = _head_mat(qkv)
-        o = K.decay_attn_packed_fwd(x, log_decay, batch, seq_len, scale, key_valid, seq_range, row_base)
+        o, ctx.args = K.decay_attn_packed_fwd(x, log_decay, batch, seq_len, scale, key_valid, seq_range, row_base)
         ctx.save_for_backward(x, log_decay, key_valid, seq_range, row_base)
-        ctx.meta = (batch, seq_len, scale, qkv.shape)
-        return o.view(*qkv.shape[:-1], o.shape[1])
+        ctx.shape = qkv.shape
+        return o if qkv.dim() == 2 else o.view(*qkv.shape[:-1], o.shape[1])
 
     @staticmethod
     @_once
     def backward(ctx, go):
-        x, log_decay, key_valid, seq_range, row_base = ctx.saved_tensors
-        batch, seq_len, scale, shape = ctx.meta
-        dx = K.decay_attn_packed_bwd(_head_mat(go, x.dtype), x, log_decay, batch, seq_len, scale, key_valid,
-                                     seq_range, row_base)
-        return dx.view(shape), None, None, None, None, None, None, None
+        saved = ctx.saved_tensors
+        dx = K.decay_attn_packed_bwd(_head_mat(go, saved[0].dtype), ctx.args, *saved)
+        return (dx if len(ctx.shape) == 2 else dx.view(ctx.shape)), None, None, None, None, None, None, None
 
 
-@_disable
+@_uncompiled
 def decay_attn(qkv, log_decay, batch, seq_len, scale=None, key_valid=None, seq_range=None, row_base=None):
     """Linear attention with a decay for each head (kernels.decay_attn_fwd) of packed
     q | k | v rows [..., 3 * heads * head_dim]; differentiable in qkv.  The decays are
     given, not learned: log_decay (fp32 [heads]) gets no gradient."""
     if log_decay.requires_grad:
         raise L.GrkError('decay_attn: log_decay gets no gradient (the decays are given, not learned)')
-    if qkv.shape[-1] % 3:
-        raise L.GrkError('qkv must hold q | k | v side by side: [rows, 3 * heads * head_dim]')
-    return _DecayAttnFn.apply(qkv, log_decay, key_valid, seq_range, row_base, int(batch), int(seq_len),
-                              None if scale is None else float(scale))
+    return _DecayAttnFn.apply(qkv, log_decay, key_valid, seq_range, row_base, batch, seq_len, scale)
 
 
 def _fp32_vec(t):
@@ -1105,25 +1113,26 @@ class _HeadNormFn(torch.autograd.Function):
     def backward(ctx, gy):
         x2, w32, b32, g2 = ctx.saved_tensors
         heads, eps, shape, gdt, wdt, bdt = ctx.meta
-        dx, dg, dw, db = K.head_norm_bwd(_head_mat(gy, x2.dtype), x2, w32, b32, heads, eps, g2)
+        dx, dg, dw, db = K.head_norm_grad(_head_mat(gy, x2.dtype), x2, w32, b32, g2, heads, eps)
         if dw is not None and wdt != torch.float32:
             dw = dw.to(wdt)
         if db is not None and bdt != torch.float32:
             db = db.to(bdt)
-        if dg is not None:
-            dg = dg.view(shape)
-            dg = dg if dg.dtype == gdt else dg.to(gdt)
-        return dx.view(shape), dw, db, dg, None, None
+        if dg is not None and dg.dtype != gdt:
+            dg = dg.to(gdt)
+        if len(shape) != 2:
+            dx, dg = dx.view(shape), dg.view(shape) if dg is not None else None
+        return dx, dw, db, dg, None, None
 
 
-@_disable
+@_uncompiled
 def head_norm(x, weight, bias, heads, eps=1e-5, gate=None):
     """Layer norm of each head's columns of x [..., heads * head_dim], times SiLU(gate)
     (kernels.head_norm_fwd); differentiable in x, weight, bias and gate.  weight / bias
     [heads * head_dim] or None; the gate has x's shape."""
     if gate is not None and gate.shape != x.shape:
         raise L.GrkError('the gate must have the shape of x')
-    return _HeadNormFn.apply(x, weight, bias, gate, int(heads), float(eps))
+    return _HeadNormFn.apply(x, weight, bias, gate, heads, eps)
 
 
 class _RotaryQKFn(torch.autograd.Function):
@@ -1148,7 +1157,7 @@ class _RotaryQKFn(torch.autograd.Function):
                 None, None, None, None, None)
 
 
-@_disable
+@_uncompiled
 def rotary_qk(qkv, positions, freqs, heads, layout='half', scale=1.0):
     """q | k | v rows [..., 3 * heads * head_dim] with q and k turned by their positions
     (kernels.rotary) and v as it is."""
@@ -1196,7 +1205,7 @@ class _DecayCoreFn(torch.autograd.Function):
         return dx.view(shape), None, dw.to(wdt), db.to(bdt), None, None, None
 
 
-@_disable
+@_uncompiled
 def decay_core(pre, log_decay, weight, bias, batch, seq_len, key_valid=None, seq_range=None, row_base=None, eps=1e-5,
                rot=None):
     """norm(decay_attn(rotary(q), rotary(k), v)) * SiLU(u) of [N, 4 D] (u | v | q | k) rows,

@@ -1154,7 +1154,7 @@ _NO_DEVICE = contextlib.nullcontext()
 
 def _on_device(index):
     """That device as the current one for a launch (no cost where it is already)."""
-    return _NO_DEVICE if index == torch.cuda.current_device() else torch.cuda.device(index)
+    return _NO_DEVICE if index == torch._C._cuda_getDevice() else torch.cuda.device(index)
 
 
 def _same_device(ref, *ts):
@@ -1342,7 +1342,8 @@ def _decay_workspace(args, backward, device):
 
 
 def decay_attn_packed_fwd(qkv, log_decay, batch, seq_len, scale=None, key_valid=None, seq_range=None, row_base=None):
-    """decay_attn_fwd of the rows q | k | v side by side, [rows, 3 * heads * head_dim]."""
+    """decay_attn_fwd of the rows q | k | v side by side, [rows, 3 * heads * head_dim]:
+    (out, the call's arguments for decay_attn_packed_bwd)."""
     dev = _same_device(qkv, log_decay, key_valid, seq_range, row_base)
     rows, cols = qkv.shape if qkv.dim() == 2 else (-1, -1)
     if cols < 0 or cols % 3:
@@ -1353,29 +1354,36 @@ def decay_attn_packed_fwd(qkv, log_decay, batch, seq_len, scale=None, key_valid=
     a = _decay_struct(layout, _row_code(dt), scale, *_thirds(x, ld, D, dt), log_decay, key_valid, seq_range, row_base,
                       rows)
     out = torch.empty((rows, D), dtype=dt, device=qkv.device)
+    lib = L.lib()
     with _on_device(dev):
-        ws, n = _decay_workspace(a, 0, qkv.device)
-        rc = L.lib().grk_decay_attn_fwd(a, None, None, out.data_ptr(), D, _ptr(ws), n, L.raw_stream(dev))
+        n = lib.grk_decay_attn_workspace(a, 0)
+        ws = torch.empty(n, dtype=torch.uint8, device=qkv.device) if n else None
+        rc = lib.grk_decay_attn_fwd(a, None, None, out.data_ptr(), D, _ptr(ws), n, L.raw_stream(dev))
     L.check(rc, 'grk_decay_attn_fwd')
-    return out
+    return out, a
 
 
-def decay_attn_packed_bwd(dout, qkv, log_decay, batch, seq_len, scale=None, key_valid=None, seq_range=None,
-                          row_base=None):
-    """Gradient of decay_attn_packed_fwd: dq | dk | dv side by side."""
-    dev = _same_device(qkv, dout, log_decay, key_valid, seq_range, row_base)
+def decay_attn_packed_bwd(dout, args, qkv, log_decay, key_valid=None, seq_range=None, row_base=None):
+    """Gradient of decay_attn_packed_fwd, dq | dk | dv side by side: args are that call's, the
+    tensors those it was given (wherever they lie by now: saved tensors may have moved)."""
+    dev = _same_device(qkv, dout)
     rows, cols = qkv.shape
     dt, D = qkv.dtype, cols // 3
-    layout = _decay_layout(log_decay, rows, D, batch, seq_len, key_valid, seq_range, row_base)
-    x, ld = _head_rows(qkv, 'qkv', rows, cols, dt)
-    a = _decay_struct(layout, _row_code(dt), scale, *_thirds(x, ld, D, dt), log_decay, key_valid, seq_range, row_base,
-                      rows)
+    a = args
+    if (qkv.data_ptr(), log_decay.data_ptr(), _ptr(key_valid), _ptr(seq_range), _ptr(row_base)) != \
+            (a.q or 0, a.log_decay, a.key_valid, a.seq_range, a.row_base):
+        x, ld = _head_rows(qkv, 'qkv', rows, cols, dt)
+        a = _decay_struct((a.batch, a.seq_len, a.heads, a.head_dim), a.dtype, a.scale, *_thirds(x, ld, D, dt),
+                          log_decay, key_valid, seq_range, row_base, rows)
     gp, gl = _head_rows(dout, 'dout', rows, D, dt)
     dx = torch.empty((rows, cols), dtype=dt, device=qkv.device)
-    (p0, _), (p1, _), (p2, _) = _thirds(dx.data_ptr(), cols, D, dt)
+    dp, step = dx.data_ptr(), D * dt.itemsize
+    lib = L.lib()
     with _on_device(dev):
-        ws, n = _decay_workspace(a, 1, qkv.device)
-        rc = L.lib().grk_decay_attn_bwd(a, gp, gl, p0, cols, p1, cols, p2, cols, _ptr(ws), n, L.raw_stream(dev))
+        n = lib.grk_decay_attn_workspace(a, 1)
+        ws = torch.empty(n, dtype=torch.uint8, device=qkv.device) if n else None
+        rc = lib.grk_decay_attn_bwd(a, gp, gl, dp, cols, dp + step, cols, dp + 2 * step, cols, _ptr(ws), n,
+                                    L.raw_stream(dev))
     L.check(rc, 'grk_decay_attn_bwd')
     return dx
 
@@ -1524,33 +1532,49 @@ def head_norm_fwd(x, weight, bias, heads, eps=1e-5, gate=None, out=None):
 def head_norm_bwd(dy, x, weight, bias, heads, eps=1e-5, gate=None, dx=None, dgate=None):
     """Gradients of head_norm_fwd: (dx, dgate or None, dweight or None, dbias or None);
     dweight / dbias fp32, in a fixed order of addition."""
-    device = x.device
-    dev = _same_device(x, dy, weight, bias, gate, dx, dgate)
-    xp, xl, gp, gl = _norm_operands(x, weight, bias, heads, gate)
-    N, cols = x.shape
-    dt = x.dtype
-    code = _row_code(dt)
-    yp, yl = _head_rows(dy, 'dy', N, cols, dt)
-    if dx is None:
-        dx = torch.empty((N, cols), dtype=dt, device=device)
-    else:
+    _same_device(x, weight, bias, gate, dx, dgate)
+    _norm_operands(x, weight, bias, heads, gate)
+    _row_code(x.dtype)
+    if dx is not None:
+        _head_rows(dx, 'dx', *x.shape, x.dtype)
         _fresh(dx, 'dx', dy, x, gate)
+    if gate is not None and dgate is not None:
+        _head_rows(dgate, 'dgate', *x.shape, x.dtype)
+        _fresh(dgate, 'dgate', dy, x, gate, dx)
+    return head_norm_grad(dy, x, weight, bias, gate, heads, eps, dx, dgate)
+
+
+def head_norm_grad(dy, x, weight, bias, gate, heads, eps, dx=None, dgate=None):
+    """head_norm_bwd of operands that head_norm_fwd has taken (only dy is looked at)."""
+    device, dt = x.device, x.dtype
+    dev = _same_device(x, dy)
+    N, cols = x.shape
+    yp, yl = _head_rows(dy, 'dy', N, cols, dt)
+    empty = torch.empty
+    if dx is None:
+        dx = empty((N, cols), dtype=dt, device=device)
+    gp, gl, dgp, dgl = None, 0, None, 0
     if gate is None:
         dgate = None
-    elif dgate is None:
-        dgate = torch.empty((N, cols), dtype=dt, device=device)
     else:
-        _fresh(dgate, 'dgate', dy, x, gate, dx)
-    dw = torch.empty(cols, dtype=torch.float32, device=device) if weight is not None else None
-    db = torch.empty(cols, dtype=torch.float32, device=device) if bias is not None else None
-    dxp, dxl = _head_rows(dx, 'dx', N, cols, dt)
-    dgp, dgl = _head_rows(dgate, 'dgate', N, cols, dt) if dgate is not None else (None, 0)
-    lib = L.lib()
+        if dgate is None:
+            dgate = empty((N, cols), dtype=dt, device=device)
+        gp, gl, dgp, dgl = gate.data_ptr(), gate.stride(0), dgate.data_ptr(), dgate.stride(0)
+    lib, nb = L.lib(), 0
+    wp = bp = dw = db = dwp = dbp = ws = None
+    if weight is not None:
+        dw = empty(cols, dtype=torch.float32, device=device)
+        wp, dwp = weight.data_ptr(), dw.data_ptr()
+    if bias is not None:
+        db = empty(cols, dtype=torch.float32, device=device)
+        bp, dbp = bias.data_ptr(), db.data_ptr()
+    if dwp or dbp:
+        nb = lib.grk_head_norm_bwd_workspace(N, heads, cols // heads)
+        ws = empty(nb, dtype=torch.uint8, device=device) if nb else None
     with _on_device(dev):
-        nb = lib.grk_head_norm_bwd_workspace(N, heads, cols // heads) if dw is not None or db is not None else 0
-        ws = torch.empty(nb, dtype=torch.uint8, device=device) if nb else None
-        rc = lib.grk_head_norm_bwd(yp, yl, xp, xl, gp, gl, _ptr(weight), _ptr(bias), eps, N, heads, cols // heads,
-                                   code, dxp, dxl, dgp, dgl, _ptr(dw), _ptr(db), _ptr(ws), nb, L.raw_stream(dev))
+        rc = lib.grk_head_norm_bwd(yp, yl, x.data_ptr(), x.stride(0), gp, gl, wp, bp, eps, N, heads, cols // heads,
+                                   _ROW_DTYPES[dt], dx.data_ptr(), dx.stride(0), dgp, dgl, dwp, dbp, _ptr(ws), nb,
+                                   L.raw_stream(dev))
     L.check(rc, 'grk_head_norm_bwd')
     return dx, dgate, dw, db
 
