@@ -1,6 +1,8 @@
 // Decayed linear attention for gfx950 (the formulas: grk_decay.h): the general kernel --
 // fp32, bf16 or fp16 rows, any head_dim up to 128 -- on the fp32 matrix instruction, the
 // segments' scan and the single-step kernel.
+#include <type_traits>
+
 #include "grk_decay.h"
 
 namespace grk {
@@ -174,50 +176,57 @@ __global__ void __launch_bounds__(DP * 4) k_decay_f32(DecayParams p) {
 }
 
 // The segments' own states -> the state before each segment (and behind the last one):
-// run <- g^len run + own, four elements of the state to a thread.
-template <int DP>
+// run <- g^len run + own, W elements of the state to a thread.  Few states are bound by the
+// latency of their loads: one element a thread, the loads of U segments (8, 16 or 32, as
+// there are) in flight at once (24 states of 64 x 64, 26 segments: 7.7 us; 4 elements and
+// 8 loads 8.8).  Many are bound by memory: 4 elements, 8 loads (32 states of 128 x 128, 16
+// segments: 7.5 us; one element 14.3).
+template <int DP, int W, int U>
 __global__ void __launch_bounds__(256) k_decay_scan(DecayParams p) {
-  constexpr int NT = DP / 16;
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;   // (role, b, h, fragment)
-  const int f = (int)(i % (DP * DP / 4));
-  const int64_t rbh = i / (DP * DP / 4);
+  constexpr int NT = DP / 16, N = DP * DP / W;
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;   // (role, b, h, elements in fragment order)
+  const int f = (int)(i % N) * W;
+  const int64_t rbh = i / N;
   if (rbh >= (int64_t)p.roles * p.batch * p.heads) return;
   const int64_t bh = rbh % ((int64_t)p.batch * p.heads);
   const int b = (int)(bh / p.heads), h = (int)(bh % p.heads);
-  const int lane = f & 63, wave = f >> 6 & (NT - 1), dt = f >> 6 >> __builtin_ctz(NT);
-  const int col = 16 * wave + (lane & 15), d0 = 16 * dt + 4 * (lane >> 4);
+  const int lane = f >> 2 & 63, tile = f >> 8, wave = tile & (NT - 1), dt = tile / NT;
+  const int e = 16 * wave + (lane & 15), d0 = 16 * dt + 4 * (lane >> 4) + (f & 3);
   int start = p.seq_range ? p.seq_range[3 * (int64_t)b] : 0;
   start = start < 0 ? 0 : (start > p.seq_len ? p.seq_len : start);
   const int len = p.seq_len - start;
-  const float lg = fminf(p.log_decay[h], 0.f);
-  f32x4 run = {0.f, 0.f, 0.f, 0.f};
+  const float lg = fminf(p.log_decay[h], 0.f), gs = decay_pow(lg, p.seg_len);
+  typedef float vec __attribute__((ext_vector_type(W)));
+  vec run = 0.f;
+  auto outside = [&](int k) { return (bh * p.head_dim + d0 + k) * p.head_dim + e; };   // in state_in / state_out
+  auto has = [&](int k) { return d0 + k < p.head_dim && e < p.head_dim; };
   if (p.state_in) {
     const float g0 = decay_pow(lg, start);
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (d0 + e < p.head_dim && col < p.head_dim)
-        run[e] = g0 * p.state_in[(bh * p.head_dim + d0 + e) * p.head_dim + col];
+    for (int k = 0; k < W; ++k)
+      if (has(k)) run[k] = g0 * p.state_in[outside(k)];
   }
-  f32x4* own = reinterpret_cast<f32x4*>(p.ws + rbh * p.nseg * DP * DP) + f;
-  constexpr int U = 8;   // loads in flight: the recurrence itself is short
+  vec* own = reinterpret_cast<vec*>(p.ws + rbh * p.nseg * DP * DP + f);
   for (int s0 = 0; s0 < p.nseg; s0 += U) {
-    f32x4 x[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (s0 + u < p.nseg) x[u] = own[(int64_t)(s0 + u) * (DP * DP / 4)];
+    vec x[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int s = s0 + u, left = len - s * p.seg_len, n = left < 0 ? 0 : (left < p.seg_len ? left : p.seg_len);
-      if (s >= p.nseg) break;
-      own[(int64_t)s * (DP * DP / 4)] = run;
-      run = run * decay_pow(lg, n) + x[u];
+      const int s = s0 + u < p.nseg ? s0 + u : p.nseg - 1;
+      x[u] = own[(int64_t)s * N];
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int s = s0 + u, left = len - s * p.seg_len;   // steps from this segment on
+      if (s < p.nseg) {
+        own[(int64_t)s * N] = run;
+        run = run * (left >= p.seg_len ? gs : decay_pow(lg, left < 0 ? 0 : left)) + x[u];
+      }
     }
   }
   if (p.state_out) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (d0 + e < p.head_dim && col < p.head_dim)
-        p.state_out[(bh * p.head_dim + d0 + e) * p.head_dim + col] = run[e];
+    for (int k = 0; k < W; ++k)
+      if (has(k)) p.state_out[outside(k)] = run[k];
   }
 }
 
@@ -252,8 +261,8 @@ __device__ __forceinline__ int64_t step_slot(const StepParams& p, int64_t i) {
 
 // Events of one slot are consecutive events of that user: the first one's workgroup
 // takes them all, in order.  links[i] = (an earlier event has this slot, the next event
-// that has it), by comparing every pair: 8 threads an event, an eighth of the others each.
-constexpr int kLinkShare = 8;
+// that has it), by comparing every pair: 32 threads an event, a part of the others each.
+constexpr int kLinkShare = 32;
 __global__ void __launch_bounds__(kStepThreads) k_step_links(StepParams p) {
   __shared__ int64_t tile[kStepThreads];
   const int64_t i = (int64_t)blockIdx.x * (kStepThreads / kLinkShare) + threadIdx.x / kLinkShare;
@@ -282,6 +291,24 @@ __global__ void __launch_bounds__(kStepThreads) k_step_links(StepParams p) {
     p.links[2 * i] = before;
     p.links[2 * i + 1] = next == 0x7fffffff ? -1 : next;
   }
+}
+
+// The states pass the caches by: each is touched once a call, and a pool is larger than they
+// are (1024 events of 8 heads of 64: 57.3 -> 52.3 us, the rate of a large copy).
+template <int V>
+__device__ __forceinline__ void state_load(const float* p, float* s) {
+  if constexpr (V == 4) {
+    const f32x4 x = __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(p));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s[i] = x[i];
+  } else {
+    s[0] = __builtin_nontemporal_load(p);
+  }
+}
+template <int V>
+__device__ __forceinline__ void state_store(float* p, const float* s) {
+  if constexpr (V == 4) __builtin_nontemporal_store(f32x4{s[0], s[1], s[2], s[3]}, reinterpret_cast<f32x4*>(p));
+  else __builtin_nontemporal_store(s[0], p);
 }
 
 template <typename T, int V>
@@ -338,14 +365,14 @@ __global__ void __launch_bounds__(kStepThreads) k_decay_step(StepParams p) {
 #pragma unroll 4
       for (int d = lr; d < hd; d += rows) {
         float s[V];
-        vload<float, V>(S + d * hd + e, s);
+        state_load<V>(S + d * hd + e, s);
         const float kd = sk[d], qd = sq[d];
 #pragma unroll
         for (int x = 0; x < V; ++x) {
           s[x] = g * s[x] + kd * v[x];
           o[x] += qd * s[x];
         }
-        vstore<float, V>(S + d * hd + e, s);
+        state_store<V>(S + d * hd + e, s);
       }
 #pragma unroll
     for (int x = 0; x < V; ++x)
@@ -363,14 +390,19 @@ __global__ void __launch_bounds__(kStepThreads) k_decay_step(StepParams p) {
 
 // ------------------------------------------------------------------ launch --
 int decay_scan_launch(const DecayParams& p, int dp, hipStream_t s) {
-  const int64_t n = (int64_t)p.roles * p.batch * p.heads * dp * dp / 4;
-  const unsigned grid = (unsigned)((n + 255) / 256);
-  switch (dp) {
-    case 16: k_decay_scan<16><<<grid, 256, 0, s>>>(p); break;
-    case 32: k_decay_scan<32><<<grid, 256, 0, s>>>(p); break;
-    case 64: k_decay_scan<64><<<grid, 256, 0, s>>>(p); break;
-    default: k_decay_scan<128><<<grid, 256, 0, s>>>(p); break;
-  }
+  const int64_t n = (int64_t)p.roles * p.batch * p.heads * dp * dp;
+  auto run = [&](auto w) {
+    constexpr int DP = decltype(w)::value;
+    const unsigned one = (unsigned)((n + 255) / 256), four = (unsigned)((n / 4 + 255) / 256);
+    if (n >= 1 << 18) k_decay_scan<DP, 4, 8><<<four, 256, 0, s>>>(p);
+    else if (p.nseg <= 8) k_decay_scan<DP, 1, 8><<<one, 256, 0, s>>>(p);
+    else if (p.nseg <= 16) k_decay_scan<DP, 1, 16><<<one, 256, 0, s>>>(p);
+    else k_decay_scan<DP, 1, 32><<<one, 256, 0, s>>>(p);
+  };
+  if (dp == 16) run(std::integral_constant<int, 16>{});
+  else if (dp == 32) run(std::integral_constant<int, 32>{});
+  else if (dp == 64) run(std::integral_constant<int, 64>{});
+  else run(std::integral_constant<int, 128>{});
   GRK_LAUNCH_CHECK();
   return GRK_OK;
 }

@@ -1049,7 +1049,9 @@ class _RotaryFn(torch.autograd.Function):
     def backward(ctx, gy):
         positions, freqs = ctx.saved_tensors
         heads, layout, scale = ctx.meta
-        g = K.rotary(_head_mat(gy), positions, freqs, heads, layout, scale, inverse=True)
+        x = _head_mat(gy)
+        g = K.rotary_turn(x, positions, freqs, heads, layout, scale, True,
+                          torch.empty(x.shape, dtype=x.dtype, device=x.device))
         return (g if gy.dim() == 2 else g.view(gy.shape)), None, None, None, None, None
 
 

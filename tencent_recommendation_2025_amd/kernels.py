@@ -1263,7 +1263,7 @@ def rotary(x, positions, freqs, heads, layout='half', scale=1.0, inverse=False, 
     positions int32 / int64 [N]; freqs float64 [r] (rotary_frequencies); layout 'half'
     (columns i, i + r) or 'interleaved' (2 i, 2 i + 1).  inverse turns back.  out: x itself
     (in place) or a matrix that shares nothing with it; a new one by default."""
-    dev = _same_device(x, positions, freqs, out)
+    _same_device(x, positions, freqs, out)
     N, cols = x.shape if x.dim() == 2 else (-1, -1)
     if x.dim() != 2 or heads <= 0 or cols % heads or cols == 0:
         raise L.GrkError('x must be [N, heads * head_dim]')
@@ -1273,20 +1273,25 @@ def rotary(x, positions, freqs, heads, layout='half', scale=1.0, inverse=False, 
         raise L.GrkError('positions must be a contiguous int32 / int64 [N] tensor')
     if freqs.dtype != torch.float64 or freqs.dim() != 1 or not freqs.is_contiguous():
         raise L.GrkError('freqs must be a contiguous float64 [rotary_dim / 2] tensor')
-    dt = x.dtype
-    code = _row_code(dt)
-    xp, xl = _head_rows(x, 'x', N, cols, dt)
     if out is None:
-        out = torch.empty((N, cols), dtype=dt, device=x.device)
-        op, ol = out.data_ptr(), cols
-    else:
-        op, ol = _head_rows(out, 'out', N, cols, dt)
-        if op != xp or ol != xl:
-            _fresh(out, 'out', x)
+        out = torch.empty((N, cols), dtype=x.dtype, device=x.device)
+    elif out.data_ptr() != x.data_ptr() or out.stride(0) != x.stride(0):
+        _fresh(out, 'out', x)
+    _row_code(x.dtype)
+    return rotary_turn(x, positions, freqs, heads, layout, scale, inverse, out)
+
+
+def rotary_turn(x, positions, freqs, heads, layout, scale, inverse, out):
+    """rotary of positions and freqs that it has taken before (only x and out are looked at)."""
+    dev = _same_device(x, positions, out)
+    N, cols = out.shape
+    dt = x.dtype
+    xp, xl = _head_rows(x, 'x', N, cols, dt)
+    op, ol = _head_rows(out, 'out', N, cols, dt)
     with _on_device(dev):
-        rc = L.lib().grk_rotary(xp, xl, op, ol, code, positions.data_ptr(), L.itype_code(positions.dtype),
-                                freqs.data_ptr(), N, heads, cols // heads, 2 * freqs.shape[0],
-                                layout == 'interleaved', scale, bool(inverse), L.raw_stream(dev))
+        rc = L.lib().grk_rotary(xp, xl, op, ol, _ROW_DTYPES[dt], positions.data_ptr(),
+                                L.itype_code(positions.dtype), freqs.data_ptr(), N, heads, cols // heads,
+                                2 * freqs.shape[0], layout == 'interleaved', scale, inverse, L.raw_stream(dev))
     L.check(rc, 'grk_rotary')
     return out
 

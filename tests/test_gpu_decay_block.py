@@ -401,7 +401,7 @@ def test_decay_step_is_the_sequence(K, H, hd, dt):
     close(o, want.view(n, T, -1)[:, 0], u_of(dt) + 300 * 2.0 ** -24)
 
 
-@pytest.mark.parametrize('n', [7, 400])
+@pytest.mark.parametrize('n', [7, 400, 1500])
 def test_decay_step_slots_that_repeat_or_hold_nothing(K, n):
     """Events of one slot are taken in their order; a negative slot holds no event, one past
     the states sets the flag; both leave every state as it is."""
