@@ -8,76 +8,93 @@
 namespace grk {
 
 // ---------------------------------------------------------- general kernel --
-// One workgroup walks a segment chunk by chunk; wave w owns columns [16 w, 16 w + 16) of
-// the state (head_dim padded to DP with zeros: DP / 16 waves), its 16-row tiles in
-// registers.  v_mfma_f32_16x16x4_f32: lane l = 16 g + c holds A[c][g], B[g][c] and
-// D[4 g + i][c], i < 4.  The four k of a 16-deep step are taken as 4 g + s (s = 0..3)
-// instead of 4 s + g: then register s of a state tile IS the B operand of step s, and the
-// row-major A operands are one 16-byte LDS read.
-constexpr int kDecayPad = 4;   // floats after each LDS row: rows 4 apart fall 16 banks apart
+// One workgroup walks a segment in chunks of 32 steps; wave w owns columns [16 w, 16 w + 16)
+// of the state and of the output (head_dim padded to DP with zeros: DP / 16 waves), its
+// 16-row tiles of the state in registers.  v_mfma_f32_16x16x4_f32: lane l = 16 g + c holds
+// A[c][g], B[g][c] and D[4 g + i][c], i < 4 -- A and B alike, so exchanging them transposes
+// D.  The four k of a 16-deep step are taken as 4 g + s (s = 0..3) instead of 4 s + g: then
+// register s of a state tile S = K^T V is the operand of step s in O^T = S^T Q^T + V^T P^T,
+// and the row-major operands are 16-byte LDS reads.  P^T and O^T come out with 4
+// neighbouring columns of one row in a lane (vector stores).
+//
+// Bound: the fp32 matrix instruction (1/16 of bf16's rate): of a 64-wide head a step takes
+// 16 K operations of the state and 6 K of its chunk -- 32 steps, not 64, keep the latter
+// small and leave LDS for 5 workgroups a CU.
+constexpr int kF32Chunk = 32;
+constexpr int kF32Pad = 4;   // floats after each LDS row: rows 4 apart fall 16 banks apart
 
 template <int DP> constexpr size_t decay_lds_f32(bool state_only) {
-  return (size_t)(state_only ? 2 : 3) * kDecayChunk * (DP + kDecayPad) * 4 +
-         (state_only ? 0 : (size_t)kDecayChunk * (kDecayChunk + kDecayPad) * 4);
+  return (size_t)((state_only ? 2 : 3) * kF32Chunk * (DP + kF32Pad) + (state_only ? 0 : kF32Chunk * (kF32Chunk + kF32Pad)) +
+                  16 + kF32Chunk + 4 + 2 * kF32Chunk) * 4;
 }
 
+// 4 elements of a row (or one, V = 1) as they lie in memory.
+template <typename T, int V> struct DecayRaw;
+template <> struct DecayRaw<float, 4> { typedef uint4 type; };
+template <> struct DecayRaw<bf16_t, 4> { typedef uint2 type; };
+template <> struct DecayRaw<f16_t, 4> { typedef uint2 type; };
+template <typename T> struct DecayRaw<T, 1> { typedef T type; };
+
+// A thread's part of a chunk on its way from memory: V columns of N rows.
 template <typename T, int V, int DP>
-__device__ __forceinline__ void decay_stage(const DecayParams& p, const DecayPlace& w, int rev, const void* src,
-                                            int64_t ld, int t0, float* dst) {
-  constexpr int ST = DP + kDecayPad, U = DP / (V > 4 ? 4 : V);   // 4-column units of a row (1 without vectors)
-  constexpr int W = DP / U;
-  for (int a = threadIdx.x; a < kDecayChunk * U; a += DP * 4) {
-    const int t = a / U, c = a % U * W;
-    const int64_t row = c < p.head_dim ? decay_row(p, w, rev, t0 + t) : -1;
-    float f[W];
+struct DecayRowsF32 {
+  typedef typename DecayRaw<T, V>::type raw;
+  static constexpr int NTH = DP * 4, U = DP / V, R = NTH / U, N = kF32Chunk / R;
+  int64_t row[N];   // -1: no event there
+  __device__ __forceinline__ void chunk(const DecayParams& p, const DecayPlace& w, int rev, int t0) {
 #pragma unroll
-    for (int e = 0; e < W; ++e) f[e] = 0.f;
-    if (row >= 0) {
-      const T* s = reinterpret_cast<const T*>(src) + row * ld + (int64_t)w.h * p.head_dim + c;
-      if constexpr (W == 1) {
-        f[0] = to_f32(*s);
-      } else if constexpr (sizeof(T) == 4) {
-        vload<T, 4>(s, f);
-      } else {
-        const uint2 x = *reinterpret_cast<const uint2*>(s);
-        T h[4];
-        __builtin_memcpy(h, &x, 8);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) f[e] = to_f32(h[e]);
-      }
-    }
-    if constexpr (W == 1) dst[t * ST + c] = f[0];
-    else *reinterpret_cast<float4*>(dst + t * ST + c) = make_float4(f[0], f[1], f[2], f[3]);
+    for (int k = 0; k < N; ++k) row[k] = decay_row(p, w, rev, t0 + (int)threadIdx.x / U + R * k);
   }
-}
-
-__device__ __forceinline__ f32x4 mfma4(float a, float b, f32x4 c) {
-  return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
-}
+  __device__ __forceinline__ void load(raw* f, const void* src, int64_t ld, int64_t hcol, int head_dim) const {
+    const int c = (int)threadIdx.x % U * V;
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      f[k] = raw{};
+      if (row[k] >= 0 && c < head_dim)
+        f[k] = *reinterpret_cast<const raw*>(reinterpret_cast<const T*>(src) + row[k] * ld + hcol + c);
+    }
+  }
+  __device__ __forceinline__ void store(const raw* f, float* dst) const {
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      T t[V];
+      __builtin_memcpy(t, &f[k], sizeof(raw));
+      float* d = dst + ((int)threadIdx.x / U + R * k) * (DP + kF32Pad) + (int)threadIdx.x % U * V;
+      if constexpr (V == 4) *reinterpret_cast<float4*>(d) = make_float4(to_f32(t[0]), to_f32(t[1]), to_f32(t[2]), to_f32(t[3]));
+      else *d = to_f32(t[0]);
+    }
+  }
+};
 
 // c += A B over 16 of the contraction: step s takes element s of both.
 __device__ __forceinline__ void mfma16(f32x4 a, f32x4 b, f32x4& c) {
 #pragma unroll
-  for (int s = 0; s < 4; ++s) c = mfma4(a[s], b[s], c);
+  for (int s = 0; s < 4; ++s) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[s], b[s], c, 0, 0, 0);
   mfma_keep(c, a, b);
 }
 
 template <typename T, int V, int DP, bool STATE>
-__global__ void __launch_bounds__(DP * 4) k_decay_f32(DecayParams p) {
-  constexpr int C = kDecayChunk, ST = DP + kDecayPad, PT = C + kDecayPad, NT = DP / 16;
+__global__ void __launch_bounds__(DP * 4, 4) k_decay_f32(DecayParams p) {
+  constexpr int C = kF32Chunk, ST = DP + kF32Pad, PT = C + kF32Pad, NT = DP / 16, NTH = DP * 4;
+  using Rows = DecayRowsF32<T, V, DP>;
   extern __shared__ __attribute__((aligned(16))) float sm[];
   float* sb = sm;
   float* sc = sb + C * ST;
   float* sa = sc + C * ST;
-  float* sp = sa + C * ST;
+  float* sp = sa + (STATE ? 0 : C * ST);
+  float* pw = sp + (STATE ? 0 : C * PT) + 16;   // scale g^n, 0 <= n <= C; 0 for -16 < n < 0
+  float* wv = pw - 16 + 16 + C + 4;             // g^(n-1-j): the weight of step j in the state
+  int* slive = reinterpret_cast<int*>(wv + C);  // the step holds an event
   const DecayPlace w = decay_place(p);
   if (!w.on) return;
   const DecayRole r = p.role[w.role];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, c = lane & 15;
-  const int64_t bh = (int64_t)w.b * p.heads + w.h;
-  const int col = 16 * wave + c;   // the state column (and output column) of this lane
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int g = lane >> 4, c = lane & 15;
+  const int64_t bh = (int64_t)w.b * p.heads + w.h, hcol = (int64_t)w.h * p.head_dim;
+  const int col = 16 * wave + c;   // the state column of this lane
   f32x4 st[NT];
   float* frag = p.ws + (((int64_t)w.role * p.batch * p.heads + bh) * p.nseg + w.seg) * DP * DP;
+  bool some = STATE || (p.nseg > 1 ? w.seg > 0 || p.state_in : p.state_in != nullptr);   // the state is not all 0
 #pragma unroll
   for (int dt = 0; dt < NT; ++dt) {
     st[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -93,69 +110,123 @@ __global__ void __launch_bounds__(DP * 4) k_decay_f32(DecayParams p) {
       }
     }
   }
-  if (!STATE) decay_zero_rows<T>(p, w, r);
+  Rows rows;
+  typename Rows::raw fa[Rows::N], fb[Rows::N], fc[Rows::N];
+  if (w.t0 < w.t1) {
+    rows.chunk(p, w, r.rev, w.t0);
+    rows.load(fb, r.b, r.ldb, hcol, p.head_dim);
+    rows.load(fc, r.c, r.ldc, hcol, p.head_dim);
+    if (!STATE) rows.load(fa, r.a, r.lda, hcol, p.head_dim);
+  }
+  if (!STATE) {
+    for (int n = threadIdx.x; n <= 16 + C; n += NTH) pw[n - 16] = n < 16 ? 0.f : p.scale * decay_pow(w.lg, n - 16);
+    decay_zero_rows<T>(p, w, r);
+  }
+  auto weights = [&](int n) {
+    for (int j = threadIdx.x; j < C; j += NTH) wv[j] = j < n ? decay_pow(w.lg, n - 1 - j) : 0.f;
+  };
+  weights(C);
+  const float gc = decay_pow(w.lg, C);
+  // A chunk: its rows to LDS | P, what the output takes from the state, the state's step |
+  // the output.  Behind the second barrier only P (and V, kept in registers) is read.
   for (int t0 = w.t0; t0 < w.t1; t0 += C) {
     const int n = w.t1 - t0 < C ? w.t1 - t0 : C;
-    __syncthreads();
-    decay_stage<T, V, DP>(p, w, r.rev, r.b, r.ldb, t0, sb);
-    decay_stage<T, V, DP>(p, w, r.rev, r.c, r.ldc, t0, sc);
-    if (!STATE) decay_stage<T, V, DP>(p, w, r.rev, r.a, r.lda, t0, sa);
-    __syncthreads();
+    const bool last = t0 + C >= w.t1;
+    rows.store(fb, sb);
+    rows.store(fc, sc);
     if constexpr (!STATE) {
-      // P: the 10 tiles on and below the diagonal, shared out over the waves
-      for (int tile = wave; tile < 10; tile += NT) {
-        int it = 0, jt = tile;
-        while (jt > it) { jt -= it + 1; ++it; }
-        f32x4 x = {0.f, 0.f, 0.f, 0.f};
+      rows.store(fa, sa);
+      if ((int)threadIdx.x % Rows::U == 0) {
 #pragma unroll
-        for (int dt = 0; dt < NT; ++dt) {
-          mfma16(*reinterpret_cast<const f32x4*>(sa + (16 * it + c) * ST + 16 * dt + 4 * g),
-                 *reinterpret_cast<const f32x4*>(sb + (16 * jt + c) * ST + 16 * dt + 4 * g), x);
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int lag = 16 * (it - jt) + 4 * g + i - c;
-          sp[(16 * it + 4 * g + i) * PT + 16 * jt + c] = lag >= 0 ? x[i] * decay_pow(w.lg, lag) : 0.f;
-        }
+        for (int k = 0; k < Rows::N; ++k) slive[(int)threadIdx.x / Rows::U + Rows::R * k] = rows.row[k] >= 0;
       }
-      __syncthreads();
-#pragma unroll
-      for (int it = 0; it < C / 16; ++it) {
+    }
+    __syncthreads();
+    if (!last) {
+      rows.chunk(p, w, r.rev, t0 + C);
+      rows.load(fb, r.b, r.ldb, hcol, p.head_dim);
+      rows.load(fc, r.c, r.ldc, hcol, p.head_dim);
+      if (!STATE) rows.load(fa, r.a, r.lda, hcol, p.head_dim);
+    }
+    if constexpr (!STATE) {
+      for (int tile = wave; tile < 3; tile += NT) {   // P^T, tiles (0, 0), (1, 0), (1, 1)
+        const int it = tile > 0, jt = tile > 1;
         f32x4 x = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int dt = 0; dt < NT; ++dt) {
-          mfma16(*reinterpret_cast<const f32x4*>(sa + (16 * it + c) * ST + 16 * dt + 4 * g), st[dt], x);
-        }
+        for (int dt = 0; dt < NT; ++dt)
+          mfma16(*reinterpret_cast<const f32x4*>(sb + (16 * jt + c) * ST + 16 * dt + 4 * g),
+                 *reinterpret_cast<const f32x4*>(sa + (16 * it + c) * ST + 16 * dt + 4 * g), x);
+        const float* lag = pw + 16 * (it - jt) + c - 4 * g;
+        *reinterpret_cast<f32x4*>(sp + (16 * it + c) * PT + 16 * jt + 4 * g) =
+            f32x4{x[0] * lag[0], x[1] * lag[-1], x[2] * lag[-2], x[3] * lag[-3]};
+      }
+    }
+    f32x4 v[2];   // V[16 jt + 4 g + s][col]
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] *= decay_pow(w.lg, 16 * it + 4 * g + i + 1);
-        for (int jt = 0; jt <= it; ++jt) {
-          const float* b = sc + (16 * jt + 4 * g) * ST + col;
-          mfma16(*reinterpret_cast<const f32x4*>(sp + (16 * it + c) * PT + 16 * jt + 4 * g),
-                 f32x4{b[0], b[ST], b[2 * ST], b[3 * ST]}, x);
-        }
+    for (int jt = 0; jt < 2; ++jt) {
+      const float* q = sc + (16 * jt + 4 * g) * ST + col;
+      v[jt] = f32x4{q[0], q[ST], q[2 * ST], q[3 * ST]};
+    }
+    f32x4 o[2];
+    bool live[2];
+    if constexpr (!STATE) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          bool live;
-          const int64_t row = decay_out_row(p, w, r.rev, t0 + 16 * it + 4 * g + i, &live);
-          if (row >= 0 && col < p.head_dim)
-            reinterpret_cast<T*>(r.out)[row * r.ldo + (int64_t)w.h * p.head_dim + col] =
-                from_f32<T>(live ? p.scale * x[i] : 0.f);
+      for (int it = 0; it < 2; ++it) {
+        live[it] = slive[16 * it + c];
+        o[it] = f32x4{0.f, 0.f, 0.f, 0.f};
+        if (some) {
+#pragma unroll
+          for (int dt = 0; dt < NT; ++dt)
+            mfma16(st[dt], *reinterpret_cast<const f32x4*>(sa + (16 * it + c) * ST + 16 * dt + 4 * g), o[it]);
+          o[it] *= pw[16 * it + c + 1];
         }
       }
     }
-    const float gn = decay_pow(w.lg, n);
+    if (STATE || !last || (p.nseg == 1 && p.state_out)) {   // (nothing reads the state behind the last chunk else)
+      some = true;
+      float gn = gc;
+      if (n < C) {   // the last chunk only
+        weights(n);
+        __syncthreads();
+        gn = decay_pow(w.lg, n);
+      }
 #pragma unroll
-    for (int dt = 0; dt < NT; ++dt) st[dt] *= gn;
+      for (int dt = 0; dt < NT; ++dt) st[dt] *= gn;
 #pragma unroll
-    for (int jt = 0; jt < C / 16; ++jt) {
-      const int j0 = 16 * jt + 4 * g;
-      f32x4 v;
+      for (int jt = 0; jt < 2; ++jt) {
+        const f32x4 y = v[jt] * *reinterpret_cast<const f32x4*>(wv + 16 * jt + 4 * g);
 #pragma unroll
-      for (int s = 0; s < 4; ++s) v[s] = j0 + s < n ? sc[(j0 + s) * ST + col] * decay_pow(w.lg, n - 1 - j0 - s) : 0.f;
+        for (int dt = 0; dt < NT; ++dt) {
+          const float* k = sb + (16 * jt + 4 * g) * ST + 16 * dt + c;
+          mfma16(f32x4{k[0], k[ST], k[2 * ST], k[3 * ST]}, y, st[dt]);
+        }
+      }
+    }
+    __syncthreads();
+    if constexpr (!STATE) {
 #pragma unroll
-      for (int dt = 0; dt < NT; ++dt) {
-        const float* k = sb + j0 * ST + 16 * dt + c;
-        mfma16(f32x4{k[0], k[ST], k[2 * ST], k[3 * ST]}, v, st[dt]);
+      for (int it = 0; it < 2; ++it) {
+#pragma unroll
+        for (int jt = 0; jt <= it; ++jt)
+          mfma16(v[jt], *reinterpret_cast<const f32x4*>(sp + (16 * it + c) * PT + 16 * jt + 4 * g), o[it]);
+        bool event;
+        const int64_t row = decay_out_row(p, w, r.rev, t0 + 16 * it + c, &event);
+        const int e = 16 * wave + 4 * g;
+        if (row >= 0 && e < p.head_dim) {
+          T* dst = reinterpret_cast<T*>(r.out) + row * r.ldo + hcol + e;
+          T y[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) y[i] = from_f32<T>(live[it] ? o[it][i] : 0.f);
+          if constexpr (V == 4) {
+            typename Rows::raw z;
+            __builtin_memcpy(&z, y, sizeof(z));
+            *reinterpret_cast<typename Rows::raw*>(dst) = z;
+          } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (e + i < p.head_dim) dst[i] = y[i];
+          }
+        }
       }
     }
   }
@@ -483,12 +554,13 @@ static int decay_run(const DecayParams& p, hipStream_t s) {
 
 static int decay_launch(const DecayParams& p, int dtype, hipStream_t s) {
   if (dtype == GRK_BF16 && decay_bf16_takes(p)) return decay_bf16_launch(p, s);
-  // 8- or 16-byte loads of 4 columns: rows and heads start on them
+  // 8- or 16-byte accesses of 4 columns: rows and heads start on them
   bool vec = p.head_dim % 4 == 0;
   const size_t b4 = 4 * dtype_size(dtype);
   for (int r = 0; r < p.roles; ++r) {
     const DecayRole& x = p.role[r];
-    vec = vec && ((uintptr_t)x.a | (uintptr_t)x.b | (uintptr_t)x.c) % b4 == 0 && (x.lda | x.ldb | x.ldc) % 4 == 0;
+    vec = vec && ((uintptr_t)x.a | (uintptr_t)x.b | (uintptr_t)x.c | (uintptr_t)x.out) % b4 == 0 &&
+          (x.lda | x.ldb | x.ldc | x.ldo) % 4 == 0;
   }
   return for_dtype(dtype, [&](auto t) {
     using T = decltype(t);
