@@ -44,21 +44,23 @@ struct DecayParams {
 
 // One workgroup's pass: a role, a (sequence, head) and a segment of it.
 struct DecayPlace {
-  int b, h, seg, role;
+  int b, h, seg, role, part;       // part: its columns of the state and the output, where they are shared out
   int start, len;                  // first position of the sequence, its steps
   int t0, t1;                      // steps of the segment
   float lg;                        // log g <= 0
   bool on;
 };
 
-// Workgroups of the roles of one (sequence, head, segment) read the same rows: their
+// Workgroups of the roles and parts of one (sequence, head, segment) read the same rows: their
 // indices differ by multiples of 8, so one XCD's L2 serves them (workgroups go round the
 // 8 XCDs in order).
-__device__ __forceinline__ DecayPlace decay_place(const DecayParams& p) {
+__device__ __forceinline__ DecayPlace decay_place(const DecayParams& p, int parts = 1) {
   DecayPlace w;
   const int64_t gid = blockIdx.x;
-  w.role = (int)((gid / 8) % p.roles);
-  const int64_t u = gid / (8 * p.roles) * 8 + gid % 8;
+  const int same = p.roles * parts, k = (int)((gid / 8) % same);
+  w.role = k % p.roles;
+  w.part = k / p.roles;
+  const int64_t u = gid / (8 * same) * 8 + gid % 8;
   w.on = u < (int64_t)p.batch * p.heads * p.nseg;
   const int64_t bh = w.on ? u / p.nseg : 0;
   w.seg = (int)(u - bh * p.nseg);

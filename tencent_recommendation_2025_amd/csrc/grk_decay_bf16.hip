@@ -1,8 +1,8 @@
 // Decayed linear attention of bf16 rows on the bf16 matrix instruction, for gfx950 (the
 // formulas: grk_decay.h; heads and rows made of 16-byte vectors).
 //
-// A workgroup walks a segment in chunks of 64 steps; each wave owns NE tiles of 16 columns
-// of the state and of the output.  v_mfma_f32_16x16x32_bf16: lane
+// A workgroup walks a segment in chunks of 64 steps with EW columns of the state (and of the
+// output); each wave owns NE tiles of 16 of them.  v_mfma_f32_16x16x32_bf16: lane
 // l = 16 g + c holds A[c][8 g + s] and B[8 g + s][c], s < 8, and D[4 g + i][c], i < 4 -- A
 // and B fragments are laid out alike, so exchanging them transposes D.  What is stored
 // comes out transposed on purpose: P^T = K Q^T and O^T = V^T P^T + S^T Q^T leave 4
@@ -21,6 +21,8 @@
 // takes every second row (4 rows 8 banks apart) has no conflicts either.  So the
 // contraction over the 64 steps takes each 8 of them in the order 0 2 4 6 1 3 5 7 ("slots"):
 // P and the weights of the state's sum are laid down in that order.
+#include <type_traits>
+
 #include "grk_decay.h"
 #include "grk_mfma.h"
 
@@ -33,8 +35,8 @@ constexpr int kDecayPowers = 16 + kDecayChunk + 4;
 template <int DP> constexpr int decay_stride() { return DP * 2 + 16; }   // bytes of an LDS row
 constexpr int kDecayPStride = decay_stride<kDecayChunk>();
 
-template <int DP> constexpr size_t decay_lds_bf16(bool state_only) {
-  return (size_t)(state_only ? 2 : 3) * kDecayChunk * decay_stride<DP>() +
+template <int DP, int EW> constexpr size_t decay_lds_bf16(bool state_only) {
+  return (size_t)kDecayChunk * ((state_only ? 1 : 2) * decay_stride<DP>() + decay_stride<EW>()) +
          (state_only ? 0 : kDecayChunk * kDecayPStride) + (kDecayPowers + 2 * kDecayChunk) * 4;
 }
 
@@ -125,23 +127,26 @@ struct DecayRows {
   }
 };
 
-// NS: bf16 parts of g^(n-1-j) v_j in the state's sum.  1 where the state only feeds bf16
-// outputs (it is rounded to bf16 as their operand anyway); 3 (all 24 bits of the fp32
-// value) where it is returned in fp32.
-template <int DP, int NE, int NS, bool STATE>
-__global__ void __launch_bounds__(DP * 4 / NE, NE == 1 ? 4 : 2) k_decay_bf16(DecayParams p) {
-  constexpr int C = kDecayChunk, NT = DP / 16, KS = DP / 32, NW = NT / NE, NTH = NW * 64;
-  constexpr int ST = decay_stride<DP>(), PS = kDecayPStride;
-  using Rows = DecayRows<DP, NTH>;
+// NS: bf16 parts of g^(n-1-j) v_j in the state's sum: 2 (16 bits; the state is rounded to
+// bf16 only as an operand of the output) or, where the state is returned in fp32, 3 (all 24
+// bits).  One part would cost 2 % (heads of 64) to 10 % (128) less time and put a third
+// rounding of 2^-9 into every output, which then lay 1.6 times as far from the exact one as
+// its own rounding; with two it is 1.4 times.
+template <int DP, int EW, int NE, int NS, bool STATE>
+__global__ void __launch_bounds__(EW * 4 / NE, NE == 1 ? 4 : 2) k_decay_bf16(DecayParams p) {
+  constexpr int C = kDecayChunk, NT = DP / 16, KS = DP / 32, NW = EW / 16 / NE, NTH = NW * 64;
+  constexpr int ST = decay_stride<DP>(), SE = decay_stride<EW>(), PS = kDecayPStride;
+  using Rows = DecayRows<DP, NTH>;    // of a and b
+  using Cols = DecayRows<EW, NTH>;    // of c
   extern __shared__ __attribute__((aligned(16))) char lds[];
   char* sb = lds;
   char* sc = sb + C * ST;
-  char* sa = sc + C * ST;
+  char* sa = sc + C * SE;
   char* sp = sa + (STATE ? 0 : C * ST);
   float* pw = reinterpret_cast<float*>(sp + (STATE ? 0 : C * PS)) + 16;
   float* wv = pw - 16 + kDecayPowers;
   int* slive = reinterpret_cast<int*>(wv + C);
-  DecayPlace w = decay_place(p);
+  DecayPlace w = decay_place(p, DP / EW);
   if (!w.on) return;
   const DecayRole r = p.role[w.role];
   const int64_t bh = (int64_t)w.b * p.heads + w.h, hcol = (int64_t)w.h * p.head_dim;
@@ -151,15 +156,15 @@ __global__ void __launch_bounds__(DP * 4 / NE, NE == 1 ? 4 : 2) k_decay_bf16(Dec
   const int g = lane >> 4, c = lane & 15;
   // (a range that grk_seq_ranges calls contiguous leaves nothing to mask)
   const bool masked = p.key_valid && !(p.seq_range && p.seq_range[3 * (int64_t)w.b + 1] == 1);
-  const int ccol = (int)threadIdx.x % (DP / 8) * 8;      // this thread's columns when rows are moved
-  const bool has = ccol < p.head_dim;
-  const int mcol = has ? ccol : 0;
+  const int rcol = (int)threadIdx.x % (DP / 8) * 8, ecol = w.part * EW + (int)threadIdx.x % (EW / 8) * 8;
+  const bool has = rcol < p.head_dim, ehas = ecol < p.head_dim;   // this thread's columns when rows are moved
+  const int et0 = w.part * (EW / 16) + NE * wave;                 // the wave's first column tile
   f32x4 st[NE][NT];
   float* frag = p.ws + (((int64_t)(w.role < 2 ? w.role : 1) * p.batch * p.heads + bh) * p.nseg + w.seg) * DP * DP;
   bool some = STATE || (p.nseg > 1 ? w.seg > 0 || p.state_in : p.state_in != nullptr);   // the state is not all 0
 #pragma unroll
   for (int x = 0; x < NE; ++x) {
-    const int et = NE * wave + x;   // the wave's column tiles
+    const int et = et0 + x;
 #pragma unroll
     for (int dt = 0; dt < NT; ++dt) {
       st[x][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -181,13 +186,20 @@ __global__ void __launch_bounds__(DP * 4 / NE, NE == 1 ? 4 : 2) k_decay_bf16(Dec
     }
   }
   Rows rows;
-  uint4 fa[Rows::N], fb[Rows::N], fc[Rows::N];
-  if (w.t0 < w.t1) {
-    rows.chunk(p, w, r.rev, base, masked, w.t0);
-    rows.load(fb, r.b, r.ldb, hcol, mcol);
-    rows.load(fc, r.c, r.ldc, hcol, mcol);
-    if (!STATE) rows.load(fa, r.a, r.lda, hcol, mcol);
-  }
+  Cols cols;
+  uint4 fa[Rows::N], fb[Rows::N], fc[Cols::N];
+  auto fetch = [&](int t0) {
+    rows.chunk(p, w, r.rev, base, masked, t0);
+    rows.load(fb, r.b, r.ldb, hcol, has ? rcol : 0);
+    if (!STATE) rows.load(fa, r.a, r.lda, hcol, has ? rcol : 0);
+    if constexpr (EW == DP) {
+      cols = rows;
+    } else {
+      cols.chunk(p, w, r.rev, base, masked, t0);
+    }
+    cols.load(fc, r.c, r.ldc, hcol, ehas ? ecol : 0);
+  };
+  if (w.t0 < w.t1) fetch(w.t0);
   if (!STATE)
     for (int n = threadIdx.x; n <= 16 + C; n += NTH) pw[n - 16] = n < 16 ? 0.f : p.scale * decay_pow(w.lg, n - 16);
   auto weights = [&](int n) {   // of a chunk of n steps, by slot
@@ -200,7 +212,7 @@ __global__ void __launch_bounds__(DP * 4 / NE, NE == 1 ? 4 : 2) k_decay_bf16(Dec
   const float gc = decay_pow(w.lg, C);
   if constexpr (!STATE) {
     for (int n = threadIdx.x; n < C * PS / 16; n += NTH) reinterpret_cast<uint4*>(sp)[n] = make_uint4(0u, 0u, 0u, 0u);
-    decay_zero_rows<bf16_t>(p, w, r);
+    if (w.part == 0) decay_zero_rows<bf16_t>(p, w, r);
   }
   const int row_b = c * ST + 16 * g, col_b = decay_col_base<ST>(lane);   // this lane's LDS bases
   // A chunk: its rows to LDS | P, what the output takes from the state, the state's step |
@@ -210,22 +222,17 @@ __global__ void __launch_bounds__(DP * 4 / NE, NE == 1 ? 4 : 2) k_decay_bf16(Dec
     const int n = w.t1 - t0 < C ? w.t1 - t0 : C;
     const bool last = t0 + C >= w.t1;
     rows.store(fb, sb, has);
-    rows.store(fc, sc, has);
+    cols.store(fc, sc, ehas);
     if constexpr (!STATE) {
       rows.store(fa, sa, has);
-      if (ccol == 0) {
+      if (rcol == 0) {
 #pragma unroll
         for (int k = 0; k < Rows::N; ++k) slive[decay_first_row<DP>() + Rows::R * k] = rows.live[k];
       }
     }
     const int64_t low = rows.low;
     __syncthreads();
-    if (!last) {
-      rows.chunk(p, w, r.rev, base, masked, t0 + C);
-      rows.load(fb, r.b, r.ldb, hcol, mcol);
-      rows.load(fc, r.c, r.ldc, hcol, mcol);
-      if (!STATE) rows.load(fa, r.a, r.lda, hcol, mcol);
-    }
+    if (!last) fetch(t0 + C);
     if constexpr (!STATE) {
       // P^T, lower tiles; the tiles above the diagonal that a 32-deep step reads stay 0
       for (int tile = wave; tile < 10; tile += NW) {
@@ -248,7 +255,7 @@ __global__ void __launch_bounds__(DP * 4 / NE, NE == 1 ? 4 : 2) k_decay_bf16(Dec
 #pragma unroll
     for (int x = 0; x < NE; ++x)
 #pragma unroll
-      for (int ks = 0; ks < 2; ++ks) vf[x][ks] = lds_col8s<ST>(sc + col_b + 32 * ks * ST + 32 * (NE * wave + x));
+      for (int ks = 0; ks < 2; ++ks) vf[x][ks] = lds_col8s<SE>(sc + decay_col_base<SE>(lane) + 32 * ks * SE + 32 * (NE * wave + x));
     f32x4 o[C / 16][NE];
     bool live[C / 16];
     if constexpr (!STATE) {
@@ -315,9 +322,9 @@ __global__ void __launch_bounds__(DP * 4 / NE, NE == 1 ? 4 : 2) k_decay_bf16(Dec
         for (int dt = 0; dt < NT; ++dt) {
           const bf16x8 k = lds_col8s<ST>(sb + col_b + 32 * ks * ST + 32 * dt);
 #pragma unroll
-          for (int x = 0; x < NE; ++x)
+          for (int q = NS - 1; q >= 0; --q)
 #pragma unroll
-            for (int q = NS - 1; q >= 0; --q) mfma32(k, part[x][q], st[x][dt]);
+            for (int x = 0; x < NE; ++x) mfma32(k, part[x][q], st[x][dt]);
         }
       }
     }
@@ -337,7 +344,7 @@ __global__ void __launch_bounds__(DP * 4 / NE, NE == 1 ? 4 : 2) k_decay_bf16(Dec
           const unsigned at = (unsigned)(r.rev ? n - 1 - t : t) * (unsigned)r.ldo;
 #pragma unroll
           for (int x = 0; x < NE; ++x) {
-            const int e = 16 * (NE * wave + x) + 4 * g;
+            const int e = 16 * (et0 + x) + 4 * g;
             const f32x4 v = o[it][x];
             const bf16x4 y = {(__bf16)v[0], (__bf16)v[1], (__bf16)v[2], (__bf16)v[3]};
             const uint2 z = live[it] ? __builtin_bit_cast(uint2, y) : make_uint2(0u, 0u);
@@ -351,7 +358,7 @@ __global__ void __launch_bounds__(DP * 4 / NE, NE == 1 ? 4 : 2) k_decay_bf16(Dec
   for (int x = 0; x < NE; ++x)
 #pragma unroll
     for (int dt = 0; dt < NT; ++dt) {
-      const int et = NE * wave + x;
+      const int et = et0 + x;
       if (STATE) {
         *reinterpret_cast<f32x4*>(frag + ((dt * NT + et) * 64 + lane) * 4) = st[x][dt];
       } else if (p.nseg == 1 && p.state_out) {
@@ -369,33 +376,32 @@ __global__ void __launch_bounds__(DP * 4 / NE, NE == 1 ? 4 : 2) k_decay_bf16(Dec
 template <int DP, int NE>
 static int decay_bf16_run(const DecayParams& p, hipStream_t s) {
   const int64_t groups = ((int64_t)p.batch * p.heads * p.nseg + 7) / 8 * 8;
-  const unsigned grid = (unsigned)(groups * p.roles);
+  auto launch = [&](auto ew, auto ne, auto ns, auto state, const DecayParams& q) -> int {
+    constexpr int EW = decltype(ew)::value, E = decltype(ne)::value, NS = decltype(ns)::value;
+    constexpr bool STATE = decltype(state)::value;
+    constexpr size_t lds = decay_lds_bf16<DP, EW>(STATE);
+    GRK_CHECK_HIP(ensure_dynamic_lds((const void*)k_decay_bf16<DP, EW, E, NS, STATE>, lds));
+    const unsigned grid = (unsigned)(groups * (DP / EW) * q.roles);
+    k_decay_bf16<DP, EW, E, NS, STATE><<<grid, EW * 4 / E, lds, s>>>(q);
+    GRK_LAUNCH_CHECK();
+    return GRK_OK;
+  };
+  typedef std::integral_constant<int, 1> one;
+  typedef std::integral_constant<int, 2> two;
+  typedef std::integral_constant<int, 3> three;
+  typedef std::integral_constant<int, DP> whole;
+  typedef std::integral_constant<int, NE> ne;
+  typedef std::integral_constant<int, (DP < 64 ? DP : 64)> half;   // (of a head of 128)
   if (p.nseg > 1) {
     DecayParams q = p;
     q.roles = p.roles < 2 ? p.roles : 2;
-    const unsigned sgrid = (unsigned)(groups * q.roles);
-    constexpr size_t lds = decay_lds_bf16<DP>(true);
-    if (p.state_out) {
-      GRK_CHECK_HIP(ensure_dynamic_lds((const void*)k_decay_bf16<DP, NE, 3, true>, lds));
-      k_decay_bf16<DP, NE, 3, true><<<sgrid, DP * 4 / NE, lds, s>>>(q);
-    } else {
-      GRK_CHECK_HIP(ensure_dynamic_lds((const void*)k_decay_bf16<DP, NE, 1, true>, lds));
-      k_decay_bf16<DP, NE, 1, true><<<sgrid, DP * 4 / NE, lds, s>>>(q);
-    }
-    GRK_LAUNCH_CHECK();
-    const int rc = decay_scan_launch(q, DP, s);
-    if (rc) return rc;
+    int rc = p.state_out ? launch(half{}, one{}, three{}, std::true_type{}, q)
+                         : launch(half{}, one{}, two{}, std::true_type{}, q);
+    if (rc || (rc = decay_scan_launch(q, DP, s))) return rc;
+    return launch(whole{}, ne{}, two{}, std::false_type{}, p);
   }
-  constexpr size_t lds = decay_lds_bf16<DP>(false);
-  if (p.nseg == 1 && p.state_out) {
-    GRK_CHECK_HIP(ensure_dynamic_lds((const void*)k_decay_bf16<DP, NE, 3, false>, lds));
-    k_decay_bf16<DP, NE, 3, false><<<grid, DP * 4 / NE, lds, s>>>(p);
-  } else {
-    GRK_CHECK_HIP(ensure_dynamic_lds((const void*)k_decay_bf16<DP, NE, 1, false>, lds));
-    k_decay_bf16<DP, NE, 1, false><<<grid, DP * 4 / NE, lds, s>>>(p);
-  }
-  GRK_LAUNCH_CHECK();
-  return GRK_OK;
+  return p.state_out ? launch(whole{}, ne{}, three{}, std::false_type{}, p)
+                     : launch(whole{}, ne{}, two{}, std::false_type{}, p);
 }
 
 // Whole 16-byte vectors: rows, strides and heads start on them (8 bytes for the output);
