@@ -287,9 +287,14 @@ static void hn_tile(const HNShape& s, HNParams& p) {
   p.rows_per_iter = groups / p.head_tile;
 }
 
+// Row blocks of a backward: each writes its partial weight gradients, so few rows take one
+// workgroup a CU and no more until each has 4 turns.
 static int hn_bwd_blocks(int64_t rows, int rows_per_iter) {
-  const int64_t b = (rows + rows_per_iter - 1) / rows_per_iter;
-  return (int)(b < kHnBwdBlocks ? b : kHnBwdBlocks);
+  const int64_t turns = (rows + rows_per_iter - 1) / rows_per_iter;
+  int64_t b = turns / 4;
+  if (b > kHnBwdBlocks) b = kHnBwdBlocks;
+  if (b < 256) b = turns < 256 ? turns : 256;
+  return (int)b;
 }
 
 template <typename T, int V, int LPG, int VPL>
@@ -359,7 +364,7 @@ extern "C" int grk_head_norm_fwd(const void* x, int64_t ldx, const void* gate, i
 
 extern "C" size_t grk_head_norm_bwd_workspace(int64_t rows, int heads, int head_dim) {
   if (rows <= 0 || heads <= 0 || head_dim <= 0) return 0;
-  // a workgroup walks one row at a time at least
+  // a workgroup walks one row at a time at least: no fewer blocks than any launch takes
   return (size_t)hn_bwd_blocks(rows, 1) * 2 * (size_t)heads * head_dim * sizeof(float);
 }
 
