@@ -624,7 +624,10 @@ int grk_rotary(const void* x, int64_t ldx, void* y, int64_t ldy, int dtype, cons
  * Positions with key_valid 0 hold no event: their q / k / v are not read (whatever
  * they hold), their output and gradient rows are zero, and the state decays over
  * them.  seq_range (int32 [batch, 3], grk_seq_ranges; optional): the same for the
- * positions before seq_range[b][0], without reading key_valid there.
+ * positions before seq_range[b][0], without reading key_valid there; it has to be this
+ * key_valid's (a range it calls contiguous is taken to have no holes behind its start).
+ * A NaN or an infinity in an event reaches the outputs behind it, and may reach those
+ * of up to 63 events before it.
  * row_base / num_rows / capacity: the packed rows of grk_attn_args (seq_range
  * required; rows [*num_rows, capacity) of every output are zeroed); else the rows are
  * [batch * seq_len].

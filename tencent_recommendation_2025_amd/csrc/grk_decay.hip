@@ -513,6 +513,7 @@ static int decay_check(const grk_decay_args* a) {
     set_error("head_dim must be in [1, 128]");
     return GRK_EUNSUPPORTED;
   }
+  GRK_CHECK_ARG(a->batch > 0 || !a->row_base || a->capacity == 0, "packed rows without a sequence: capacity must be 0");
   GRK_CHECK_ARG((int64_t)a->batch * a->heads < (1 << 21) && a->seq_len < (1 << 30),
                 "batch * heads must be below 2^21 and seq_len below 2^30");
   return GRK_OK;

@@ -169,18 +169,9 @@ def _valid_bytes(token_type):
     return kv.to(torch.uint8) if torch.compiler.is_compiling() else kv.view(torch.uint8)
 
 
-_ROW_POSITIONS = {}
-
-
 def _row_positions(B, T, device):
-    """Cached int32 [B * T]: the position of each row of a [B, T] batch."""
-    key = (int(B), int(T), str(device))
-    p = _ROW_POSITIONS.get(key)
-    if p is None:
-        if len(_ROW_POSITIONS) > 64:
-            _ROW_POSITIONS.clear()
-        p = _ROW_POSITIONS[key] = torch.arange(T, dtype=torch.int32).repeat(B).to(device)
-    return p
+    """int32 [B * T]: the position of each row of a [B, T] batch."""
+    return torch.arange(T, dtype=torch.int32, device=device).repeat(B)
 
 
 _UNIT_ROWS = {}
@@ -964,6 +955,8 @@ class BaselineModel(torch.nn.Module):
         else:
             key_valid = _valid_bytes(mask.to(dev, non_blocking=True))
             kw = dict(key_valid=key_valid, seq_range=torch.ops.grk.seq_ranges(key_valid))  # one launch serves every layer
+            if self.rotary:
+                kw['positions'] = _row_positions(B, T, dev)
         if timestamps is not None and self.block == 'hstu':
             kw['timestamps'] = timestamps.to(dev, torch.int64, non_blocking=True).contiguous()
         if self.block in ('hstu', 'decay'):

@@ -51,9 +51,9 @@ def test_decay_attn_refusals(lib):
     for kw, word in ((dict(dtype=9), 'dtype'), (dict(batch=-1), 'batch'), (dict(heads=0), 'heads'),
                      (dict(seq_len=-1), 'seq_len'), (dict(q=None), 'q required'), (dict(ldk=127), 'k: row stride'),
                      (dict(log_decay=None), 'log_decay'), (dict(row_base=P), 'seq_range'),
-                     (dict(batch=1 << 21), '2^21')):
+                     (dict(batch=1 << 21), '2^21'), (dict(batch=0, row_base=P, seq_range=P, capacity=3), 'capacity')):
         for f in (fwd, bwd):
-            if 'row_base' in kw:
+            if 'row_base' in kw and 'capacity' not in kw:
                 kw = dict(kw, capacity=10)
             assert f(args(**kw)) == L.GRK_EINVAL and word in err(lib), (kw, err(lib))
     assert fwd(args(head_dim=129, ldq=300, ldk=300, ldv=300)) == L.GRK_EUNSUPPORTED and '128' in err(lib)

@@ -154,6 +154,68 @@ def test_softmax_attention_with_rotary():
 
 # ---------------------------------------------------------------- the model ----
 @pytest.mark.parametrize('block', ['decay', 'softmax'])
+def test_compiled_model_under_fp16_autocast(block):
+    """torch.compile(model) under fp16 autocast with a GradScaler: the operators run outside
+    the compiled graphs; logits and gradients follow the eager ones (fp16: u = 2^-11, about
+    16 roundings a layer and the compiler's own order of sums)."""
+    res = []
+    for compiled in (False, True):
+        torch._dynamo.reset()
+        m, batch, _ = make(block)
+        m.train()
+        model = torch.compile(m) if compiled else m
+        scaler = torch.amp.GradScaler('cuda')
+        with torch.amp.autocast('cuda'):
+            p, n = model(*batch[:9])
+            ntt = batch[4] == 1
+            loss = F.softplus(-p[ntt].float()).mean() + F.softplus(n[ntt].float()).mean()
+        scaler.scale(loss).backward()
+        res.append((p.detach().float(), {k: w.grad.float() for k, w in m.named_parameters() if w.grad is not None}))
+    (pe, ge), (pc, gc) = res
+    assert nrel(pc, pe) < 32 * 2.0 ** -11 and set(ge) == set(gc)
+    for k in ge:
+        # softmax scores do not change with the keys' bias: its gradient is rounding alone
+        if k.startswith('attention_layers') and not k.endswith('k_linear.bias') and float(ge[k].norm()) > 0:
+            assert bool(torch.isfinite(gc[k]).all()) and nrel(gc[k], ge[k]) < 100 * 2.0 ** -11, k
+
+
+def test_sharded_optimizer_trains_a_model_without_positions_in_its_tables():
+    """World size 1: the sharded trainer follows the fused one when no lookup reads the
+    position table."""
+    import os
+    import socket
+
+    import torch.distributed as dist
+
+    from tencent_recommendation_2025_amd import synthetic as S
+    from tencent_recommendation_2025_amd.optim import FusedAdamW
+    from tencent_recommendation_2025_amd.sharding import ShardedFusedAdamW
+    from tencent_recommendation_2025_amd.train import Trainer
+    s = socket.socket()
+    s.bind(('127.0.0.1', 0))
+    os.environ.update(MASTER_ADDR='127.0.0.1', MASTER_PORT=str(s.getsockname()[1]))
+    s.close()
+    dist.init_process_group('nccl', rank=0, world_size=1, device_id=torch.device(DEV, 0))
+    try:
+        m1, _, cfg = make(hidden=64)
+        m2, _, _ = make(hidden=64)
+        kw = dict(lr=2e-3, table_dtype=torch.float32, defer_period=2)
+        t1 = Trainer(m1, FusedAdamW(m1, **kw), loss='bce', amp_dtype=None)
+        t2 = Trainer(m2, ShardedFusedAdamW(m2, **kw), loss='bce', amp_dtype=None)
+        g = torch.Generator(device=DEV).manual_seed(0)
+        for _ in range(4):
+            b = S.make_batch(cfg, g, torch.device(DEV))
+            l1, l2 = t1.step(b), t2.step(b)
+            assert abs(l1.item() - l2.item()) < 1e-4 * max(1.0, abs(l1.item()))
+        s1, s2 = m1.state_dict(), m2.state_dict()
+        for k in s1:
+            if k not in ('item_emb.weight', 'user_emb.weight'):   # held as shards
+                torch.testing.assert_close(s1[k].float(), s2[k].float(), rtol=1e-3, atol=2e-5, msg=k)
+    finally:
+        dist.destroy_process_group()
+
+
+@pytest.mark.parametrize('block', ['decay', 'softmax'])
 def test_model_trains_and_leaves_the_position_table(block):
     m, batch, _ = make(block)
     m.train()
