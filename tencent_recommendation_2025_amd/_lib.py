@@ -262,9 +262,7 @@ def stream_ptr(device=None) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
-def raw_stream(index: int) -> int:
-    """stream_ptr of a device index, without the stream object."""
-    return torch._C._cuda_getCurrentRawStream(index)
+raw_stream = torch._C._cuda_getCurrentRawStream   # stream_ptr of a device index, without the stream object
 
 
 def dtype_code(t: torch.dtype) -> int:

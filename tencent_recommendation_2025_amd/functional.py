@@ -1051,7 +1051,7 @@ class _RotaryFn(torch.autograd.Function):
         heads, layout, scale = ctx.meta
         x = _head_mat(gy)
         g = K.rotary_turn(x, positions, freqs, heads, layout, scale, True,
-                          torch.empty(x.shape, dtype=x.dtype, device=x.device))
+                          x.new_empty(x.shape))
         return (g if gy.dim() == 2 else g.view(gy.shape)), None, None, None, None, None
 
 
@@ -1106,24 +1106,19 @@ class _HeadNormFn(torch.autograd.Function):
         w32, b32 = _fp32_vec(weight), _fp32_vec(bias)
         y = K.head_norm_fwd(x2, w32, b32, heads, eps, g2)
         ctx.save_for_backward(x2, w32, b32, g2)
-        ctx.meta = (heads, eps, x.shape, None if gate is None else gate.dtype,
-                    None if weight is None else weight.dtype, None if bias is None else bias.dtype)
-        return y.view(x.shape)
+        ctx.meta = (heads, eps)
+        ctx.inputs = x.shape, [t is not None and t.dtype for t in (weight, bias, gate)]
+        return y if x.dim() == 2 else y.view(x.shape)
 
     @staticmethod
     @_once
     def backward(ctx, gy):
         x2, w32, b32, g2 = ctx.saved_tensors
-        heads, eps, shape, gdt, wdt, bdt = ctx.meta
-        dx, dg, dw, db = K.head_norm_grad(_head_mat(gy, x2.dtype), x2, w32, b32, g2, heads, eps)
-        if dw is not None and wdt != torch.float32:
-            dw = dw.to(wdt)
-        if db is not None and bdt != torch.float32:
-            db = db.to(bdt)
-        if dg is not None and dg.dtype != gdt:
-            dg = dg.to(gdt)
+        dx, dg, dw, db = K.head_norm_grad(_head_mat(gy, x2.dtype), x2, w32, b32, g2, *ctx.meta)
+        shape, dtypes = ctx.inputs
         if len(shape) != 2:
-            dx, dg = dx.view(shape), dg.view(shape) if dg is not None else None
+            dx, dg = dx.view(shape), dg if dg is None else dg.view(shape)
+        dw, db, dg = (t if t is None or t.dtype == dt else t.to(dt) for t, dt in zip((dw, db, dg), dtypes))
         return dx, dw, db, dg, None, None
 
 

@@ -7,7 +7,6 @@ built library.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes as C
 import math
 import os
@@ -1149,12 +1148,18 @@ def emb_combine_bwd(gy, a, b, scale, relu=True, dropout_p=0.0, seed=0, want=(Tru
 # has its own) with cold caches: what they check costs more than the launch, so each
 # operand is looked at once and a refusal is worded only after it has failed.
 _ROW_DTYPES = {torch.float32: L.GRK_F32, torch.bfloat16: L.GRK_BF16, torch.float16: L.GRK_F16}
-_NO_DEVICE = contextlib.nullcontext()
+_current_device = torch._C._cuda_getDevice
 
 
-def _on_device(index):
-    """That device as the current one for a launch (no cost where it is already)."""
-    return _NO_DEVICE if index == torch._C._cuda_getDevice() else torch.cuda.device(index)
+def _launch(fn, name, dev, *args):
+    """One call of the library with that device current (its stream the last argument)."""
+    if dev == _current_device():
+        rc = fn(*args, L.raw_stream(dev))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, L.raw_stream(dev))
+    if rc:
+        L.check(rc, name)
 
 
 def _same_device(ref, *ts):
@@ -1274,7 +1279,7 @@ def rotary(x, positions, freqs, heads, layout='half', scale=1.0, inverse=False, 
     if freqs.dtype != torch.float64 or freqs.dim() != 1 or not freqs.is_contiguous():
         raise L.GrkError('freqs must be a contiguous float64 [rotary_dim / 2] tensor')
     if out is None:
-        out = torch.empty((N, cols), dtype=x.dtype, device=x.device)
+        out = x.new_empty(x.shape)
     elif out.data_ptr() != x.data_ptr() or out.stride(0) != x.stride(0):
         _fresh(out, 'out', x)
     _row_code(x.dtype)
@@ -1288,11 +1293,9 @@ def rotary_turn(x, positions, freqs, heads, layout, scale, inverse, out):
     dt = x.dtype
     xp, xl = _head_rows(x, 'x', N, cols, dt)
     op, ol = _head_rows(out, 'out', N, cols, dt)
-    with _on_device(dev):
-        rc = L.lib().grk_rotary(xp, xl, op, ol, _ROW_DTYPES[dt], positions.data_ptr(),
-                                L.itype_code(positions.dtype), freqs.data_ptr(), N, heads, cols // heads,
-                                2 * freqs.shape[0], layout == 'interleaved', scale, inverse, L.raw_stream(dev))
-    L.check(rc, 'grk_rotary')
+    _launch(L.lib().grk_rotary, 'grk_rotary', dev, xp, xl, op, ol, _ROW_DTYPES[dt], positions.data_ptr(),
+            L.itype_code(positions.dtype), freqs.data_ptr(), N, heads, cols // heads, 2 * freqs.shape[0],
+            layout == 'interleaved', scale, inverse)
     return out
 
 
@@ -1358,13 +1361,11 @@ def decay_attn_packed_fwd(qkv, log_decay, batch, seq_len, scale=None, key_valid=
     x, ld = _head_rows(qkv, 'qkv', rows, cols, dt)
     a = _decay_struct(layout, _row_code(dt), scale, *_thirds(x, ld, D, dt), log_decay, key_valid, seq_range, row_base,
                       rows)
-    out = torch.empty((rows, D), dtype=dt, device=qkv.device)
+    out = qkv.new_empty((rows, D))
     lib = L.lib()
-    with _on_device(dev):
-        n = lib.grk_decay_attn_workspace(a, 0)
-        ws = torch.empty(n, dtype=torch.uint8, device=qkv.device) if n else None
-        rc = lib.grk_decay_attn_fwd(a, None, None, out.data_ptr(), D, _ptr(ws), n, L.raw_stream(dev))
-    L.check(rc, 'grk_decay_attn_fwd')
+    n = lib.grk_decay_attn_workspace(a, 0)
+    ws = torch.empty(n, dtype=torch.uint8, device=qkv.device) if n else None
+    _launch(lib.grk_decay_attn_fwd, 'grk_decay_attn_fwd', dev, a, None, None, out.data_ptr(), D, _ptr(ws), n)
     return out, a
 
 
@@ -1381,15 +1382,13 @@ def decay_attn_packed_bwd(dout, args, qkv, log_decay, key_valid=None, seq_range=
         a = _decay_struct((a.batch, a.seq_len, a.heads, a.head_dim), a.dtype, a.scale, *_thirds(x, ld, D, dt),
                           log_decay, key_valid, seq_range, row_base, rows)
     gp, gl = _head_rows(dout, 'dout', rows, D, dt)
-    dx = torch.empty((rows, cols), dtype=dt, device=qkv.device)
+    dx = qkv.new_empty((rows, cols))
     dp, step = dx.data_ptr(), D * dt.itemsize
     lib = L.lib()
-    with _on_device(dev):
-        n = lib.grk_decay_attn_workspace(a, 1)
-        ws = torch.empty(n, dtype=torch.uint8, device=qkv.device) if n else None
-        rc = lib.grk_decay_attn_bwd(a, gp, gl, dp, cols, dp + step, cols, dp + 2 * step, cols, _ptr(ws), n,
-                                    L.raw_stream(dev))
-    L.check(rc, 'grk_decay_attn_bwd')
+    n = lib.grk_decay_attn_workspace(a, 1)
+    ws = torch.empty(n, dtype=torch.uint8, device=qkv.device) if n else None
+    _launch(lib.grk_decay_attn_bwd, 'grk_decay_attn_bwd', dev, a, gp, gl, dp, cols, dp + step, cols, dp + 2 * step,
+            cols, _ptr(ws), n)
     return dx
 
 
@@ -1429,10 +1428,8 @@ def decay_attn_fwd(q, k, v, log_decay, batch, seq_len, scale=None, key_valid=Non
     else:
         _fresh(out, 'out', q, k, v)
     op, ol = _head_rows(out, 'out', q.shape[0], q.shape[1], q.dtype)
-    with _on_device(dev):
-        ws, n = _decay_workspace(a, 0, q.device)
-        rc = L.lib().grk_decay_attn_fwd(a, _ptr(state), _ptr(state_out), op, ol, _ptr(ws), n, L.raw_stream(dev))
-    L.check(rc, 'grk_decay_attn_fwd')
+    ws, n = _decay_workspace(a, 0, q.device)
+    _launch(L.lib().grk_decay_attn_fwd, 'grk_decay_attn_fwd', dev, a, _ptr(state), _ptr(state_out), op, ol, _ptr(ws), n)
     return (out, state_out) if return_state else out
 
 
@@ -1449,10 +1446,8 @@ def decay_attn_bwd(dout, q, k, v, log_decay, batch, seq_len, scale=None, key_val
     for i, t in enumerate(grads):
         _fresh(t, ('dq', 'dk', 'dv')[i], dout, q, k, v, *grads[:i])
     (p0, l0), (p1, l1), (p2, l2) = ptrs
-    with _on_device(dev):
-        ws, n = _decay_workspace(a, 1, q.device)
-        rc = L.lib().grk_decay_attn_bwd(a, gp, gl, p0, l0, p1, l1, p2, l2, _ptr(ws), n, L.raw_stream(dev))
-    L.check(rc, 'grk_decay_attn_bwd')
+    ws, n = _decay_workspace(a, 1, q.device)
+    _launch(L.lib().grk_decay_attn_bwd, 'grk_decay_attn_bwd', dev, a, gp, gl, p0, l0, p1, l1, p2, l2, _ptr(ws), n)
     return tuple(grads)
 
 
@@ -1490,14 +1485,12 @@ def decay_attn_step(q, k, v, log_decay, state, slots=None, scale=None, err_flag=
         _fresh(out, 'out', q, k, v)
     op, ol = _head_rows(out, 'out', n, cols, dt)
     lib = L.lib()
-    with _on_device(dev):
-        nb = lib.grk_decay_attn_step_workspace(n, slots is not None)
-        ws = torch.empty(nb, dtype=torch.uint8, device=q.device) if nb else None
-        rc = lib.grk_decay_attn_step(qp, ql, kp, kl, vp, vl, code, log_decay.data_ptr(), n, H, hd,
-                                     hd ** -0.5 if scale is None else scale, state.data_ptr(), state.shape[0],
-                                     _ptr(slots), L.itype_code(slots.dtype) if slots is not None else L.GRK_I64,
-                                     _ptr(err_flag), op, ol, _ptr(ws), nb, L.raw_stream(dev))
-    L.check(rc, 'grk_decay_attn_step')
+    nb = lib.grk_decay_attn_step_workspace(n, slots is not None)
+    ws = torch.empty(nb, dtype=torch.uint8, device=q.device) if nb else None
+    _launch(lib.grk_decay_attn_step, 'grk_decay_attn_step', dev, qp, ql, kp, kl, vp, vl, code,
+            log_decay.data_ptr(), n, H, hd, hd ** -0.5 if scale is None else scale, state.data_ptr(),
+            state.shape[0], _ptr(slots), L.itype_code(slots.dtype) if slots is not None else L.GRK_I64,
+            _ptr(err_flag), op, ol, _ptr(ws), nb)
     return out
 
 
@@ -1522,15 +1515,13 @@ def head_norm_fwd(x, weight, bias, heads, eps=1e-5, gate=None, out=None):
     dt = x.dtype
     code = _row_code(dt)
     if out is None:
-        out = torch.empty((N, cols), dtype=dt, device=x.device)
+        out = x.new_empty(x.shape)
         op, ol = out.data_ptr(), cols
     else:
         op, ol = _head_rows(out, 'out', N, cols, dt)
         _fresh(out, 'out', *[t for t, p, ld in ((x, xp, xl), (gate, gp, gl)) if t is not None and (p, ld) != (op, ol)])
-    with _on_device(dev):
-        rc = L.lib().grk_head_norm_fwd(xp, xl, gp, gl, _ptr(weight), _ptr(bias), eps, N, heads, cols // heads, code,
-                                       op, ol, L.raw_stream(dev))
-    L.check(rc, 'grk_head_norm_fwd')
+    _launch(L.lib().grk_head_norm_fwd, 'grk_head_norm_fwd', dev, xp, xl, gp, gl, _ptr(weight), _ptr(bias), eps, N,
+            heads, cols // heads, code, op, ol)
     return out
 
 
@@ -1551,36 +1542,41 @@ def head_norm_bwd(dy, x, weight, bias, heads, eps=1e-5, gate=None, dx=None, dgat
 
 def head_norm_grad(dy, x, weight, bias, gate, heads, eps, dx=None, dgate=None):
     """head_norm_bwd of operands that head_norm_fwd has taken (only dy is looked at)."""
-    device, dt = x.device, x.dtype
     dev = _same_device(x, dy)
-    N, cols = x.shape
+    shape, dt = x.shape, x.dtype
+    N, cols = shape
     yp, yl = _head_rows(dy, 'dy', N, cols, dt)
-    empty = torch.empty
     if dx is None:
-        dx = empty((N, cols), dtype=dt, device=device)
-    gp, gl, dgp, dgl = None, 0, None, 0
+        dx = x.new_empty(shape)
+    gp = dgp = None
+    gl = dgl = 0
     if gate is None:
         dgate = None
     else:
         if dgate is None:
-            dgate = empty((N, cols), dtype=dt, device=device)
+            dgate = x.new_empty(shape)
         gp, gl, dgp, dgl = gate.data_ptr(), gate.stride(0), dgate.data_ptr(), dgate.stride(0)
-    lib, nb = L.lib(), 0
-    wp = bp = dw = db = dwp = dbp = ws = None
+    wp = bp = dw = db = dwp = dbp = None
     if weight is not None:
-        dw = empty(cols, dtype=torch.float32, device=device)
-        wp, dwp = weight.data_ptr(), dw.data_ptr()
-    if bias is not None:
-        db = empty(cols, dtype=torch.float32, device=device)
+        wp = weight.data_ptr()
+        if bias is not None:
+            dw, db = weight.new_empty((2, cols)).unbind(0)
+        else:
+            dw = weight.new_empty((cols,))
+        dwp = dw.data_ptr()
+    elif bias is not None:
+        db = bias.new_empty((cols,))
+    if db is not None:
         bp, dbp = bias.data_ptr(), db.data_ptr()
+    lib, ws, wsp, nb = L.lib(), None, None, 0
+    hd = cols // heads
     if dwp or dbp:
-        nb = lib.grk_head_norm_bwd_workspace(N, heads, cols // heads)
-        ws = empty(nb, dtype=torch.uint8, device=device) if nb else None
-    with _on_device(dev):
-        rc = lib.grk_head_norm_bwd(yp, yl, x.data_ptr(), x.stride(0), gp, gl, wp, bp, eps, N, heads, cols // heads,
-                                   _ROW_DTYPES[dt], dx.data_ptr(), dx.stride(0), dgp, dgl, dwp, dbp, _ptr(ws), nb,
-                                   L.raw_stream(dev))
-    L.check(rc, 'grk_head_norm_bwd')
+        nb = lib.grk_head_norm_bwd_workspace(N, heads, hd)
+        if nb:
+            ws = torch.empty(nb // 4, device=x.device)
+            wsp = ws.data_ptr()
+    _launch(lib.grk_head_norm_bwd, 'grk_head_norm_bwd', dev, yp, yl, x.data_ptr(), x.stride(0), gp, gl, wp, bp, eps, N,
+            heads, hd, _ROW_DTYPES[dt], dx.data_ptr(), dx.stride(0), dgp, dgl, dwp, dbp, wsp, nb)
     return dx, dgate, dw, db
 
 
