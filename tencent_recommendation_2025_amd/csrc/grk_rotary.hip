@@ -38,7 +38,7 @@ __device__ __forceinline__ void turn(float& a, float& b, float2 w) {
 // The angle is reduced in 64 bits: at position 10^6 an fp32 product p * freq is off by
 // up to 0.03 rad, the fp64 one by 10^-10.  What is left, a fraction of a turn, is an
 // fp32 argument of sincospi (2^-25 of half a turn).
-template <typename T, int V>
+template <typename T, int V, bool PAST>
 __global__ void __launch_bounds__(kRotThreads) k_rotary(RotParams p) {
   __shared__ float2 cs[kRotAngles];
   const int64_t row0 = (int64_t)blockIdx.x * p.rows_per_block;
@@ -70,13 +70,13 @@ __global__ void __launch_bounds__(kRotThreads) k_rotary(RotParams p) {
       vload<T, V>(x + p.r + u * V, xb);
 #pragma unroll
       for (int e = 0; e < V; ++e) turn(xa[e], xb[e], t[u * V + e]);
-      vstore<T, V>(y + u * V, xa);
-      vstore<T, V>(y + p.r + u * V, xb);
+      vstore<T, V, PAST>(y + u * V, xa);
+      vstore<T, V, PAST>(y + p.r + u * V, xb);
     } else if (!p.interleaved) {
       const int c = 2 * p.r + (u - turned) * V;
       float v[V];
       vload<T, V>(x + c, v);
-      vstore<T, V>(y + c, v);
+      vstore<T, V, PAST>(y + c, v);
     } else {
       static_assert(V == 1 || V % 2 == 0, "");
       const int c = u * V;
@@ -97,7 +97,7 @@ __global__ void __launch_bounds__(kRotThreads) k_rotary(RotParams p) {
 #pragma unroll
         for (int e = 0; e < V; e += 2)
           if (c + e < 2 * p.r) turn(v[e], v[e + 1], t[(c + e) >> 1]);
-        vstore<T, V>(y + c, v);
+        vstore<T, V, PAST>(y + c, v);
       }
     }
   }
@@ -132,6 +132,11 @@ extern "C" int grk_rotary(const void* x, int64_t ldx, void* y, int64_t ldy, int 
   // whole vectors: the rows, the heads in them and, in the half layout, both halves
   const bool vec = vec_rows(x, ldx, dtype) && vec_rows(y, ldy, dtype) && head_dim % ve == 0 &&
                    (p.interleaved || p.r % ve == 0);
+  // An output of a quarter of the 256 MB cache or more passes it by and leaves it to what was
+  // there, the input among it (32771 rows of 8 heads of 80, fp32, 84 MB: 39.7 -> 27.4 us);
+  // smaller ones stay for their reader (25728 rows of 16 heads of 64, bf16, 53 MB: 23.4 us,
+  // past the cache 25.2).
+  const bool past = rows * cols * (int64_t)dtype_size(dtype) >= (64 << 20);
   // rows of a workgroup: enough that it streams 32 KB, few enough that the grid holds
   // 1024 workgroups (4 on each CU) and their angles fit the LDS table
   int64_t rpb = 32768 / (cols * (int64_t)dtype_size(dtype));
@@ -144,8 +149,9 @@ extern "C" int grk_rotary(const void* x, int64_t ldx, void* y, int64_t ldy, int 
   hipStream_t s = (hipStream_t)stream;
   const int rc = for_dtype(dtype, [&](auto t) {
     using T = decltype(t);
-    if (vec) k_rotary<T, vec_elems<T>()><<<(unsigned)grid, kRotThreads, 0, s>>>(p);
-    else k_rotary<T, 1><<<(unsigned)grid, kRotThreads, 0, s>>>(p);
+    if (vec && past) k_rotary<T, vec_elems<T>(), true><<<(unsigned)grid, kRotThreads, 0, s>>>(p);
+    else if (vec) k_rotary<T, vec_elems<T>(), false><<<(unsigned)grid, kRotThreads, 0, s>>>(p);
+    else k_rotary<T, 1, false><<<(unsigned)grid, kRotThreads, 0, s>>>(p);
     return 0;
   });
   (void)rc;

@@ -39,7 +39,8 @@ __device__ __forceinline__ void vload(const T* p, float* f) {
   }
 }
 
-template <typename T, int V>
+// PAST: the store passes the caches by.
+template <typename T, int V, bool PAST = false>
 __device__ __forceinline__ void vstore(T* p, const float* f) {
   if constexpr (V == 1) {
     *p = from_f32<T>(f[0]);
@@ -48,9 +49,11 @@ __device__ __forceinline__ void vstore(T* p, const float* f) {
     T t[V];
 #pragma unroll
     for (int e = 0; e < V; ++e) t[e] = from_f32<T>(f[e]);
-    uint4 w;
+    typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+    u32x4 w;
     __builtin_memcpy(&w, t, 16);
-    *reinterpret_cast<uint4*>(p) = w;
+    if constexpr (PAST) __builtin_nontemporal_store(w, reinterpret_cast<u32x4*>(p));
+    else *reinterpret_cast<u32x4*>(p) = w;
   }
 }
 
