@@ -2,7 +2,7 @@
 //
 //   S_t = g S_{t-1} + k_t v_t^T,   o_t = scale q_t S_t,   g = exp(log_decay[h])
 //
-// In chunks of 64 steps this is three products per chunk (i, j: steps of the chunk,
+// In chunks of steps this is three products per chunk (i, j: steps of the chunk,
 // n: its length, S: the state before it):
 //   P_ij = [j <= i] g^(i-j) q_i . k_j,   o_i = scale (sum_j P_ij v_j + g^(i+1) q_i S),
 //   S   <- g^n S + sum_j g^(n-1-j) k_j v_j^T.

@@ -1,7 +1,7 @@
 // Decayed linear attention of bf16 rows on the bf16 matrix instruction, for gfx950 (the
 // formulas: grk_decay.h; heads and rows made of 16-byte vectors).
 //
-// A workgroup walks a segment in chunks of 64 steps with EW columns of the state (and of the
+// A workgroup walks a segment in chunks of C steps with EW columns of the state (and of the
 // output); each wave owns NE tiles of 16 of them.  v_mfma_f32_16x16x32_bf16: lane
 // l = 16 g + c holds A[c][8 g + s] and B[8 g + s][c], s < 8, and D[4 g + i][c], i < 4 -- A
 // and B fragments are laid out alike, so exchanging them transposes D.  What is stored
@@ -11,15 +11,19 @@
 // if the contraction takes its 32 d in the order (4 g + i, 16 + 4 g + i), so Q is read
 // from LDS in that order (two 8-byte reads) and the state never leaves its registers.
 //
-// Per chunk and wave (DP = 64): P^T 6 MFMA (lower tiles only), O^T 8 + 6, S 8: 28, a
-// quarter of the time the chunk's 32 KB take from HBM on one CU of 256, so the kernel is
-// bound by memory and by what hides its latency: the next chunk is loaded to registers
-// while this one is computed, and 4 workgroups share a CU.
+// Bound: heads of 64, memory's latency -- a wave takes some 20 MFMA, 190 VALU operations and
+// 26 LDS accesses for 32 steps, half of the time that their 16 KB take from HBM on one CU
+// of 256; what is left is the wait of a chunk's two barriers, which the next chunk's loads
+// (to registers, while this one is computed) and 4 waves a SIMD cover in part.  128
+// sequences of up to 201 events (16 K packed rows) of 8 heads of 64: forward 19.6 us (66
+// MB, 3.4 TB/s), gradients 38.1 us (116 MB, 3.0 TB/s).  Heads of 128: LDS, read for every
+// operand of 4 products a chunk.  8 x 4096 events of 4 heads: 39 us and gradients 93 us
+// after 40 and 48 us for the segment states.
 //
 // LDS rows are 16 bytes longer than the head: 16 rows' 16-byte pieces fall on all 64 banks
 // at once, every address is a lane's base plus a constant, and a transposing read that
 // takes every second row (4 rows 8 banks apart) has no conflicts either.  So the
-// contraction over the 64 steps takes each 8 of them in the order 0 2 4 6 1 3 5 7 ("slots"):
+// contraction over a chunk's steps takes each 8 of them in the order 0 2 4 6 1 3 5 7 ("slots"):
 // P and the weights of the state's sum are laid down in that order.
 #include <type_traits>
 
@@ -28,16 +32,15 @@
 
 namespace grk {
 
-// Tables in LDS: scale g^n for 0 <= n <= 64, 0 for -16 < n < 0 (above the diagonal); the
-// state's weights g^(63 - j) by slot; one word a step that holds an event.
-constexpr int kDecayPowers = 16 + kDecayChunk + 4;
+// Tables in LDS: scale g^n for 0 <= n <= C, 0 for -16 < n < 0 (above the diagonal); the
+// state's weights g^(C - 1 - j) by slot; one word a step that holds an event.
+template <int C> constexpr int decay_powers() { return 16 + C + 4; }
 
 template <int DP> constexpr int decay_stride() { return DP * 2 + 16; }   // bytes of an LDS row
-constexpr int kDecayPStride = decay_stride<kDecayChunk>();
 
-template <int DP, int EW> constexpr size_t decay_lds_bf16(bool state_only) {
-  return (size_t)kDecayChunk * ((state_only ? 1 : 2) * decay_stride<DP>() + decay_stride<EW>()) +
-         (state_only ? 0 : kDecayChunk * kDecayPStride) + (kDecayPowers + 2 * kDecayChunk) * 4;
+template <int DP, int EW, int C> constexpr size_t decay_lds_bf16(bool state_only) {
+  return (size_t)C * ((state_only ? 1 : 2) * decay_stride<DP>() + decay_stride<EW>()) +
+         (state_only ? 0 : C * decay_stride<C>()) + (decay_powers<C>() + 2 * C) * 4;
 }
 
 __device__ __forceinline__ void mfma32(bf16x8 a, bf16x8 b, f32x4& c) {
@@ -94,15 +97,16 @@ __device__ __forceinline__ int decay_first_row() {
 // row is a uniform pointer, a lane's offset from it 32 bits (the host admits row strides
 // below 2^24 elements).  Masked steps are loaded too (their row exists) and zeroed by
 // selection, so the loads do not wait for the mask.
-template <int DP, int NTH>
+template <int DP, int NTH, int C>
 struct DecayRows {
-  static constexpr int R = NTH / (DP / 8), N = kDecayChunk / R;
+  static constexpr int R = NTH / (DP / 8), N = C / R;
+  static_assert(N * R == C, "whole turns");
   unsigned at[N];    // the row's place above the chunk's lowest
   bool live[N];      // it holds an event
   int64_t low;       // the chunk's lowest row
   __device__ __forceinline__ void chunk(const DecayParams& p, const DecayPlace& w, int rev, int64_t base, bool masked,
                                         int t0) {
-    const int n = w.t1 - t0 < kDecayChunk ? w.t1 - t0 : kDecayChunk;
+    const int n = w.t1 - t0 < C ? w.t1 - t0 : C;
     const int pos0 = rev ? p.seq_len - t0 - n : w.start + t0;
     low = base + pos0;
 #pragma unroll
@@ -132,19 +136,19 @@ struct DecayRows {
 // bits).  One part would cost 2 % (heads of 64) to 10 % (128) less time and put a third
 // rounding of 2^-9 into every output, which then lay 1.6 times as far from the exact one as
 // its own rounding; with two it is 1.4 times.
-template <int DP, int EW, int NE, int NS, bool STATE>
-__global__ void __launch_bounds__(EW * 4 / NE, NE == 1 ? 4 : 2) k_decay_bf16(DecayParams p) {
-  constexpr int C = kDecayChunk, NT = DP / 16, KS = DP / 32, NW = EW / 16 / NE, NTH = NW * 64;
-  constexpr int ST = decay_stride<DP>(), SE = decay_stride<EW>(), PS = kDecayPStride;
-  using Rows = DecayRows<DP, NTH>;    // of a and b
-  using Cols = DecayRows<EW, NTH>;    // of c
+template <int DP, int EW, int NE, int C, int NS, bool STATE>
+__global__ void __launch_bounds__(EW * 4 / NE, NE == 1 ? 4 : C == 32 ? 3 : 2) k_decay_bf16(DecayParams p) {
+  constexpr int CK = C / 32, NT = DP / 16, KS = DP / 32, NW = EW / 16 / NE, NTH = NW * 64;
+  constexpr int ST = decay_stride<DP>(), SE = decay_stride<EW>(), PS = decay_stride<C>();
+  using Rows = DecayRows<DP, NTH, C>;    // of a and b
+  using Cols = DecayRows<EW, NTH, C>;    // of c
   extern __shared__ __attribute__((aligned(16))) char lds[];
   char* sb = lds;
   char* sc = sb + C * ST;
   char* sa = sc + C * SE;
   char* sp = sa + (STATE ? 0 : C * ST);
   float* pw = reinterpret_cast<float*>(sp + (STATE ? 0 : C * PS)) + 16;
-  float* wv = pw - 16 + kDecayPowers;
+  float* wv = pw - 16 + decay_powers<C>();
   int* slive = reinterpret_cast<int*>(wv + C);
   DecayPlace w = decay_place(p, DP / EW);
   if (!w.on) return;
@@ -235,7 +239,7 @@ __global__ void __launch_bounds__(EW * 4 / NE, NE == 1 ? 4 : 2) k_decay_bf16(Dec
     if (!last) fetch(t0 + C);
     if constexpr (!STATE) {
       // P^T, lower tiles; the tiles above the diagonal that a 32-deep step reads stay 0
-      for (int tile = wave; tile < 10; tile += NW) {
+      for (int tile = wave; tile < C / 16 * (C / 16 + 1) / 2; tile += NW) {
         const int it = tile >= 6 ? 3 : tile >= 3 ? 2 : tile >= 1 ? 1 : 0, jt = tile - it * (it + 1) / 2;
         const char* q = sa + 16 * it * ST + row_b;
         const char* k = sb + 16 * jt * ST + row_b;
@@ -251,11 +255,11 @@ __global__ void __launch_bounds__(EW * 4 / NE, NE == 1 ? 4 : 2) k_decay_bf16(Dec
         *reinterpret_cast<unsigned*>(dst + 8) = z.y;
       }
     }
-    bf16x8 vf[NE][2];
+    bf16x8 vf[NE][CK];
 #pragma unroll
     for (int x = 0; x < NE; ++x)
 #pragma unroll
-      for (int ks = 0; ks < 2; ++ks) vf[x][ks] = lds_col8s<SE>(sc + decay_col_base<SE>(lane) + 32 * ks * SE + 32 * (NE * wave + x));
+      for (int ks = 0; ks < CK; ++ks) vf[x][ks] = lds_col8s<SE>(sc + decay_col_base<SE>(lane) + 32 * ks * SE + 32 * (NE * wave + x));
     f32x4 o[C / 16][NE];
     bool live[C / 16];
     if constexpr (!STATE) {
@@ -302,7 +306,7 @@ __global__ void __launch_bounds__(EW * 4 / NE, NE == 1 ? 4 : 2) k_decay_bf16(Dec
 #pragma unroll
         for (int dt = 0; dt < NT; ++dt) st[x][dt] *= gn;
 #pragma unroll
-      for (int ks = 0; ks < 2; ++ks) {
+      for (int ks = 0; ks < CK; ++ks) {
         bf16x8 part[NE][NS];
         const f32x4 w0 = *reinterpret_cast<const f32x4*>(wv + 32 * ks + 8 * g);
         const f32x4 w1 = *reinterpret_cast<const f32x4*>(wv + 32 * ks + 8 * g + 4);
@@ -373,16 +377,17 @@ __global__ void __launch_bounds__(EW * 4 / NE, NE == 1 ? 4 : 2) k_decay_bf16(Dec
 
 // Segment states are those of roles 0 and 1: role 2 (K, Q, dO) sums q dO^T where role 1
 // (V, dO, Q) sums dO q^T.
-template <int DP, int NE>
+template <int DP, int NE, int MC>
 static int decay_bf16_run(const DecayParams& p, hipStream_t s) {
   const int64_t groups = ((int64_t)p.batch * p.heads * p.nseg + 7) / 8 * 8;
   auto launch = [&](auto ew, auto ne, auto ns, auto state, const DecayParams& q) -> int {
     constexpr int EW = decltype(ew)::value, E = decltype(ne)::value, NS = decltype(ns)::value;
+    constexpr int C = decltype(state)::value ? kDecayChunk : MC;
     constexpr bool STATE = decltype(state)::value;
-    constexpr size_t lds = decay_lds_bf16<DP, EW>(STATE);
-    GRK_CHECK_HIP(ensure_dynamic_lds((const void*)k_decay_bf16<DP, EW, E, NS, STATE>, lds));
+    constexpr size_t lds = decay_lds_bf16<DP, EW, C>(STATE);
+    GRK_CHECK_HIP(ensure_dynamic_lds((const void*)k_decay_bf16<DP, EW, E, C, NS, STATE>, lds));
     const unsigned grid = (unsigned)(groups * (DP / EW) * q.roles);
-    k_decay_bf16<DP, EW, E, NS, STATE><<<grid, EW * 4 / E, lds, s>>>(q);
+    k_decay_bf16<DP, EW, E, C, NS, STATE><<<grid, EW * 4 / E, lds, s>>>(q);
     GRK_LAUNCH_CHECK();
     return GRK_OK;
   };
@@ -416,10 +421,18 @@ bool decay_bf16_takes(const DecayParams& p) {
   return ok;
 }
 
+// Chunks of 32 steps for heads of up to 64 columns (128 sequences of up to 201 events,
+// 8 heads of 64: forward 19.6 us, with 64 steps 21.8), of 64 steps above (8 x 4096 events, 4
+// heads of 128: gradients 93 us, with 32 steps 105).  Heads of 64: two column tiles a wave
+// halve what the waves read from LDS and pay once there are workgroups for two rounds
+// (the former's gradients, 3072 workgroups: 38.1 us, one tile 41.7); with fewer, more waves
+// hide more latency (forward, 1024 workgroups: 19.6 us, two tiles 20.9).  Heads of 128:
+// two tiles always (gradients 93 us, one tile 105).
 int decay_bf16_launch(const DecayParams& p, hipStream_t s) {
-  if (p.head_dim <= 32) return decay_bf16_run<32, 1>(p, s);
-  if (p.head_dim <= 64) return decay_bf16_run<64, 1>(p, s);
-  return decay_bf16_run<128, 2>(p, s);
+  if (p.head_dim <= 32) return decay_bf16_run<32, 1, 32>(p, s);
+  if (p.head_dim > 64) return decay_bf16_run<128, 2, 64>(p, s);
+  if ((int64_t)p.roles * p.batch * p.heads * p.nseg >= 2048) return decay_bf16_run<64, 2, 32>(p, s);
+  return decay_bf16_run<64, 1, 32>(p, s);
 }
 
 }  // namespace grk

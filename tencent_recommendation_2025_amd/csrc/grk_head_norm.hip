@@ -7,7 +7,9 @@
 //
 // Bound: memory -- x, u, y once forward; dy, x, u, dx, du once backward.  Nothing is
 // saved between the two: the backward has x in registers anyway and takes mean and rstd
-// from it again, which is cheaper than a statistics buffer's traffic.
+// from it again, which is cheaper than a statistics buffer's traffic.  25728 rows of 8 heads
+// of 64, bf16, gated: forward 16.6 us (79 MB, 4.8 TB/s), backward 30 us (132 MB, 4.4 TB/s)
+// and 5 us for the sums of its 1024 row blocks.
 //
 // Layout: LPG lanes (a power of two, at most a wave) hold one head's columns as VPL
 // vectors each, so a head's sums are log2(LPG) lane exchanges and no LDS.  A thread keeps
