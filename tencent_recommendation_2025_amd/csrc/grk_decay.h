@@ -42,6 +42,9 @@ struct DecayParams {
   float* ws;                       // segment states [role][batch, heads][segment][DP * DP], fragment order
 };
 
+// min(log g, 0); NaN stays (fminf would make it 0).
+__device__ __forceinline__ float decay_log(float lg) { return lg > 0.f ? 0.f : lg; }
+
 // One workgroup's pass: a role, a (sequence, head) and a segment of it.
 struct DecayPlace {
   int b, h, seg, role, part;       // part: its columns of the state and the output, where they are shared out
@@ -71,7 +74,7 @@ __device__ __forceinline__ DecayPlace decay_place(const DecayParams& p, int part
   w.len = p.seq_len - w.start;
   w.t0 = w.seg * p.seg_len;
   w.t1 = w.t0 + p.seg_len < w.len ? w.t0 + p.seg_len : w.len;
-  w.lg = fminf(p.log_decay[w.h], 0.f);
+  w.lg = decay_log(p.log_decay[w.h]);
   return w;
 }
 

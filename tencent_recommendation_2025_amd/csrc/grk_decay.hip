@@ -269,7 +269,7 @@ __global__ void __launch_bounds__(256) k_decay_scan(DecayParams p) {
   int start = p.seq_range ? p.seq_range[3 * (int64_t)b] : 0;
   start = start < 0 ? 0 : (start > p.seq_len ? p.seq_len : start);
   const int len = p.seq_len - start;
-  const float lg = fminf(p.log_decay[h], 0.f), gs = decay_pow(lg, p.seg_len);
+  const float lg = decay_log(p.log_decay[h]), gs = decay_pow(lg, p.seg_len);
   typedef float vec __attribute__((ext_vector_type(W)));
   vec run = 0.f;
   auto outside = [&](int k) { return (bh * p.head_dim + d0 + k) * p.head_dim + e; };   // in state_in / state_out
@@ -402,7 +402,7 @@ __global__ void __launch_bounds__(kStepThreads) k_decay_step(StepParams p) {
       reinterpret_cast<T*>(p.out)[i0 * p.ldo + (int64_t)h * hd + c] = from_f32<T>(0.f);
     return;
   }
-  const float g = expf(fminf(p.log_decay[h], 0.f));
+  const float g = expf(decay_log(p.log_decay[h]));
   float* S = p.state + (slot * p.heads + h) * hd * hd;
   for (int64_t i = i0; i >= 0;) {
     // the slot's other events

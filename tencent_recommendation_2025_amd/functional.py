@@ -1158,6 +1158,10 @@ class _RotaryQKFn(torch.autograd.Function):
 def rotary_qk(qkv, positions, freqs, heads, layout='half', scale=1.0):
     """q | k | v rows [..., 3 * heads * head_dim] with q and k turned by their positions
     (kernels.rotary) and v as it is."""
+    if freqs.requires_grad:
+        raise L.GrkError('rotary: freqs get no gradient')
+    if int(heads) < 1 or qkv.shape[-1] % (3 * int(heads)):
+        raise L.GrkError('qkv must hold q | k | v side by side: [..., 3 * heads * head_dim]')
     return _RotaryQKFn.apply(qkv, positions, freqs, int(heads), layout, float(scale))
 
 
@@ -1208,6 +1212,10 @@ def decay_core(pre, log_decay, weight, bias, batch, seq_len, key_valid=None, seq
     """norm(decay_attn(rotary(q), rotary(k), v)) * SiLU(u) of [N, 4 D] (u | v | q | k) rows,
     [N, D] out: the decay block between its projections.  rot: (positions [N], freqs,
     layout, scale) of kernels.rotary, or None."""
+    if log_decay.requires_grad:
+        raise L.GrkError('decay_core: log_decay gets no gradient (the decays are given, not learned)')
+    if pre.shape[-1] % (4 * log_decay.shape[0]) or weight is None or bias is None:
+        raise L.GrkError('pre must hold u | v | q | k side by side, [N, 4 * heads * head_dim], with weight and bias')
     return _DecayCoreFn.apply(pre, log_decay, weight, bias, float(eps), rot,
                               (int(batch), int(seq_len), key_valid, seq_range, row_base))
 

@@ -1195,8 +1195,8 @@ def _row_code(dtype):
 def _overlap(a, b):
     """Whether two row-major matrices of one dtype share an element (column views of one
     buffer with one row stride are told apart; other interleavings count as shared)."""
-    if not a.numel() or not b.numel():
-        return False
+    if a.dim() != 2 or b.dim() != 2 or not a.numel() or not b.numel():
+        return False   # (another shape is refused where the rows are looked at)
     es = a.element_size()
 
     def end(t):
@@ -1209,6 +1209,17 @@ def _overlap(a, b):
         return True
     gap = gap // es % ld
     return not (gap >= a.shape[1] and gap + b.shape[1] <= ld)
+
+
+def _meet(a, b):
+    """Whether the memory from the first to the last element of a and b has bytes in common."""
+    def ends(t):
+        lo = t.data_ptr()
+        return lo, lo + (sum((s - 1) * st for s, st in zip(t.shape, t.stride())) + 1) * t.element_size()
+    if not a.numel() or not b.numel():
+        return False
+    (a0, a1), (b0, b1) = ends(a), ends(b)
+    return a0 < b1 and b0 < a1
 
 
 def _fresh(out, name, *inputs):
@@ -1280,6 +1291,8 @@ def rotary(x, positions, freqs, heads, layout='half', scale=1.0, inverse=False, 
         raise L.GrkError('freqs must be a contiguous float64 [rotary_dim / 2] tensor')
     if out is None:
         out = x.new_empty(x.shape)
+    elif out.shape != x.shape:
+        raise L.GrkError(f'out: shape {tuple(out.shape)}, expected {tuple(x.shape)}')
     elif out.data_ptr() != x.data_ptr() or out.stride(0) != x.stride(0):
         _fresh(out, 'out', x)
     _row_code(x.dtype)
@@ -1376,8 +1389,8 @@ def decay_attn_packed_bwd(dout, args, qkv, log_decay, key_valid=None, seq_range=
     rows, cols = qkv.shape
     dt, D = qkv.dtype, cols // 3
     a = args
-    if (qkv.data_ptr(), log_decay.data_ptr(), _ptr(key_valid), _ptr(seq_range), _ptr(row_base)) != \
-            (a.q or 0, a.log_decay, a.key_valid, a.seq_range, a.row_base):
+    if (qkv.data_ptr(), qkv.stride(0), log_decay.data_ptr(), _ptr(key_valid), _ptr(seq_range), _ptr(row_base)) != \
+            (a.q or 0, a.ldq, a.log_decay, a.key_valid, a.seq_range, a.row_base):
         x, ld = _head_rows(qkv, 'qkv', rows, cols, dt)
         a = _decay_struct((a.batch, a.seq_len, a.heads, a.head_dim), a.dtype, a.scale, *_thirds(x, ld, D, dt),
                           log_decay, key_valid, seq_range, row_base, rows)
@@ -1421,12 +1434,18 @@ def decay_attn_fwd(q, k, v, log_decay, batch, seq_len, scale=None, key_valid=Non
         _state_ok(state, 'state', shape)
     if state_out is not None:
         _state_ok(state_out, 'state_out', shape)
+        for t, m in ((state, 'state'), (q, 'q'), (k, 'k'), (v, 'v'), (log_decay, 'log_decay')):
+            if t is not None and not (m == 'state' and t.data_ptr() == state_out.data_ptr()) and _meet(state_out, t):
+                raise L.GrkError(f'state_out must not overlap {m}' + (' (it may be state)' if m == 'state' else ''))
     elif return_state:
         state_out = torch.empty(shape, dtype=torch.float32, device=q.device)
     if out is None:
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     else:
         _fresh(out, 'out', q, k, v)
+        for t, m in ((state, 'state'), (state_out, 'state_out'), (log_decay, 'log_decay')):
+            if t is not None and _meet(out, t):
+                raise L.GrkError(f'out must not overlap {m}')
     op, ol = _head_rows(out, 'out', q.shape[0], q.shape[1], q.dtype)
     ws, n = _decay_workspace(a, 0, q.device)
     _launch(L.lib().grk_decay_attn_fwd, 'grk_decay_attn_fwd', dev, a, _ptr(state), _ptr(state_out), op, ol, _ptr(ws), n)
@@ -1483,6 +1502,8 @@ def decay_attn_step(q, k, v, log_decay, state, slots=None, scale=None, err_flag=
         out = torch.empty((n, cols), dtype=dt, device=q.device)
     else:
         _fresh(out, 'out', q, k, v)
+        if _meet(out, state):
+            raise L.GrkError('out must not overlap state')
     op, ol = _head_rows(out, 'out', n, cols, dt)
     lib = L.lib()
     nb = lib.grk_decay_attn_step_workspace(n, slots is not None)
@@ -1531,6 +1552,7 @@ def head_norm_bwd(dy, x, weight, bias, heads, eps=1e-5, gate=None, dx=None, dgat
     _same_device(x, weight, bias, gate, dx, dgate)
     _norm_operands(x, weight, bias, heads, gate)
     _row_code(x.dtype)
+    _head_rows(dy, 'dy', *x.shape, x.dtype)
     if dx is not None:
         _head_rows(dx, 'dx', *x.shape, x.dtype)
         _fresh(dx, 'dx', dy, x, gate)
@@ -1573,7 +1595,7 @@ def head_norm_grad(dy, x, weight, bias, gate, heads, eps, dx=None, dgate=None):
     if dwp or dbp:
         nb = lib.grk_head_norm_bwd_workspace(N, heads, hd)
         if nb:
-            ws = torch.empty(nb // 4, device=x.device)
+            ws = torch.empty(nb, dtype=torch.uint8, device=x.device)
             wsp = ws.data_ptr()
     _launch(lib.grk_head_norm_bwd, 'grk_head_norm_bwd', dev, yp, yl, x.data_ptr(), x.stride(0), gp, gl, wp, bp, eps, N,
             heads, hd, _ROW_DTYPES[dt], dx.data_ptr(), dx.stride(0), dgp, dgl, dwp, dbp, wsp, nb)

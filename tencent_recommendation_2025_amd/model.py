@@ -1046,8 +1046,7 @@ class BaselineModel(torch.nn.Module):
         if slots is None:
             if n != stream.position.numel():
                 raise ValueError(f'{n} events for the {stream.position.numel()} users of the stream: slots needed')
-            pos = stream.position.clone()
-            stream.position += 1
+            pos, passed = stream.position.clone(), 1
         else:
             slots = slots.to(dev, torch.int64).contiguous()
             if slots.shape != (n,):
@@ -1056,10 +1055,11 @@ class BaselineModel(torch.nn.Module):
             at = torch.where(inside, slots, 0)
             earlier = torch.tril(slots[:, None] == slots[None, :], -1).sum(1)
             pos = stream.position[at] + earlier
-            stream.position.index_add_(0, at, inside.to(torch.int64))
+            passed = torch.zeros_like(stream.position).index_add_(0, at, inside.to(torch.int64))
         self.flush_tables()
         with self._inference_autocast():
-            seqs = self._stream_rows(ids, feature, token_type)
+            seqs = self._stream_rows(ids, feature, token_type)   # (features that it refuses leave the stream as it was)
+            stream.position += passed
 
             def layer(i, x):
                 y = self.attention_layers[i].step(x.reshape(n, -1), pos, stream.states[i], slots, stream.err)

@@ -126,6 +126,32 @@ def test_overlap_of_views():
     assert not K._overlap(b[1:], a) and K._overlap(buf[:, 16:48], b)
 
 
+def test_ranges_that_meet():
+    buf = torch.zeros(4, 2, 8, 8)
+    assert K._meet(buf, buf) and K._meet(buf[:3], buf[1:]) and not K._meet(buf[:2], buf[2:])
+    rows = buf.view(16, 32)
+    assert K._meet(rows[:, 16:], buf[3:]) and not K._meet(rows[:4, :16], buf[1:])
+    assert not K._meet(buf[:0], buf) and not K._meet(torch.zeros(4), buf)
+    # what is no matrix is refused by its shape, not compared
+    assert not K._overlap(torch.zeros(8), rows) and not K._overlap(rows, buf)
+
+
+def test_layers_refuse_columns_that_they_cannot_split():
+    pos, f = torch.zeros(4, dtype=torch.int64), torch.ones(4, dtype=torch.float64)
+    for cols in (100, 3 * 65):
+        with pytest.raises(L.GrkError, match='side by side'):
+            G.rotary_qk(torch.zeros(4, cols), pos, f, 2)
+    with pytest.raises(L.GrkError, match='freqs'):
+        G.rotary_qk(torch.zeros(4, 96), pos, f.clone().requires_grad_(True), 2)
+    w, lg = torch.ones(16), torch.zeros(2)
+    with pytest.raises(L.GrkError, match='side by side'):
+        G.decay_core(torch.zeros(4, 66), lg, w, w, 1, 4)
+    with pytest.raises(L.GrkError, match='side by side'):
+        G.decay_core(torch.zeros(4, 64), lg, w, None, 1, 4)
+    with pytest.raises(L.GrkError, match='log_decay'):
+        G.decay_core(torch.zeros(4, 64), lg.clone().requires_grad_(True), w, w, 1, 4)
+
+
 def test_rotary_frequencies():
     f, s = K.rotary_frequencies(8)
     assert f.dtype == torch.float64 and s == 1.0

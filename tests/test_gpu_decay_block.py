@@ -447,6 +447,43 @@ def test_decay_step_far_in_a_large_pool(K):
     close(pool[slots].view(2 * H, -1), sw.view(2 * H, -1), 300 * 2.0 ** -24)
 
 
+def test_a_decay_that_is_no_number_shows(K):
+    """NaN in log_decay reaches every later event of its head, and no other head."""
+    lg = torch.tensor([-0.1, float('nan')], device=DEV)
+    g = gen('nan decay')
+    for dt in DT.values():
+        q, k, v = (randn(g, 300, 2 * 32, dt=dt) for _ in range(3))
+        o, s = K.decay_attn_fwd(q, k, v, lg, 1, 300, return_state=True)
+        want = K.decay_attn_fwd(q, k, v, torch.full((2,), -0.1, device=DEV), 1, 300, return_state=True)[0]
+        assert torch.equal(o[:, :32], want[:, :32]) and bool(o[1:, 32:].isnan().all()) and bool(s[0, 1].isnan().all())
+        state = torch.ones(1, 2, 32, 32, device=DEV)
+        e = K.decay_attn_step(q[:1], k[:1], v[:1], lg, state)
+        assert bool(e[:, 32:].isnan().all()) and not bool(e[:, :32].isnan().any())
+        assert bool(state[:, 1].isnan().all()) and not bool(state[:, 0].isnan().any())
+
+
+def test_results_may_not_lie_on_operands(K):
+    from tencent_recommendation_2025_amd._lib import GrkError
+    lg = decays(2)
+    x = torch.zeros(10, 128, device=DEV)
+    pool = torch.zeros(4, 2, 64, 64, device=DEV)
+    in_pool = pool.view(-1, 128)[:10]
+    for bad in (lambda: K.decay_attn_fwd(x, x, x, lg, 2, 5, state=pool[:2], state_out=pool[1:3]),
+                lambda: K.decay_attn_fwd(x, x, in_pool, lg, 2, 5, state_out=pool[:2]),
+                lambda: K.decay_attn_fwd(x, x, x, lg, 2, 5, state=pool[:2], out=in_pool),
+                lambda: K.decay_attn_fwd(x, x, x, lg, 2, 5, state_out=pool[:2], out=in_pool),
+                lambda: K.decay_attn_step(x[:4], x[:4], x[:4], lg, pool, out=in_pool[:4]),
+                lambda: K.decay_attn_fwd(x, x, x, lg, 2, 5, out=x[0]),
+                lambda: K.rotary(x, torch.zeros(10, dtype=torch.int64, device=DEV),
+                                 torch.ones(32, dtype=torch.float64, device=DEV), 2, out=x[1]),
+                lambda: K.head_norm_bwd(x[0], x, None, None, 2, dx=torch.empty_like(x))):
+        with pytest.raises(GrkError):
+            bad()
+    # the states in place are fine
+    o, s = K.decay_attn_fwd(x, x, x, lg, 2, 5, state=pool[:2], return_state=True, state_out=pool[:2])
+    assert s.data_ptr() == pool.data_ptr()
+
+
 def test_decay_refusals(K):
     from tencent_recommendation_2025_amd._lib import GrkError
     lg = decays(2)
@@ -545,6 +582,21 @@ def test_head_norm_of_constant_and_empty_rows(K):
     assert dx.shape == (0, 64) and bool((dw == 0).all() and (db == 0).all())
     y = K.head_norm_fwd(x, w, b, 4, out=x)   # in place
     assert y is x and bool((x == 0.5).all())
+
+
+def test_head_norm_under_another_default_dtype(K):
+    """The weight gradients' workspace does not follow torch's default dtype."""
+    g = gen('default dtype')
+    x, dy, w = randn(g, 1000, 256), randn(g, 1000, 256), 1 + 0.2 * randn(g, 256)
+    want = K.head_norm_bwd(dy, x, w, w, 4)
+    kept = torch.get_default_dtype()
+    torch.set_default_dtype(torch.bfloat16)
+    try:
+        got = K.head_norm_bwd(dy, x, w, w, 4)
+    finally:
+        torch.set_default_dtype(kept)
+    for i in (0, 2, 3):
+        assert got[i].dtype == torch.float32 and torch.equal(got[i], want[i])
 
 
 def test_offsets_past_32_bits(K):
@@ -670,6 +722,35 @@ def test_graph_replays_match_eager(K, G):
             torch.cuda.synchronize()
             for a, b in zip(outs[i], eager):
                 assert torch.equal(a, b), (turn, i)
+
+
+def test_saved_rows_that_come_back_elsewhere(K, G):
+    """A gradient whose saved rows were kept on the host, from rows of a wider buffer: they
+    come back dense, maybe at their old address."""
+    g = gen('saved')
+    B, T, H, hd = 2, 70, 2, 32
+    wide = randn(g, B * T, 4 * H * hd, dt=torch.bfloat16)
+    qkv = wide[:, :3 * H * hd].detach().requires_grad_(True)
+    lg, do = decays(H), randn(g, B * T, H * hd, dt=torch.bfloat16)
+    want, = torch.autograd.grad(G.decay_attn(qkv, lg, B, T), qkv, do)
+    home = {}
+
+    def pack(t):
+        home[t.data_ptr()] = t
+        return t.data_ptr(), t.cpu().contiguous()
+
+    def unpack(kept):
+        at = home[kept[0]]
+        if at.shape != (B * T, 3 * H * hd):
+            return at
+        back = wide.view(-1)[:at.numel()].view(at.shape)   # the old address, another stride
+        back.copy_(kept[1])
+        return back
+
+    with torch.autograd.graph.saved_tensors_hooks(pack, unpack):
+        o = G.decay_attn(qkv, lg, B, T)
+    got, = torch.autograd.grad(o, qkv, do)
+    assert torch.equal(got, want)
 
 
 def test_another_stream(K):

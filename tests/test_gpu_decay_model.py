@@ -320,6 +320,18 @@ def test_stream_events_of_one_user_in_one_call_and_free_slots():
         both.check()
 
 
+def test_a_refused_event_leaves_the_stream():
+    m, batch, _ = make(B=2)
+    m.eval()
+    seq, tt, feat = batch[0], batch[3], batch[6]
+    _, s = m.stream_begin(seq, to_rows(feat, slice(0, seq.shape[1])), tt)
+    was = s.position.tolist()
+    for slots in (None, torch.tensor([0, 1], device=DEV)):
+        with pytest.raises(KeyError):
+            m.stream_step(s, seq[:, 0], {}, tt[:, 0], slots)   # (no features at all)
+    assert s.position.tolist() == was
+
+
 def test_stream_and_block_refusals():
     m, batch, _ = make(B=2)
     a = (batch[0], batch[6], batch[3])
