@@ -320,6 +320,50 @@ def test_stream_events_of_one_user_in_one_call_and_free_slots():
         both.check()
 
 
+def test_stream_step_in_a_graph():
+    """A captured step, replayed with eager work between: every replay has the eager step's
+    features, states and positions, events of one slot and empty events among its inputs."""
+    m, batch, _ = make(B=4)
+    m.eval()
+    seq, tt, feat = batch[0], batch[3], batch[6]
+    T = seq.shape[1]
+    cut = T - 6
+    head = slice(0, cut)
+    _, a = m.stream_begin(seq[:, head], to_rows(feat, head), tt[:, head], slots=6)
+    _, b = m.stream_begin(seq[:, head], to_rows(feat, head), tt[:, head], slots=6)
+    orders = torch.tensor([[0, 1, 2, 3], [2, 2, 0, -1], [5, 1, 1, 1], [3, 2, 1, 0]], device=DEV)
+    ids, kind, slots = seq[:, cut].clone(), tt[:, cut].clone(), orders[0].clone()
+    rows = {k: v[:, cut:cut + 1].clone() for k, v in feat.items()}
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    kept = [s.clone() for s in a.states], a.position.clone()
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            m.stream_step(a, ids, rows, kind, slots)
+    torch.cuda.current_stream().wait_stream(side)
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr):
+        out = m.stream_step(a, ids, rows, kind, slots)
+    for s, was in zip((*a.states, a.position), (*kept[0], kept[1])):
+        s.copy_(was)
+    for turn in range(4):
+        at = slice(cut + turn, cut + turn + 1)
+        ids.copy_(seq[:, cut + turn])
+        kind.copy_(tt[:, cut + turn])
+        slots.copy_(orders[turn])
+        for k, v in feat.items():
+            rows[k].copy_(v[:, at])
+        gr.replay()
+        torch.cuda.synchronize()
+        want = m.stream_step(b, ids, rows, kind, slots)
+        torch.cuda.synchronize()
+        live = slots >= 0
+        assert nrel(out[live], want[live]) < 2 * 2000 * 2.0 ** -24, turn
+        assert torch.equal(a.position, b.position), turn
+        for x, y in zip(a.states, b.states):
+            assert nrel(x, y) < 2 * 2000 * 2.0 ** -24, turn
+
+
 def test_a_refused_event_leaves_the_stream():
     m, batch, _ = make(B=2)
     m.eval()
