@@ -625,7 +625,8 @@ int grk_rotary(const void* x, int64_t ldx, void* y, int64_t ldy, int dtype, cons
  * they hold), their output and gradient rows are zero, and the state decays over
  * them.  seq_range (int32 [batch, 3], grk_seq_ranges; optional): the same for the
  * positions before seq_range[b][0], without reading key_valid there; it has to be this
- * key_valid's (a range it calls contiguous is taken to have no holes behind its start).
+ * key_valid's (a range it calls contiguous is taken to have no holes behind its start,
+ * and its order of the sequences to name each of them once).
  * A NaN or an infinity in an event reaches the outputs behind it, and may reach those
  * of up to 63 events before it.
  * row_base / num_rows / capacity: the packed rows of grk_attn_args (seq_range

@@ -15,8 +15,8 @@
 // 26 LDS accesses for 32 steps, half of the time that their 16 KB take from HBM on one CU
 // of 256; what is left is the wait of a chunk's two barriers, which the next chunk's loads
 // (to registers, while this one is computed) and 4 waves a SIMD cover in part.  128
-// sequences of up to 201 events (16 K packed rows) of 8 heads of 64: forward 19.6 us (66
-// MB, 3.4 TB/s), gradients 38.1 us (116 MB, 3.0 TB/s).  Heads of 128: LDS, read for every
+// sequences of up to 201 events (16 K packed rows) of 8 heads of 64: forward 18.4 us (66
+// MB, 3.6 TB/s), gradients 36.1 us (116 MB, 3.2 TB/s).  Heads of 128: LDS, read for every
 // operand of 4 products a chunk.  8 x 4096 events of 4 heads: 39 us and gradients 93 us
 // after 40 and 48 us for the segment states.
 //
@@ -422,7 +422,7 @@ bool decay_bf16_takes(const DecayParams& p) {
 }
 
 // Chunks of 32 steps for heads of up to 64 columns (128 sequences of up to 201 events,
-// 8 heads of 64: forward 19.6 us, with 64 steps 21.8), of 64 steps above (8 x 4096 events, 4
+// 8 heads of 64: forward 19.6 us, with 64 steps 22.0), of 64 steps above (8 x 4096 events, 4
 // heads of 128: gradients 93 us, with 32 steps 105).  Heads of 64: two column tiles a wave
 // halve what the waves read from LDS and pay once there are workgroups for two rounds
 // (the former's gradients, 3072 workgroups: 38.1 us, one tile 41.7); with fewer, more waves

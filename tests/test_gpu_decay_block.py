@@ -261,6 +261,28 @@ def test_decay_attn(K, G, B, T, H, hd, dt, mask):
     close(st.reshape(B * H, -1), want[1].reshape(B * H, -1), 300 * 2.0 ** -24)   # fp32 whatever the rows are
 
 
+@pytest.mark.parametrize('dt', list(DT))
+@pytest.mark.parametrize('T,hd', [(45, 64), (33, 40), (1, 56)])
+def test_decay_attn_many_sequences(K, T, hd, dt):
+    """More (sequence, head) pairs than workgroups that run at once, with states."""
+    dt = DT[dt]
+    B, H = 300, 7
+    g = gen('many', T, hd)
+    valid = mask_of('holes', B, T, g)
+    q, k, v, do = (randn(g, B * T, H * hd, dt=dt) for _ in range(4))
+    s0, lg = randn(g, B, H, hd, hd), decays(H)
+    heads = lambda x: x.view(B, T, H, hd)  # noqa: E731
+    kv = valid.to(torch.uint8)
+    want = decay_ref(heads(q), heads(k), heads(v), lg, valid, hd ** -0.5, state=s0)
+    o, s = K.decay_attn_fwd(q, k, v, lg, B, T, key_valid=kv, state=s0, return_state=True)
+    close(o, want[0], decay_tol(dt))
+    close(s.view(B * H, -1), want[1].view(B * H, -1), 300 * 2.0 ** -24)
+    want = decay_ref(heads(q), heads(k), heads(v), lg, valid, hd ** -0.5, heads(do))
+    close(K.decay_attn_fwd(q, k, v, lg, B, T, key_valid=kv), want[0], decay_tol(dt))
+    for a, b in zip(K.decay_attn_bwd(do, q, k, v, lg, B, T, key_valid=kv), want[2:]):
+        close(a, b, decay_tol(dt))
+
+
 def test_decay_attn_extreme_decays(K):
     """g = 1 (0, and above 0), g = 0 (-inf) and a decay that underflows inside a chunk."""
     lg = torch.tensor([0.0, 3.0, float('-inf'), -50.0], device=DEV)
@@ -350,6 +372,33 @@ def test_decay_attn_packed_rows(K, B, T, H, hd, dt):
     want = decay_ref(*(s.reshape(B, T, H, hd) for s in x.split(D, 1)), lg, valid, hd ** -0.5, do.view(B, T, H, hd))
     for a, b in zip((o, *d), (want[0], *want[2:])):
         close(a, b, decay_tol(dt))
+
+
+@pytest.mark.parametrize('dt', list(DT))
+def test_the_order_of_the_sequences_is_free(K, dt):
+    """Ranges list the sequences longest first; any order that names each once gives the
+    same bits, packed and padded, in one segment and in several."""
+    dt = DT[dt]
+    g = gen('order')
+    for B, T, H, hd in ((9, 70, 2, 32), (3, 1100, 1, 64)):
+        kv = mask_of('left', B, T, g)
+        kv[:, -1] = True
+        kv = kv.to(torch.uint8)
+        n = int(kv.sum())
+        rng, base, _, _ = K.jagged_layout(kv, n)
+        D = H * hd
+        x, do, lg = randn(g, n, 3 * D, dt=dt), randn(g, n, D, dt=dt), decays(H)
+        xp, dp = randn(g, B * T, 3 * D, dt=dt), randn(g, B * T, D, dt=dt)
+        got = []
+        for order in (rng[:, 2], torch.arange(B, device=DEV), torch.randperm(B, generator=g, device=DEV)):
+            r = rng.clone()
+            r[:, 2] = order
+            kw, kp = dict(key_valid=kv, seq_range=r, row_base=base), dict(key_valid=kv, seq_range=r)
+            got.append([K.decay_attn_fwd(*x.split(D, 1), lg, B, T, **kw), *K.decay_attn_bwd(do, *x.split(D, 1), lg, B, T, **kw),
+                        *K.decay_attn_fwd(*xp.split(D, 1), lg, B, T, return_state=True, **kp),
+                        *K.decay_attn_bwd(dp, *xp.split(D, 1), lg, B, T, **kp)])
+        for other in got[1:]:
+            assert all(torch.equal(a, b) for a, b in zip(got[0], other))
 
 
 def test_decay_attn_gradient_against_differences(G):
