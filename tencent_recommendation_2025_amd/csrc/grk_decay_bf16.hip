@@ -425,7 +425,7 @@ bool decay_bf16_takes(const DecayParams& p) {
 // 8 heads of 64: forward 19.6 us, with 64 steps 22.0), of 64 steps above (8 x 4096 events, 4
 // heads of 128: gradients 93 us, with 32 steps 105).  Heads of 64: two column tiles a wave
 // halve what the waves read from LDS and pay once there are workgroups for two rounds
-// (the former's gradients, 3072 workgroups: 38.1 us, one tile 41.7); with fewer, more waves
+// (the former's gradients, 3 x 1024 workgroups: 38.1 us, one tile 41.7); with fewer, more waves
 // hide more latency (forward, 1024 workgroups: 19.6 us, two tiles 20.9).  Heads of 128:
 // two tiles always (gradients 93 us, one tile 105).
 int decay_bf16_launch(const DecayParams& p, hipStream_t s) {
