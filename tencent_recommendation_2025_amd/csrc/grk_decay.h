@@ -82,6 +82,12 @@ __device__ __forceinline__ DecayPlace decay_place(const DecayParams& p, int part
   return w;
 }
 
+// Whether a later segment, or state_out, takes this one's sums (the workspace of the others is
+// never written, and the scan's sums with it are never used).
+__device__ __forceinline__ bool decay_state_used(const DecayParams& p, const DecayPlace& w) {
+  return p.state_out || w.t0 + p.seg_len < w.len;
+}
+
 // g^n for n >= 0 (g^0 = 1 also for g = 0).
 __device__ __forceinline__ float decay_pow(float lg, int n) { return n == 0 ? 1.f : expf(lg * (float)n); }
 

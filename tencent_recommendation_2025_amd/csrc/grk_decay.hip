@@ -89,7 +89,7 @@ __global__ void __launch_bounds__(DP * 4, 4) k_decay_f32(DecayParams p) {
   float* wv = pw - 16 + 16 + C + 4;             // g^(n-1-j): the weight of step j in the state
   int* slive = reinterpret_cast<int*>(wv + C);  // the step holds an event
   const DecayPlace w = decay_place(p);
-  if (!w.on) return;
+  if (!w.on || (STATE && !decay_state_used(p, w))) return;
   const DecayRole r = p.role[w.role];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = lane >> 4, c = lane & 15;

@@ -151,7 +151,7 @@ __global__ void __launch_bounds__(EW * 4 / NE, NE == 1 ? 4 : C == 32 ? 3 : 2) k_
   float* wv = pw - 16 + decay_powers<C>();
   int* slive = reinterpret_cast<int*>(wv + C);
   DecayPlace w = decay_place(p, DP / EW);
-  if (!w.on) return;
+  if (!w.on || (STATE && !decay_state_used(p, w))) return;
   const DecayRole r = p.role[w.role];
   const int64_t bh = (int64_t)w.b * p.heads + w.h, hcol = (int64_t)w.h * p.head_dim;
   const int64_t base = p.row_base ? p.row_base[w.b] : (int64_t)w.b * p.seq_len;
