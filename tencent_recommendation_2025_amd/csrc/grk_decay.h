@@ -48,6 +48,7 @@ __device__ __forceinline__ float decay_log(float lg) { return lg > 0.f ? 0.f : l
 // One workgroup's pass: a role, a (sequence, head) and a segment of it.
 struct DecayPlace {
   int b, h, seg, role, part;       // part: its columns of the state and the output, where they are shared out
+  int64_t base;                    // row of position 0
   int start, len;                  // first position of the sequence, its steps
   int t0, t1;                      // steps of the segment
   float lg;                        // log g <= 0
@@ -73,6 +74,7 @@ __device__ __forceinline__ DecayPlace decay_place(const DecayParams& p, int part
     const int by_length = p.seq_range[3 * (int64_t)w.b + 2];
     if ((unsigned)by_length < (unsigned)p.batch) w.b = by_length;
   }
+  w.base = p.row_base ? p.row_base[w.b] : (int64_t)w.b * p.seq_len;
   int s = p.seq_range ? p.seq_range[3 * (int64_t)w.b] : 0;
   w.start = s < 0 ? 0 : (s > p.seq_len ? p.seq_len : s);
   w.len = p.seq_len - w.start;
@@ -91,23 +93,11 @@ __device__ __forceinline__ bool decay_state_used(const DecayParams& p, const Dec
 // g^n for n >= 0 (g^0 = 1 also for g = 0).
 __device__ __forceinline__ float decay_pow(float lg, int n) { return n == 0 ? 1.f : expf(lg * (float)n); }
 
-// Row of step t, or -1 when the step holds nothing (masked, or past the segment).
+// Row of step t, masked or not, or -1 past the segment (or where no row exists).
 __device__ __forceinline__ int64_t decay_row(const DecayParams& p, const DecayPlace& w, int rev, int t) {
   if (t >= w.t1) return -1;
   const int pos = rev ? p.seq_len - 1 - t : w.start + t;
-  if (p.key_valid && !p.key_valid[(int64_t)w.b * p.seq_len + pos]) return -1;
-  const int64_t row = (p.row_base ? p.row_base[w.b] : (int64_t)w.b * p.seq_len) + pos;
-  return row >= 0 && row < p.capacity ? row : -1;
-}
-
-// Same, for the output: the row also of a masked step (it gets zeros).
-__device__ __forceinline__ int64_t decay_out_row(const DecayParams& p, const DecayPlace& w, int rev, int t,
-                                                 bool* live) {
-  *live = false;
-  if (t >= w.t1) return -1;
-  const int pos = rev ? p.seq_len - 1 - t : w.start + t;
-  *live = !p.key_valid || p.key_valid[(int64_t)w.b * p.seq_len + pos];
-  const int64_t row = (p.row_base ? p.row_base[w.b] : (int64_t)w.b * p.seq_len) + pos;
+  const int64_t row = w.base + pos;
   return row >= 0 && row < p.capacity ? row : -1;
 }
 

@@ -43,11 +43,27 @@ template <typename T, int V, int DP>
 struct DecayRowsF32 {
   typedef typename DecayRaw<T, V>::type raw;
   static constexpr int NTH = DP * 4, U = DP / V, R = NTH / U, N = kF32Chunk / R;
-  int64_t row[N];   // -1: no event there
+  int64_t row[N];    // -1: no step there
+  bool inside[N];    // (whether there is: kept longer than row)
+  unsigned mask[N];  // its byte of key_valid, as it comes from memory (looked at when the row is laid down)
   __device__ __forceinline__ void chunk(const DecayParams& p, const DecayPlace& w, int rev, int t0) {
 #pragma unroll
-    for (int k = 0; k < N; ++k) row[k] = decay_row(p, w, rev, t0 + (int)threadIdx.x / U + R * k);
+    for (int k = 0; k < N; ++k) {
+      row[k] = decay_row(p, w, rev, t0 + (int)threadIdx.x / U + R * k);
+      inside[k] = row[k] >= 0;
+      mask[k] = 1;
+    }
+    if (p.key_valid) {
+      const uint8_t* q = p.key_valid + (int64_t)w.b * p.seq_len;
+#pragma unroll
+      for (int k = 0; k < N; ++k) {
+        int t = t0 + (int)threadIdx.x / U + R * k;
+        t = t < w.t1 ? t : w.t1 - 1;
+        mask[k] = q[rev ? p.seq_len - 1 - t : w.start + t];
+      }
+    }
   }
+  __device__ __forceinline__ bool live(int k) const { return inside[k] && mask[k] != 0; }   // it holds an event
   __device__ __forceinline__ void load(raw* f, const void* src, int64_t ld, int64_t hcol, int head_dim) const {
     const int c = (int)threadIdx.x % U * V;
 #pragma unroll
@@ -60,8 +76,9 @@ struct DecayRowsF32 {
   __device__ __forceinline__ void store(const raw* f, float* dst) const {
 #pragma unroll
     for (int k = 0; k < N; ++k) {
+      const raw z = live(k) ? f[k] : raw{};
       T t[V];
-      __builtin_memcpy(t, &f[k], sizeof(raw));
+      __builtin_memcpy(t, &z, sizeof(raw));
       float* d = dst + ((int)threadIdx.x / U + R * k) * (DP + kF32Pad) + (int)threadIdx.x % U * V;
       if constexpr (V == 4) *reinterpret_cast<float4*>(d) = make_float4(to_f32(t[0]), to_f32(t[1]), to_f32(t[2]), to_f32(t[3]));
       else *d = to_f32(t[0]);
@@ -130,6 +147,9 @@ __global__ void __launch_bounds__(DP * 4, 4) k_decay_f32(DecayParams p) {
   };
   weights(C);
   const float gc = decay_pow(w.lg, C);
+  // (the state's loads are waited for before the loop: grk_decay_bf16.hip)
+#pragma unroll
+  for (int dt = 0; dt < NT; ++dt) asm volatile("" : "+v"(st[dt]));
   // A chunk: its rows to LDS | P, what the output takes from the state, the state's step |
   // the output.  Behind the second barrier only P (and V, kept in registers) is read.
   for (int t0 = w.t0; t0 < w.t1; t0 += C) {
@@ -141,7 +161,7 @@ __global__ void __launch_bounds__(DP * 4, 4) k_decay_f32(DecayParams p) {
       rows.store(fa, sa);
       if ((int)threadIdx.x % Rows::U == 0) {
 #pragma unroll
-        for (int k = 0; k < Rows::N; ++k) slive[(int)threadIdx.x / Rows::U + Rows::R * k] = rows.row[k] >= 0;
+        for (int k = 0; k < Rows::N; ++k) slive[(int)threadIdx.x / Rows::U + Rows::R * k] = rows.live(k);
       }
     }
     __syncthreads();
@@ -212,8 +232,7 @@ __global__ void __launch_bounds__(DP * 4, 4) k_decay_f32(DecayParams p) {
 #pragma unroll
         for (int jt = 0; jt <= it; ++jt)
           mfma16(v[jt], *reinterpret_cast<const f32x4*>(sp + (16 * it + c) * PT + 16 * jt + 4 * g), o[it]);
-        bool event;
-        const int64_t row = decay_out_row(p, w, r.rev, t0 + 16 * it + c, &event);
+        const int64_t row = decay_row(p, w, r.rev, t0 + 16 * it + c);
         const int e = 16 * wave + 4 * g;
         if (row >= 0 && e < p.head_dim) {
           T* dst = reinterpret_cast<T*>(r.out) + row * r.ldo + hcol + e;

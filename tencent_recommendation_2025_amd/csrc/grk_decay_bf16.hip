@@ -15,10 +15,10 @@
 // 26 LDS accesses for 32 steps, half of the time that their 16 KB take from HBM on one CU
 // of 256; what is left is the wait of a chunk's two barriers, which the next chunk's loads
 // (to registers, while this one is computed) and 4 waves a SIMD cover in part.  128
-// sequences of up to 201 events (16 K packed rows) of 8 heads of 64: forward 18.4 us (66
-// MB, 3.6 TB/s), gradients 36.1 us (116 MB, 3.2 TB/s).  Heads of 128: LDS, read for every
-// operand of 4 products a chunk.  8 x 4096 events of 4 heads: 39 us and gradients 93 us
-// after 40 and 48 us for the segment states.
+// sequences of up to 201 events (16 K packed rows) of 8 heads of 64: forward 17.3 us (66
+// MB, 3.8 TB/s), gradients 36.2 us (116 MB, 3.2 TB/s).  Heads of 128: LDS, read for every
+// operand of 4 products a chunk.  8 x 4096 events of 4 heads: 40 us and gradients 90 us
+// after 40 and 45 us for the segment states.
 //
 // LDS rows are 16 bytes longer than the head: 16 rows' 16-byte pieces fall on all 64 banks
 // at once, every address is a lane's base plus a constant, and a transposing read that
@@ -96,13 +96,15 @@ __device__ __forceinline__ int decay_first_row() {
 // its first row and of every R-th after it, R = threads / (DP / 8).  The chunk's lowest
 // row is a uniform pointer, a lane's offset from it 32 bits (the host admits row strides
 // below 2^24 elements).  Masked steps are loaded too (their row exists) and zeroed by
-// selection, so the loads do not wait for the mask.
+// selection when they are laid down: nothing waits for the mask before that (3 x 8191
+// events, 8 heads of 64, a mask: 25.4 us -> 24.2).
 template <int DP, int NTH, int C>
 struct DecayRows {
   static constexpr int R = NTH / (DP / 8), N = C / R;
   static_assert(N * R == C, "whole turns");
   unsigned at[N];    // the row's place above the chunk's lowest
-  bool live[N];      // it holds an event
+  bool inside[N];    // the step is one of the chunk's
+  unsigned mask[N];  // its byte of key_valid, as it comes from memory
   int64_t low;       // the chunk's lowest row
   __device__ __forceinline__ void chunk(const DecayParams& p, const DecayPlace& w, int rev, int64_t base, bool masked,
                                         int t0) {
@@ -113,10 +115,16 @@ struct DecayRows {
     for (int k = 0; k < N; ++k) {
       const int t = decay_first_row<DP>() + R * k, s = t < n ? t : n - 1;
       at[k] = rev ? n - 1 - s : s;
-      live[k] = t < n;
-      if (masked) live[k] = live[k] && p.key_valid[(int64_t)w.b * p.seq_len + pos0 + at[k]] != 0;
+      inside[k] = t < n;
+      mask[k] = 1;
+    }
+    if (masked) {
+      const uint8_t* q = p.key_valid + (int64_t)w.b * p.seq_len + pos0;
+#pragma unroll
+      for (int k = 0; k < N; ++k) mask[k] = q[at[k]];
     }
   }
+  __device__ __forceinline__ bool live(int k) const { return inside[k] && mask[k] != 0; }   // it holds an event
   __device__ __forceinline__ void load(uint4* f, const void* src, int64_t ld, int64_t col, int ccol) const {
     const char* q = reinterpret_cast<const char*>(src) + (low * ld + col) * 2;
 #pragma unroll
@@ -127,7 +135,7 @@ struct DecayRows {
 #pragma unroll
     for (int k = 0; k < N; ++k)
       *reinterpret_cast<uint4*>(dst + (decay_first_row<DP>() + R * k) * decay_stride<DP>() +
-                                (int)threadIdx.x % (DP / 8) * 16) = live[k] && has ? f[k] : make_uint4(0u, 0u, 0u, 0u);
+                                (int)threadIdx.x % (DP / 8) * 16) = live(k) && has ? f[k] : make_uint4(0u, 0u, 0u, 0u);
   }
 };
 
@@ -154,7 +162,7 @@ __global__ void __launch_bounds__(EW * 4 / NE, NE == 1 ? 4 : C == 32 ? 3 : 2) k_
   if (!w.on || (STATE && !decay_state_used(p, w))) return;
   const DecayRole r = p.role[w.role];
   const int64_t bh = (int64_t)w.b * p.heads + w.h, hcol = (int64_t)w.h * p.head_dim;
-  const int64_t base = p.row_base ? p.row_base[w.b] : (int64_t)w.b * p.seq_len;
+  const int64_t base = w.base;
   if (base + w.start < 0 || base + p.seq_len > p.capacity) w.t1 = w.t0;   // rows that do not exist: no step
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = lane >> 4, c = lane & 15;
@@ -218,6 +226,12 @@ __global__ void __launch_bounds__(EW * 4 / NE, NE == 1 ? 4 : C == 32 ? 3 : 2) k_
     for (int n = threadIdx.x; n < C * PS / 16; n += NTH) reinterpret_cast<uint4*>(sp)[n] = make_uint4(0u, 0u, 0u, 0u);
     if (w.part == 0) decay_zero_rows<bf16_t>(p, w, r);
   }
+  // The state's loads are waited for here, by a use that is none: left to its first use in the
+  // loop, every chunk would wait there for the next chunk's rows as well (18.5 us, not 17.3).
+#pragma unroll
+  for (int x = 0; x < NE; ++x)
+#pragma unroll
+    for (int dt = 0; dt < NT; ++dt) asm volatile("" : "+v"(st[x][dt]));
   const int row_b = c * ST + 16 * g, col_b = decay_col_base<ST>(lane);   // this lane's LDS bases
   // A chunk: its rows to LDS | P, what the output takes from the state, the state's step |
   // the output.  Two barriers: behind the second one only P is read, so the next chunk's
@@ -231,7 +245,7 @@ __global__ void __launch_bounds__(EW * 4 / NE, NE == 1 ? 4 : C == 32 ? 3 : 2) k_
       rows.store(fa, sa, has);
       if (rcol == 0) {
 #pragma unroll
-        for (int k = 0; k < Rows::N; ++k) slive[decay_first_row<DP>() + Rows::R * k] = rows.live[k];
+        for (int k = 0; k < Rows::N; ++k) slive[decay_first_row<DP>() + Rows::R * k] = rows.live(k);
       }
     }
     const int64_t low = rows.low;
@@ -266,8 +280,6 @@ __global__ void __launch_bounds__(EW * 4 / NE, NE == 1 ? 4 : C == 32 ? 3 : 2) k_
 #pragma unroll
       for (int it = 0; it < C / 16; ++it) {
         live[it] = slive[16 * it + c];
-#pragma unroll
-        for (int x = 0; x < NE; ++x) o[it][x] = f32x4{0.f, 0.f, 0.f, 0.f};
       }
       if (some) {
         bf16x8 sf[NE][KS];
@@ -285,12 +297,20 @@ __global__ void __launch_bounds__(EW * 4 / NE, NE == 1 ? 4 : C == 32 ? 3 : 2) k_
           for (int ks = 0; ks < KS; ++ks) {
             const bf16x8 q = lds_row_pair(sa + c * ST + 8 * g + 16 * it * ST + 64 * ks);
 #pragma unroll
-            for (int x = 0; x < NE; ++x) mfma32(sf[x][ks], q, o[it][x]);
+            for (int x = 0; x < NE; ++x) {
+              if (ks == 0) o[it][x] = f32x4{0.f, 0.f, 0.f, 0.f};
+              mfma32(sf[x][ks], q, o[it][x]);
+            }
           }
           const float rise = pw[16 * it + c + 1];
 #pragma unroll
           for (int x = 0; x < NE; ++x) o[it][x] *= rise;
         }
+      } else {
+#pragma unroll
+        for (int it = 0; it < C / 16; ++it)
+#pragma unroll
+          for (int x = 0; x < NE; ++x) o[it][x] = f32x4{0.f, 0.f, 0.f, 0.f};
       }
     }
     if (STATE || !last || (p.nseg == 1 && p.state_out)) {   // (nothing reads the state behind the last chunk else)
@@ -317,9 +337,12 @@ __global__ void __launch_bounds__(EW * 4 / NE, NE == 1 ? 4 : C == 32 ? 3 : 2) k_
           for (int s = 0; s < 8; ++s) f[s] = (float)vf[x][ks][s] * (s < 4 ? w0[s & 3] : w1[s & 3]);
 #pragma unroll
           for (int q = 0; q < NS; ++q) {
-            part[x][q] = pack8(f);
+            uint4 y = __builtin_bit_cast(uint4, pack8(f));
+            asm("" : "+v"(y.x), "+v"(y.y), "+v"(y.z), "+v"(y.w));   // (else the compiler rounds each again to subtract it)
+            part[x][q] = __builtin_bit_cast(bf16x8, y);
+            const unsigned u[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
-            for (int s = 0; s < 8; ++s) f[s] -= (float)part[x][q][s];
+            for (int s = 0; s < 8; ++s) f[s] -= __uint_as_float(s & 1 ? u[s / 2] & 0xffff0000u : u[s / 2] << 16);
           }
         }
 #pragma unroll
