@@ -145,7 +145,7 @@ struct DecayRows {
 // rounding of 2^-9 into every output, which then lay 1.6 times as far from the exact one as
 // its own rounding; with two it is 1.4 times.
 template <int DP, int EW, int NE, int C, int NS, bool STATE>
-__global__ void __launch_bounds__(EW * 4 / NE, NE == 1 ? 4 : C == 32 ? 3 : 2) k_decay_bf16(DecayParams p) {
+__global__ void __launch_bounds__(EW * 4 / NE, NE == 1 ? 4 : 2) k_decay_bf16(DecayParams p) {
   constexpr int CK = C / 32, NT = DP / 16, KS = DP / 32, NW = EW / 16 / NE, NTH = NW * 64;
   constexpr int ST = decay_stride<DP>(), SE = decay_stride<EW>(), PS = decay_stride<C>();
   using Rows = DecayRows<DP, NTH, C>;    // of a and b
@@ -446,16 +446,14 @@ bool decay_bf16_takes(const DecayParams& p) {
 
 // Chunks of 32 steps for heads of up to 64 columns (128 sequences of up to 201 events,
 // 8 heads of 64: forward 19.6 us, with 64 steps 22.0), of 64 steps above (8 x 4096 events, 4
-// heads of 128: gradients 93 us, with 32 steps 105).  Heads of 64: two column tiles a wave
-// halve what the waves read from LDS and pay once there are workgroups for two rounds
-// (the former's gradients, 3 x 1024 workgroups: 38.1 us, one tile 41.7); with fewer, more waves
-// hide more latency (forward, 1024 workgroups: 19.6 us, two tiles 20.9).  Heads of 128:
-// two tiles always (gradients 93 us, one tile 105).
+// heads of 128: gradients 91 us, with 32 steps and one tile a wave 95).  Two column tiles a
+// wave halve what the waves read from LDS: taken where that bounds them, at 128 columns (the
+// same 91 us, one tile 104); at 64 more waves hide more latency (the former's forward 17.3
+// us, two tiles 19.2; its gradients 36 us with either).
 int decay_bf16_launch(const DecayParams& p, hipStream_t s) {
   if (p.head_dim <= 32) return decay_bf16_run<32, 1, 32>(p, s);
-  if (p.head_dim > 64) return decay_bf16_run<128, 2, 64>(p, s);
-  if ((int64_t)p.roles * p.batch * p.heads * p.nseg >= 2048) return decay_bf16_run<64, 2, 32>(p, s);
-  return decay_bf16_run<64, 1, 32>(p, s);
+  if (p.head_dim <= 64) return decay_bf16_run<64, 1, 32>(p, s);
+  return decay_bf16_run<128, 2, 64>(p, s);
 }
 
 }  // namespace grk
