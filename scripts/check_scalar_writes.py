@@ -1,10 +1,9 @@
 #!/usr/bin/env python
-"""Build guard: no GPU code object of libgrk writes memory through the scalar
-data cache (scalar stores or scalar atomics, or that cache's write-back /
-discard).  The compiler is not expected to emit any for this code; runs of
-such code on this pool were followed by machine resets, so the build checks
-the disassembly instead of trusting that.  Host-only checker: listed in
-.gpurunignore (it names the instructions it looks for).
+"""Build guard: the scalar memory instructions of libgrk's GPU code objects read,
+and do nothing else.  A write through the scalar data cache is not expected of the
+compiler for this code; the build looks at the disassembly instead of trusting
+that.  What is not in the list below fails, so it names no instruction that may
+not be there.
 
     python scripts/check_scalar_writes.py build/obj/grk_*.o
 """
@@ -15,16 +14,23 @@ import sys
 sys.path.insert(0, os.path.dirname(os.path.abspath(__file__)))
 from check_mfma_overlap import disassemble  # noqa: E402
 
-PATTERN = re.compile(r'^\s+(s_store_\w+|s_buffer_store_\w+|s_scratch_store_\w+|s_atomic_\w+|s_buffer_atomic_\w+|'
-                     r's_dcache_wb\w*|s_dcache_discard\w*)\b', re.M)
+SMEM = 0b110000   # bits 31..26 of a scalar memory instruction's first word (gfx9)
+READS = re.compile(r'(s_load|s_buffer_load|s_scratch_load)_dword(x\d+)?|s_memtime|s_memrealtime')
+LINE = re.compile(r'^\s+(\w+)[^\n]*//\s*[0-9A-F]+:\s*([0-9A-F]{8})', re.M)
+
+
+def scalar_memory(disasm_text):
+    """Mnemonics of the scalar memory instructions, told by their encoding."""
+    return [m.group(1) for m in LINE.finditer(disasm_text) if int(m.group(2), 16) >> 26 == SMEM]
 
 
 def scalar_writes(obj):
-    """[(mnemonic, count)] of scalar-cache writes in one object's GPU code."""
-    found = {}
-    for m in PATTERN.finditer(disassemble(obj)):
-        found[m.group(1)] = found.get(m.group(1), 0) + 1
-    return sorted(found.items())
+    """[(mnemonic, count)] of the scalar memory instructions of one object's GPU code
+    that are not plain reads."""
+    seen = scalar_memory(disassemble(obj))
+    if not seen:   # every kernel reads its arguments this way
+        raise ValueError(f'{obj}: no scalar memory instruction found (another disassembly format?)')
+    return sorted((n, seen.count(n)) for n in set(seen) if not READS.fullmatch(n))
 
 
 def main(paths):
