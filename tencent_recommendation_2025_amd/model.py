@@ -61,9 +61,13 @@ class Rotary:
     def at(self, positions):
         """(positions, freqs, layout, scale) on the positions' device."""
         dev = positions.device
-        if dev not in self._on:
-            self._on[dev] = self._freqs.to(dev)
-        return positions, self._on[dev], self.layout, self.scale
+        freqs = self._on.get(dev)
+        if freqs is None:
+            # an ordinary tensor, also where the first call comes under inference mode: later
+            # forwards save it for their backward
+            with torch.inference_mode(False):
+                freqs = self._on[dev] = self._freqs.to(dev, copy=True)
+        return positions, freqs, self.layout, self.scale
 
 
 class FlashMultiHeadAttention(torch.nn.Module):
