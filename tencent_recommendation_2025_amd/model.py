@@ -1003,6 +1003,7 @@ class BaselineModel(torch.nn.Module):
         return self._embed(seq, seq_feature, mask=mask, include_user=True, with_pos=False,
                            combine=(self.item_emb.embedding_dim ** 0.5, 0.0))[0]
 
+    @torch.inference_mode(False)   # (the states outlive the call: later steps write them in any mode)
     @torch.no_grad()
     def stream_begin(self, log_seqs, seq_feature, mask, slots=None):
         """Read B users' events [B, T] (left-padded, as predict takes them) into kept states:

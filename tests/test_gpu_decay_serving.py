@@ -56,3 +56,25 @@ def test_trainer_after_predict_under_inference_mode():
             m.train()
         losses.append(torch.stack([tr.step(batch).clone() for _ in range(3)]))
     assert torch.equal(*losses)
+
+
+def test_a_stream_begun_under_inference_mode_goes_on_outside():
+    m, batch, _ = make(B=3)
+    m.eval()
+    seq, tt, feat = batch[0], batch[3], batch[6]
+    T = seq.shape[1]
+    head, last = slice(0, T - 1), slice(T - 1, T)
+    _, plain = m.stream_begin(seq[:, head], to_rows(feat, head), tt[:, head])
+    want = m.stream_step(plain, seq[:, -1], to_rows(feat, last), tt[:, -1])
+    with torch.inference_mode():
+        first, stream = m.stream_begin(seq[:, head], to_rows(feat, head), tt[:, head], slots=4)
+    got = m.stream_step(stream, seq[:, -1], to_rows(feat, last), tt[:, -1], torch.arange(3, device=DEV))
+    assert nrel(got, want) < TOL and stream.position.tolist() == [T, T, T, 0]
+    stream.place(torch.tensor([3, 1, 0], device=DEV), plain)
+    stream.clear(torch.tensor([2], device=DEV))
+    assert stream.position.tolist() == [T, T, 0, T] and torch.equal(stream.states[0][3], plain.states[0][0])
+    stream.check()
+    with torch.inference_mode():   # and back under it
+        m.stream_step(stream, seq[:1, -1], to_rows({k: v[:1] for k, v in feat.items()}, last), tt[:1, -1],
+                      torch.tensor([2], device=DEV))
+    assert stream.position.tolist() == [T, T, 1, T]
