@@ -1042,21 +1042,29 @@ class BaselineModel(torch.nn.Module):
         dicts) of their features as [n, 1] sequences, slots int64 [n] the users' (None: the
         stream's in order).  Returns the features [n, D] behind the events, what predict
         gives for the longer history.  Events of one slot in a call are that user's next
-        events in order; a negative slot holds no event."""
+        events in order.  A negative slot holds no event, and neither does token_type 0
+        (padding): such a row leaves its user's states and position as they are, and its
+        features say nothing."""
         if self.training:
             raise RuntimeError('stream_step: call eval() first')
         dev = self._device()
         ids, token_type = ids.reshape(-1, 1), token_type.reshape(-1, 1)
         n = ids.shape[0]
+        if token_type.shape[0] != n:
+            raise ValueError(f'{n} events, {token_type.shape[0]} token types')
+        event = token_type.to(dev).reshape(-1) != 0
         if slots is None:
             if n != stream.position.numel():
                 raise ValueError(f'{n} events for the {stream.position.numel()} users of the stream: slots needed')
-            pos, passed = stream.position.clone(), 1
+            slots = torch.where(event, torch.arange(n, device=dev), -1)
+            pos, passed = stream.position.clone(), event.to(torch.int64)
         else:
             slots = slots.to(dev, torch.int64).contiguous()
             if slots.shape != (n,):
                 raise ValueError(f'{n} events, slots of shape {tuple(slots.shape)}')
             inside = (slots >= 0) & (slots < stream.position.numel())
+            slots = torch.where(inside & ~event, -1, slots)   # (one outside the stream is still named by check)
+            inside = inside & event
             at = torch.where(inside, slots, 0)
             earlier = torch.tril(slots[:, None] == slots[None, :], -1).sum(1)
             pos = stream.position[at] + earlier

@@ -78,3 +78,68 @@ def test_a_stream_begun_under_inference_mode_goes_on_outside():
         m.stream_step(stream, seq[:1, -1], to_rows({k: v[:1] for k, v in feat.items()}, last), tt[:1, -1],
                       torch.tensor([2], device=DEV))
     assert stream.position.tolist() == [T, T, 1, T]
+
+
+@pytest.mark.parametrize('by_slots', [False, True])
+def test_rows_without_an_event_leave_their_user(by_slots):
+    """token_type 0 is padding, to a step as to predict: the row's user keeps states and
+    position, the others get what a step of their own gives them, and the next event follows
+    predict on the history without the row."""
+    m, batch, _ = make(B=4)
+    m.eval()
+    seq, tt, feat = batch[0], batch[3].clone(), batch[6]
+    T = seq.shape[1]
+    head, last = slice(0, T - 1), slice(T - 1, T)
+    _, s = m.stream_begin(seq[:, head], to_rows(feat, head), tt[:, head])
+    kept, was = [x.clone() for x in s.states], s.position.clone()
+    kind = tt[:, -1].clone()
+    assert bool((kind > 0).all())
+    kind[1] = kind[3] = 0
+    order = torch.arange(4, device=DEV) if by_slots else None
+    got = m.stream_step(s, seq[:, -1], to_rows(feat, last), kind, order)
+    want = m.predict(seq, feat, tt)
+    for u in range(4):
+        if kind[u] == 0:
+            assert all(torch.equal(x[u], k[u]) for x, k in zip(s.states, kept)) and s.position[u] == was[u]
+        else:
+            assert nrel(got[u], want[u]) < TOL and s.position[u] == was[u] + 1
+    late = torch.tensor([1, 3], device=DEV)
+    got = m.stream_step(s, seq[late, -1], {k: v[late, -1:] for k, v in feat.items()}, tt[late, -1], late)
+    assert nrel(got, want[late]) < TOL
+    s.check()
+
+
+def test_padding_between_the_events_of_one_user():
+    m, batch, _ = make(B=2)
+    m.eval()
+    seq, tt, feat = batch[0], batch[3], batch[6]
+    T = seq.shape[1]
+    head = slice(0, T - 2)
+    _, a = m.stream_begin(seq[:, head], to_rows(feat, head), tt[:, head])
+    _, b = m.stream_begin(seq[:, head], to_rows(feat, head), tt[:, head])
+    at = torch.tensor([T - 2, T - 1], device=DEV)
+    user = torch.zeros(2, dtype=torch.int64, device=DEV)
+    want = m.stream_step(a, seq[user, at], {k: v[user, at][:, None] for k, v in feat.items()}, tt[user, at], user)
+    at, user = torch.tensor([T - 2, T - 2, T - 1], device=DEV), torch.zeros(3, dtype=torch.int64, device=DEV)
+    kind = tt[user, at].clone()
+    kind[1] = 0
+    got = m.stream_step(b, seq[user, at], {k: v[user, at][:, None] for k, v in feat.items()}, kind, user)
+    assert nrel(got[[0, 2]], want) < TOL and a.position.tolist() == b.position.tolist() == [T, T - 2]
+    for x, y in zip(a.states, b.states):
+        assert nrel(x, y) < TOL
+    # a slot outside the stream is named all the same
+    m.stream_step(b, seq[:1, 0], {k: v[:1, :1] for k, v in feat.items()}, torch.zeros_like(tt[:1, 0]),
+                  torch.tensor([7], device=DEV))
+    with pytest.raises(ValueError):
+        b.check()
+
+
+def test_token_types_of_another_count_are_refused():
+    m, batch, _ = make(B=2)
+    m.eval()
+    seq, tt, feat = batch[0], batch[3], batch[6]
+    _, s = m.stream_begin(seq, feat, tt)
+    was = s.position.tolist()
+    with pytest.raises(ValueError):
+        m.stream_step(s, seq[:, 0], to_rows(feat, slice(0, 1)), tt[:1, 0])
+    assert s.position.tolist() == was
