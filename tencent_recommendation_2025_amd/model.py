@@ -352,6 +352,19 @@ class DecayAttention(torch.nn.Module):
                                                                            err_flag=err_flag))
 
 
+def _earlier_of_slot(slots, most):
+    """int64 [n]: how many entries before each one of ``slots`` (int64 [n] in [0, most],
+    most < 2^31) are equal to it.  Few are compared pair by pair, more of them by a stable
+    sort: n^2 bytes against some 100 n."""
+    n = slots.shape[0]
+    if n <= 256:
+        return torch.tril(slots[:, None] == slots[None, :], -1).sum(1)
+    index = torch.arange(n, device=slots.device)
+    with torch.cuda.device(slots.device):
+        run, order = K.sort_pairs(slots.to(torch.int32), index, end_bit=max(1, most.bit_length()))
+    return torch.empty_like(slots).scatter_(0, order, index - torch.searchsorted(run, run))
+
+
 class DecayStream:
     """What BaselineModel.stream_begin keeps of its users: of each layer the states
     (fp32 [slots, heads, head_dim, head_dim]), the position of each user's next event and a
@@ -1016,7 +1029,7 @@ class BaselineModel(torch.nn.Module):
         dev = self._device()
         B, T = log_seqs.shape
         n = B if slots is None else int(slots)
-        if n < B:
+        if not B <= n < 1 << 31:
             raise ValueError(f'{n} slots for {B} users')
         self.flush_tables()
         with self._inference_autocast():
@@ -1066,8 +1079,8 @@ class BaselineModel(torch.nn.Module):
             slots = torch.where(inside & ~event, -1, slots)   # (one outside the stream is still named by check)
             inside = inside & event
             at = torch.where(inside, slots, 0)
-            earlier = torch.tril(slots[:, None] == slots[None, :], -1).sum(1)
-            pos = stream.position[at] + earlier
+            pos = stream.position[at] + _earlier_of_slot(torch.where(inside, slots, stream.position.numel()),
+                                                         stream.position.numel())
             passed = torch.zeros_like(stream.position).index_add_(0, at, inside.to(torch.int64))
         self.flush_tables()
         with self._inference_autocast():

@@ -143,3 +143,66 @@ def test_token_types_of_another_count_are_refused():
     with pytest.raises(ValueError):
         m.stream_step(s, seq[:, 0], to_rows(feat, slice(0, 1)), tt[:1, 0])
     assert s.position.tolist() == was
+
+
+@pytest.mark.parametrize('n,pool', [(1, 1), (7, 3), (256, 40), (257, 40), (5000, 1), (5000, 300), (70001, 2 ** 17 - 1),
+                                    (70001, 2 ** 31 - 1)])
+def test_earlier_events_of_a_slot(n, pool):
+    """Counted without an n^2 buffer: 200 bytes an event at most beside the sort's own counts
+    (8 KB for 1024 events)."""
+    from tencent_recommendation_2025_amd.model import _earlier_of_slot
+    g = torch.Generator(device=DEV).manual_seed(n)
+    slots = torch.randint(0, pool, (n,), generator=g, device=DEV)
+    slots[torch.rand(n, generator=g, device=DEV) < 0.1] = pool
+    seen, want = {}, []
+    for s in slots.tolist():
+        want.append(seen.get(s, 0))
+        seen[s] = want[-1] + 1
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    got = _earlier_of_slot(slots, pool)
+    assert got.dtype == torch.int64 and got.tolist() == want
+    assert torch.cuda.max_memory_allocated() - before < 210 * n + (1 << 20)
+
+
+def test_many_events_in_one_step():
+    """900 events of 6 users in one call, in a graph too: the users' states are those of 150
+    calls, and every replay has the eager call's."""
+    m, batch, _ = make(B=6)
+    m.eval()
+    seq, tt, feat = batch[0], batch[3], batch[6]
+    T = seq.shape[1]
+    cut, turns = T - 5, 150
+    head = slice(0, cut)
+    first = lambda: m.stream_begin(seq[:, head], to_rows(feat, head), tt[:, head])[1]  # noqa: E731
+    one, all_, kept = first(), first(), first()
+    g = torch.Generator(device=DEV).manual_seed(7)
+    at = torch.randint(cut, T, (turns, 6), generator=g, device=DEV)
+    user = torch.stack([torch.randperm(6, generator=g, device=DEV) for _ in range(turns)])
+    rows = lambda u, t: {k: v[u, t][:, None] for k, v in feat.items()}  # noqa: E731
+    want = torch.cat([m.stream_step(one, seq[u, t], rows(u, t), tt[u, t], u) for u, t in zip(user, at)])
+    user, at = user.reshape(-1), at.reshape(-1)
+    args = seq[user, at], rows(user, at), tt[user, at], user
+    got = m.stream_step(all_, *args)
+    # 150 events more pass through the states than in one call of 6: sums of 150 more terms
+    tol = 2 * TOL
+    assert nrel(got, want) < tol and all_.position.tolist() == one.position.tolist() == [cut + turns] * 6
+    for x, y in zip(all_.states, one.states):
+        assert nrel(x, y) < tol
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        m.stream_step(kept, *args)
+    torch.cuda.current_stream().wait_stream(side)
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr):
+        out = m.stream_step(kept, *args)
+    for _ in range(3):
+        gr.replay()
+        torch.cuda.synchronize()
+        again = m.stream_step(all_, *args)
+        torch.cuda.synchronize()
+        assert torch.equal(out, again) and torch.equal(kept.position, all_.position)
+        for x, y in zip(kept.states, all_.states):
+            assert torch.equal(x, y)
