@@ -659,7 +659,7 @@ int grk_decay_attn_bwd(const grk_decay_args* a, const void* dout, int64_t lddo, 
  * NULL: event i takes state i.  Events of one slot are that user's next events, taken in
  * the order of their index.  A negative slot holds no event (output row zero); one at or
  * past num_slots as well, and sets *err_flag (optional).  Workspace:
- * grk_decay_attn_step_workspace(n, slots != NULL) bytes. */
+ * grk_decay_attn_step_workspace(n, slots != NULL) bytes, aligned to 8. */
 size_t grk_decay_attn_step_workspace(int64_t n, int has_slots);
 int grk_decay_attn_step(const void* q, int64_t ldq, const void* k, int64_t ldk, const void* v, int64_t ldv, int dtype,
                         const float* log_decay, int64_t n, int heads, int head_dim, float scale, float* state,

@@ -1,0 +1,135 @@
+"""Single events of many users in one call (kernels.decay_attn_step): slots that are all
+different, that repeat, that hold nothing; pools whose slots pass 32 bits; time that grows
+with the events, not with their pairs.
+
+Tolerance: a state is a sum of its m events' products and the state before, outputs of
+head_dim more terms, all in fp32: (m + head_dim + 4) 2^-24, of rows of about unit terms;
+300 * 2^-24 covers the 40 events of a slot here."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+DEV = 'cuda'
+
+
+@pytest.fixture(scope='module')
+def K():
+    from tencent_recommendation_2025_amd import kernels
+    return kernels
+
+
+def draw(n, pool, H, hd, dt, how, seed):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    q, k, v = (torch.randn(n, H * hd, generator=g, device=DEV).to(dt) for _ in range(3))
+    state = torch.randn(pool, H, hd, hd, generator=g, device=DEV)
+    lg = torch.log1p(-torch.exp2(-torch.linspace(3.0, 8.0, H, device=DEV)))
+    if how == 'distinct':
+        slots = torch.randperm(pool, generator=g, device=DEV)[:n]
+    else:   # about n / 16 users, 5 % rows without an event, 5 % outside the pool
+        slots = torch.randint(0, max(1, n // 16), (n,), generator=g, device=DEV)
+        r = torch.rand(n, generator=g, device=DEV)
+        slots = torch.where(r < 0.05, -1 - slots, torch.where(r > 0.95, pool + slots, slots))
+    return q, k, v, state, lg, slots
+
+
+def plain(q, k, v, state, lg, slots):
+    """Event after event of every slot, in 64 bits: the t-th events of all slots at once."""
+    n, H, hd = q.shape[0], state.shape[1], state.shape[2]
+    q, k, v = (x.double().view(n, H, hd) for x in (q, k, v))
+    s, o = state.double(), torch.zeros(n, H, hd, dtype=torch.float64, device=DEV)
+    g = torch.exp(lg.double())[:, None, None]
+    seen, rank = {}, []
+    for x in slots.tolist():
+        rank.append(seen.get(x, 0))
+        seen[x] = rank[-1] + 1
+    rank = torch.tensor(rank, device=DEV)
+    live = (slots >= 0) & (slots < state.shape[0])
+    for t in range(int(rank[live].max()) + 1):
+        i = torch.nonzero(live & (rank == t))[:, 0]
+        s[slots[i]] = s[slots[i]] * g + k[i][..., :, None] * v[i][..., None, :]
+        o[i] = (q[i][..., :, None] * s[slots[i]]).sum(-2)
+    return o.view(n, -1), s
+
+
+def close(got, want, tol):
+    err = (got.double() - want).norm(dim=1) / want.norm(dim=1).clamp(min=1e-3)
+    assert float(err.max()) < tol, float(err.max())
+
+
+@pytest.mark.parametrize('n,H,hd,dt', [(8192, 2, 16, torch.float32), (8193, 2, 16, torch.float32),
+                                       (9000, 3, 33, torch.bfloat16), (50001, 1, 16, torch.float32),
+                                       (117187, 1, 16, torch.float16)])
+@pytest.mark.parametrize('how', ['distinct', 'repeated'])
+def test_many_events(K, n, H, hd, dt, how):
+    pool = n + 37
+    q, k, v, state, lg, slots = draw(n, pool, H, hd, dt, how, n)
+    want, want_state = plain(q, k, v, state, lg, slots)
+    flag = torch.zeros(1, dtype=torch.int32, device=DEV)
+    mine, again = state.clone(), state.clone()
+    o = K.decay_attn_step(q, k, v, lg, mine, slots, scale=1.0, err_flag=flag)
+    close(o, want, {torch.float32: 0.0, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}[dt] + 300 * 2.0 ** -24)
+    close(mine.view(pool, -1), want_state.view(pool, -1), 300 * 2.0 ** -24)
+    assert int(flag) == (how == 'repeated')
+    # the same events in calls of fewer: the same bits
+    parts = [K.decay_attn_step(*(x[i:i + 1000] for x in (q, k, v)), lg, again, slots[i:i + 1000].int(), scale=1.0)
+             for i in range(0, n, 1000)]
+    assert torch.equal(torch.cat(parts), o) and torch.equal(again, mine)
+
+
+def test_slots_past_32_bits(K):
+    """A pool of more than 2^32 states: slots that agree in their low 32 bits are apart."""
+    far = 2 ** 32
+    state = torch.empty(far + 8, 1, 1, 1, device=DEV)
+    n = 9000
+    g = torch.Generator(device=DEV).manual_seed(1)
+    q, k, v = (torch.randn(n, 1, generator=g, device=DEV) for _ in range(3))
+    used = torch.tensor([0, 1, 5, far - 1, far, far + 1, far + 5, far + 7], device=DEV)
+    which = torch.randint(0, 9, (n,), generator=g, device=DEV)
+    slots = torch.cat([used, torch.tensor([far + 8], device=DEV)])[which]
+    small = torch.randn(8, 1, 1, 1, generator=g, device=DEV)
+    state[used] = small
+    lg = torch.tensor([-0.05], device=DEV)
+    flag = torch.zeros(1, dtype=torch.int32, device=DEV)
+    o = K.decay_attn_step(q, k, v, lg, state, slots, scale=1.0, err_flag=flag)
+    want = K.decay_attn_step(q, k, v, lg, small, which, scale=1.0)   # the same users in a pool of 8
+    assert torch.equal(o, want) and torch.equal(state[used], small) and int(flag) == 1
+
+
+def test_many_events_in_a_graph(K):
+    n, pool = 9100, 700
+    q, k, v, state, lg, slots = draw(n, pool, 2, 16, torch.bfloat16, 'repeated', 9)
+    a, b = state.clone(), state.clone()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        K.decay_attn_step(q, k, v, lg, state, slots)
+    torch.cuda.current_stream().wait_stream(side)
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr):
+        out = K.decay_attn_step(q, k, v, lg, a, slots)
+    for turn in range(4):
+        slots.copy_(slots.roll(turn + 1))
+        gr.replay()
+        torch.cuda.synchronize()
+        want = K.decay_attn_step(q, k, v, lg, b, slots)
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and torch.equal(a, b), turn
+
+
+def test_time_grows_with_the_events(K):
+    """4 times the events (16-wide states, all different): 4 times the bytes.  Their pairs
+    would be 16 times as many; 8 is between the two."""
+    took = []
+    for n in (30000, 120000):
+        q, k, v, state, lg, slots = draw(n, n, 1, 16, torch.bfloat16, 'distinct', 3)
+        best = 1e9
+        for _ in range(12):
+            start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            start.record()
+            for _ in range(5):
+                K.decay_attn_step(q, k, v, lg, state, slots)
+            end.record()
+            end.synchronize()
+            best = min(best, start.elapsed_time(end))
+        took.append(best)
+    assert took[1] < 8 * took[0], took
