@@ -374,17 +374,47 @@ class DecayStream:
         self.states, self.position = states, position
         self.err = torch.zeros(1, dtype=torch.int32, device=position.device)
 
+    def _slots(self, slots):
+        """int64 slots on the host (a bool mask or a slice of the slots: those it takes); a
+        negative one names no user, one past the stream is refused."""
+        n = self.position.numel()
+        if isinstance(slots, slice):
+            return torch.arange(n)[slots]
+        t = torch.as_tensor(slots).reshape(-1).cpu()
+        if t.dtype == torch.bool:
+            if t.numel() != n:
+                raise ValueError(f'a mask of {t.numel()} for the {n} slots of the stream')
+            return torch.nonzero(t)[:, 0]
+        if t.numel() and (t.is_floating_point() or t.is_complex()):
+            raise ValueError(f'slots of dtype {t.dtype}')
+        t = t.to(torch.int64)
+        if bool((t >= n).any()):
+            raise ValueError(f'slot {int(t.max())} outside the {n} of the stream')
+        return t
+
     def place(self, slots, other):
-        """The users of another stream (stream_begin's, in its order) into these slots."""
-        for mine, theirs in zip(self.states, other.states):
-            mine[slots] = theirs
-        self.position[slots] = other.position
+        """The users of another stream (stream_begin's, in its order) into these slots, each
+        into one of its own; one with a negative slot stays out.  (Slots on the device are
+        read back first: a host sync.)"""
+        to = self._slots(slots)
+        if to.numel() != other.position.numel():
+            raise ValueError(f'{to.numel()} slots for the {other.position.numel()} users of the other stream')
+        if [s.shape[1:] for s in self.states] != [s.shape[1:] for s in other.states]:
+            raise ValueError('the streams are of different models')
+        users = torch.nonzero(to >= 0)[:, 0]
+        to = to[users]
+        if torch.unique(to).numel() != to.numel():
+            raise ValueError('a slot takes one user')
+        to, users = to.to(self.position.device), users.to(self.position.device)
+        for mine, theirs in zip((*self.states, self.position), (*other.states, other.position)):
+            mine[to] = theirs[users]
 
     def clear(self, slots):
-        """These slots as users without a history."""
-        for s in self.states:
-            s[slots] = 0
-        self.position[slots] = 0
+        """These slots as users without a history (a negative one names none)."""
+        at = self._slots(slots)
+        at = at[at >= 0].to(self.position.device)
+        for s in (*self.states, self.position):
+            s[at] = 0
 
     def check(self):
         if int(self.err.item()):
