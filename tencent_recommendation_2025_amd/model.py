@@ -1102,9 +1102,9 @@ class BaselineModel(torch.nn.Module):
             slots = torch.where(event, torch.arange(n, device=dev), -1)
             pos, passed = stream.position.clone(), event.to(torch.int64)
         else:
+            if slots.shape != (n,) or slots.dtype == torch.bool or slots.is_floating_point():
+                raise ValueError(f'{n} events, slots of shape {tuple(slots.shape)} and {slots.dtype}')
             slots = slots.to(dev, torch.int64).contiguous()
-            if slots.shape != (n,):
-                raise ValueError(f'{n} events, slots of shape {tuple(slots.shape)}')
             inside = (slots >= 0) & (slots < stream.position.numel())
             slots = torch.where(inside & ~event, -1, slots)   # (one outside the stream is still named by check)
             inside = inside & event

@@ -206,3 +206,19 @@ def test_many_events_in_one_step():
         assert torch.equal(out, again) and torch.equal(kept.position, all_.position)
         for x, y in zip(kept.states, all_.states):
             assert torch.equal(x, y)
+
+
+def test_slots_that_are_no_numbers_of_slots_are_refused():
+    """A mask would be read as slots 0 and 1."""
+    m, batch, _ = make(B=2)
+    m.eval()
+    seq, tt, feat = batch[0], batch[3], batch[6]
+    _, s = m.stream_begin(seq, feat, tt)
+    was = s.position.tolist()
+    for slots in (torch.tensor([True, False], device=DEV), torch.tensor([0.0, 1.0], device=DEV)):
+        with pytest.raises(ValueError):
+            m.stream_step(s, seq[:, 0], to_rows(feat, slice(0, 1)), tt[:, 0], slots)
+    assert s.position.tolist() == was
+    m.stream_step(s, seq[:, -1], to_rows(feat, slice(seq.shape[1] - 1, None)), tt[:, -1],
+                  torch.tensor([1, 0], dtype=torch.int16))
+    assert s.position.tolist() == [w + 1 for w in was]
