@@ -627,8 +627,8 @@ int grk_rotary(const void* x, int64_t ldx, void* y, int64_t ldy, int dtype, cons
  * positions before seq_range[b][0], without reading key_valid there; it has to be this
  * key_valid's (a range it calls contiguous is taken to have no holes behind its start,
  * and its order of the sequences to name each of them once).
- * A NaN or an infinity in an event reaches the outputs behind it, and may reach those
- * of up to 63 events before it.
+ * A NaN or an infinity in an event reaches the outputs that depend on it (an infinity as
+ * either), and no others.
  * row_base / num_rows / capacity: the packed rows of grk_attn_args (seq_range
  * required; rows [*num_rows, capacity) of every output are zeroed); else the rows are
  * [batch * seq_len].

@@ -93,6 +93,8 @@ __device__ __forceinline__ bool decay_state_used(const DecayParams& p, const Dec
 // g^n for n >= 0 (g^0 = 1 also for g = 0).
 __device__ __forceinline__ float decay_pow(float lg, int n) { return n == 0 ? 1.f : expf(lg * (float)n); }
 
+__device__ __forceinline__ bool decay_finite(float x) { return (__float_as_uint(x) & 0x7f800000u) != 0x7f800000u; }
+
 // Row of step t, masked or not, or -1 past the segment (or where no row exists).
 __device__ __forceinline__ int64_t decay_row(const DecayParams& p, const DecayPlace& w, int rev, int t) {
   if (t >= w.t1) return -1;

@@ -98,6 +98,30 @@ __device__ __forceinline__ void mfma16(f32x4 a, f32x4 b, f32x4& c) {
   mfma_keep(c, a, b);
 }
 
+// P V of a chunk with infinities or NaNs in V (grk_decay_bf16.hip): they leave the operand,
+// and are added to the outputs of the rows i >= j, one by one.
+template <int PT>
+__device__ __forceinline__ void decay_odd_steps(f32x4 (&v)[2], f32x4 (&o)[2], const float* sp, int lane) {
+  asm volatile("" : "+v"(lane));   // (its addresses are not kept through the chunks)
+  const int g = lane >> 4, c = lane & 15;
+#pragma unroll
+  for (int at = 0; at < 8; ++at) {
+    const float f = v[at / 4][at % 4];
+    if (!decay_finite(f)) v[at / 4][at % 4] = 0.f;
+    for (uint64_t m = __ballot(!decay_finite(f)); m; m &= m - 1) {
+      const int l = __builtin_ctzll(m), j = 16 * (at / 4) + 4 * (l >> 4) + at % 4, col = l & 15;
+      const float x = __shfl(f, l);
+#pragma unroll
+      for (int it = 0; it < 2; ++it) {
+        const float y = sp[(16 * it + c) * PT + j] * x;
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (4 * g + k == col && 16 * it + c >= j) o[it][k] += y;
+      }
+    }
+  }
+}
+
 template <typename T, int V, int DP, bool STATE>
 __global__ void __launch_bounds__(DP * 4, 4) k_decay_f32(DecayParams p) {
   constexpr int C = kF32Chunk, ST = DP + kF32Pad, PT = C + kF32Pad, NT = DP / 16, NTH = DP * 4;
@@ -185,8 +209,11 @@ __global__ void __launch_bounds__(DP * 4, 4) k_decay_f32(DecayParams p) {
           mfma16(*reinterpret_cast<const f32x4*>(sb + (16 * jt + c) * ST + 16 * dt + 4 * g),
                  *reinterpret_cast<const f32x4*>(sa + (16 * it + c) * ST + 16 * dt + 4 * g), x);
         const float* lag = pw + 16 * (it - jt) + c - 4 * g;
-        *reinterpret_cast<f32x4*>(sp + (16 * it + c) * PT + 16 * jt + 4 * g) =
-            f32x4{x[0] * lag[0], x[1] * lag[-1], x[2] * lag[-2], x[3] * lag[-3]};
+        x *= f32x4{lag[0], lag[-1], lag[-2], lag[-3]};
+        const int ahead = 16 * (it - jt) + c - 4 * g;   // steps from j = 4 g to i
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = ahead < i ? 0.f : x[i];   // (no product by 0: K_j may hold a NaN)
+        *reinterpret_cast<f32x4*>(sp + (16 * it + c) * PT + 16 * jt + 4 * g) = x;
       }
     }
     f32x4 v[2];   // V[16 jt + 4 g + s][col]
@@ -230,8 +257,11 @@ __global__ void __launch_bounds__(DP * 4, 4) k_decay_f32(DecayParams p) {
         }
       }
     }
+    const f32x4 sum = v[0] + v[1];   // not finite where an element is not (or the sum overflows)
+    const bool odd = !STATE && __any(!decay_finite((sum[0] + sum[1]) + (sum[2] + sum[3])));
     __syncthreads();
     if constexpr (!STATE) {
+      if (__builtin_expect(odd, 0)) decay_odd_steps<PT>(v, o, sp, lane);
 #pragma unroll
       for (int it = 0; it < 2; ++it) {
 #pragma unroll

@@ -139,13 +139,62 @@ struct DecayRows {
   }
 };
 
+// c + 0 * each element.
+__device__ __forceinline__ float times_zero(bf16x8 v, float c) {
+  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+  const bf16x2 zero = {(__bf16)0.f, (__bf16)0.f};
+#pragma unroll
+  for (int i = 0; i < 8; i += 2) c = __builtin_amdgcn_fdot2_f32_bf16(bf16x2{v[i], v[i + 1]}, zero, c, false);
+  return c;
+}
+
+// P V of a chunk with infinities or NaNs in V: a matrix product takes every step's V_j to
+// every row, as 0 * V_j to the rows before j.  So they leave the fragments here, and are
+// added to the outputs of the rows i >= j, one by one.  (Looking for them and selecting P
+// instead of multiplying it by 0 costs 2 to 3 % of the kernel where there are none.)
+template <int NE, int CK>
+__device__ __forceinline__ void decay_odd_steps(bf16x8 (&vf)[NE][CK], f32x4 (&o)[2 * CK][NE], const char* sp, int lane) {
+  constexpr int PS = decay_stride<32 * CK>();
+  asm volatile("" : "+v"(lane));   // (else its addresses are kept in registers through every chunk)
+  const int g = lane >> 4, c = lane & 15;
+#pragma unroll
+  for (int x = 0; x < NE; ++x)
+    for (;;) {
+      int at = -1;   // one of the lanes' 8 CK slots that has any
+      float f = 0.f;
+#pragma unroll
+      for (int k = 0; k < 8 * CK; ++k) {
+        const float y = (float)vf[x][k / 8][k % 8];
+        if (__any(!decay_finite(y))) { at = k; f = y; }
+      }
+      if (at < 0) break;
+#pragma unroll
+      for (int k = 0; k < 8 * CK; ++k)
+        if (k == at && !decay_finite(f)) vf[x][k / 8][k % 8] = (__bf16)0.f;
+      for (uint64_t m = __ballot(!decay_finite(f)); m; m &= m - 1) {
+        const int l = __builtin_ctzll(m), q = at & 7, col = l & 15;
+        const int slot = (at & ~7) * 4 + 8 * (l >> 4) + q, j = slot - q + (q < 4 ? 2 * q : 2 * q - 7);
+        const float v = __shfl(f, l);
+#pragma unroll
+        for (int it = 0; it < 2 * CK; ++it) {
+          const float y = (float)*reinterpret_cast<const __bf16*>(sp + (16 * it + c) * PS + 2 * slot) * v;
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            if (4 * g + k == col && 16 * it + c >= j) o[it][x][k] += y;
+        }
+      }
+    }
+}
+
 // NS: bf16 parts of g^(n-1-j) v_j in the state's sum: 2 (16 bits; the state is rounded to
 // bf16 only as an operand of the output) or, where the state is returned in fp32, 3 (all 24
 // bits).  One part would cost 2 % (heads of 64) to 10 % (128) less time and put a third
 // rounding of 2^-9 into every output, which then lay 1.6 times as far from the exact one as
 // its own rounding; with two it is 1.4 times.
+// Waves a SIMD: 5 with heads of up to 64 (96 registers; gradients of 128 sequences of up to 201
+// events, 8 heads of 64: 36 us, with 4 waves 37.5).
 template <int DP, int EW, int NE, int C, int NS, bool STATE>
-__global__ void __launch_bounds__(EW * 4 / NE, NE == 1 ? 4 : 2) k_decay_bf16(DecayParams p) {
+__global__ void __launch_bounds__(EW * 4 / NE, NE == 2 ? 2 : DP <= 64 ? 5 : 4) k_decay_bf16(DecayParams p) {
   constexpr int CK = C / 32, NT = DP / 16, KS = DP / 32, NW = EW / 16 / NE, NTH = NW * 64;
   constexpr int ST = decay_stride<DP>(), SE = decay_stride<EW>(), PS = decay_stride<C>();
   using Rows = DecayRows<DP, NTH, C>;    // of a and b
@@ -261,8 +310,11 @@ __global__ void __launch_bounds__(EW * 4 / NE, NE == 1 ? 4 : 2) k_decay_bf16(Dec
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) mfma32(lds_b128(k + 64 * ks), lds_b128(q + 64 * ks), x);
         const float* lag = pw + 16 * (it - jt) + c - 4 * g;
-        const bf16x4 y = {(__bf16)(x[0] * lag[0]), (__bf16)(x[2] * lag[-2]), (__bf16)(x[1] * lag[-1]),
-                          (__bf16)(x[3] * lag[-3])};
+        x *= f32x4{lag[0], lag[-1], lag[-2], lag[-3]};
+        const int ahead = 16 * (it - jt) + c - 4 * g;   // steps from j = 4 g to i
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = ahead < i ? 0.f : x[i];   // (no product by 0: K_j may hold a NaN)
+        const bf16x4 y = {(__bf16)x[0], (__bf16)x[2], (__bf16)x[1], (__bf16)x[3]};
         const uint2 z = __builtin_bit_cast(uint2, y);   // steps 0 2 | 1 3 of four
         char* dst = sp + (16 * it + c) * PS + (2 * jt + (g >> 1)) * 16 + 4 * (g & 1);
         *reinterpret_cast<unsigned*>(dst) = z.x;
@@ -355,8 +407,18 @@ __global__ void __launch_bounds__(EW * 4 / NE, NE == 1 ? 4 : 2) k_decay_bf16(Dec
         }
       }
     }
+    bool odd = false;   // an infinity or a NaN in the wave's V: 0 times it is a NaN
+    if constexpr (!STATE) {
+      float z = 0.f;
+#pragma unroll
+      for (int x = 0; x < NE; ++x)
+#pragma unroll
+        for (int ks = 0; ks < CK; ++ks) z = times_zero(vf[x][ks], z);
+      odd = __any(z != 0.f);
+    }
     __syncthreads();
     if constexpr (!STATE) {
+      if (__builtin_expect(odd, 0)) decay_odd_steps<NE, CK>(vf, o, sp, lane);
       char* out = reinterpret_cast<char*>(r.out) + (low * r.ldo + hcol) * 2;
 #pragma unroll
       for (int it = 0; it < C / 16; ++it) {

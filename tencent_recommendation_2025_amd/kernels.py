@@ -1427,8 +1427,8 @@ def decay_attn_fwd(q, k, v, log_decay, batch, seq_len, scale=None, key_valid=Non
     hold no event.  scale: head_dim^-0.5 by default.
     state: the states before the first position, fp32 [B, heads, head_dim, head_dim];
     return_state: also those behind the last one (into state_out, which may be state).
-    A NaN or an infinity in an event's own row reaches all rows of its chunk of steps (as 0 *
-    inf in the masked half of a product); what lies in masked rows reaches none."""
+    A NaN or an infinity in an event's own row reaches the outputs that depend on it (an
+    infinity as either), no earlier ones; what lies in masked rows reaches none."""
     a = _decay_args(q, k, v, log_decay, batch, seq_len, scale, key_valid, seq_range, row_base)
     dev = _same_device(q, state, state_out, out)
     shape = (a.batch, a.heads, a.head_dim, a.head_dim)
