@@ -604,9 +604,17 @@ int grk_add_norm_bwd(const void* gx, int64_t ldgx, int gx_dtype, const void* gs,
  * decay for each head, and the norm of each head with a SiLU gate.  Rows hold
  * heads side by side: head h at columns [h * head_dim, (h + 1) * head_dim).
  * dtype (GRK_F32, GRK_BF16, GRK_F16) is the type of every row operand of a call;
- * arithmetic and sums are fp32, outputs rounded once.  Any row stride of at
- * least heads * head_dim elements; rows, strides and head_dim made of 16-byte
- * vectors take the vector kernels.
+ * sums, states and statistics are fp32, outputs rounded once.  Arithmetic is fp32
+ * but for
+ *   - grk_decay_attn_fwd / _bwd of bf16 rows made of 16-byte vectors, on the bf16 matrix
+ *     instruction: each of the scores and the state, as operands of the output, are
+ *     rounded to bf16 (2^-9 of a term), the terms of the state's sum to 16 bits
+ *     (24 where a state is returned).  Measured, normwise against 64 bits: 0.0023 to 0.0024,
+ *     with fp32 products rounded once 0.0017;
+ *   - rotary's sine and cosine: fp32 functions of an angle reduced in 64 bits;
+ *   - the norm's sigmoid of 16-bit rows: the hardware exponential (2^-21).
+ * Any row stride of at least heads * head_dim elements; rows, strides and head_dim made
+ * of 16-byte vectors take the vector kernels.
  * ------------------------------------------------------------------------ */
 /* Each head's first rotary_dim columns (even, <= head_dim) as rotary_dim / 2
  * pairs -- (i, i + rotary_dim / 2), or (2 i, 2 i + 1) with interleaved -- turned by
@@ -621,10 +629,10 @@ int grk_rotary(const void* x, int64_t ldx, void* y, int64_t ldy, int dtype, cons
 
 /* S_t = g S_{t-1} + k_t v_t^T, o_t = scale * q_t S_t with g = exp(min(log_decay[h], 0))
  * for every (sequence, head); head_dim in [1, 128] (GRK_EUNSUPPORTED above).
- * Positions with key_valid 0 hold no event: their q / k / v are not read (whatever
- * they hold), their output and gradient rows are zero, and the state decays over
- * them.  seq_range (int32 [batch, 3], grk_seq_ranges; optional): the same for the
- * positions before seq_range[b][0], without reading key_valid there; it has to be this
+ * Positions with key_valid 0 hold no event: what their rows of q / k / v hold is not used
+ * (the rows have to be readable), their output and gradient rows are zero, and the state
+ * decays over them.  seq_range (int32 [batch, 3], grk_seq_ranges; optional): the same for
+ * the positions before seq_range[b][0], whose rows and key_valid are not read; it has to be this
  * key_valid's (a range it calls contiguous is taken to have no holes behind its start,
  * and its order of the sequences to name each of them once).
  * A NaN or an infinity in an event reaches the outputs that depend on it (an infinity as

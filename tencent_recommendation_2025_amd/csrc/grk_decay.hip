@@ -26,8 +26,8 @@ int sort_pairs(unsigned* k0, unsigned long long* v0, unsigned* k1, unsigned long
 // 16 K operations of the state and 6 K of its chunk -- 32 steps, not 64, keep the latter
 // small and leave LDS for 5 workgroups a CU.  (33 x 101 events of 2 heads of 32 in fp32: 12 us
 // forward, 12 us the gradients -- 66 and 198 workgroups of 4 chunks each, latency.  Rows
-// enough for the card keep the instruction half busy: 16 K rows of 8 heads of 64, both
-// directions, 155 us with autograd.)
+// enough for the card keep the instruction half busy: 80 x 204 events of 8 heads of 64, fp32 48
+// us forward and 113 us the gradients, fp16 45 and 108.)
 constexpr int kF32Chunk = 32;
 constexpr int kF32Pad = 4;   // floats after each LDS row: rows 4 apart fall 16 banks apart
 
@@ -362,9 +362,13 @@ __global__ void __launch_bounds__(256) k_decay_scan(DecayParams p) {
 // One workgroup per (event, head): S <- g S + k v^T in place, o = scale q S.  The state
 // is read and written once, in rows of `lanes` threads of V columns; a thread keeps its
 // columns, so o is a sum over the thread rows in LDS.  Bound: memory, 8 head_dim^2 bytes
-// of state per (event, head).
+// of state per (event, head), with heads of 64 and more; narrow ones leave threads without a
+// row (heads of 16: 192 of 256) and are bound by the workgroups' number.  States of 240 MB, read
+// and written, part of them in the cache: heads of 128 49 us, 64 41, 32 62, 16 276.
 constexpr int kStepThreads = 256;
-constexpr int kStepInline = 256;   // events up to which every workgroup looks for its slot's others itself
+// Events up to which every workgroup looks for its slot's others itself (a call of 8 heads of 64:
+// 256 events 14.5 us, with links 17.5; 1024 events 54 and 55.5).
+constexpr int kStepInline = 256;
 // Events up to which every pair is compared (one launch); more are sorted by slot (8 launches).
 // A call of 8192 events of one 16-wide head: 49 us with the pairs, 53 sorted; 12000: 79 and 63;
 // 4096: 25 and 43.

@@ -136,7 +136,10 @@ extern "C" int grk_rotary(const void* x, int64_t ldx, void* y, int64_t ldy, int 
   // An output of a quarter of the 256 MB cache or more passes it by and leaves it to what was
   // there, the input among it (32771 rows of 8 heads of 80, fp32, 84 MB: 39.7 -> 27.4 us);
   // smaller ones stay for their reader (25728 rows of 16 heads of 64, bf16, 53 MB: 23.4 us,
-  // past the cache 25.2).
+  // past the cache 25.2).  Heads of 64, three inputs and outputs in turn, stored to the cache
+  // and past it: bf16 32 MB 12.5 and 13.6 us, 64 MB 29.2 and 25.4, 128 MB 52.9 and 51.2; fp32 12.1
+  // and 12.3, 26.6 and 22.0, 50.3 and 48.7.  48 MB gain too (22.2 and 19.3), unless the same
+  // buffers come again (17.2 and 19.3).
   const bool past = rows * cols * (int64_t)dtype_size(dtype) >= (64 << 20);
   // rows of a workgroup: enough that it streams 32 KB, few enough that the grid holds
   // 1024 workgroups (4 on each CU) and their angles fit the LDS table

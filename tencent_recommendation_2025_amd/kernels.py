@@ -1475,6 +1475,7 @@ def decay_attn_bwd(dout, q, k, v, log_decay, batch, seq_len, scale=None, key_val
 def decay_attn_step(q, k, v, log_decay, state, slots=None, scale=None, err_flag=None, out=None):
     """One event of each of n users (grk_decay_attn_step): state[slot] <- g state[slot] +
     k v^T in place, and scale q state[slot] as a new [n, heads * head_dim] (or into out).
+    No other operand may lie in the states.
 
     state fp32 [slots, heads, head_dim, head_dim]; slots int32 / int64 [n] (None: event i
     takes state i).  Events of one slot are taken in the order of their index.  A negative
