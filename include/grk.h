@@ -42,6 +42,7 @@ enum { GRK_F32 = 0, GRK_BF16 = 1, GRK_F16 = 2 };    /* floating dtypes */
 enum { GRK_F32_BF16 = 3 };  /* pair logits: fp32 h, bf16 e_pos / e_neg (and their gradients) */
 enum { GRK_FP8_E4M3 = 4 };  /* attention q/k/v: OCP fp8 e4m3 (gfx950's fp8 format) */
 enum { GRK_I32 = 0, GRK_I64 = 1 };                  /* index dtypes */
+enum { GRK_SLOTS_DIFFER = 256 };                     /* grk_decay_attn_step: added to itype */
 
 /* How a lookup derives its row id from the index tensor value v at token
  * (n = b*T + t):  model/BaseLine/model.py:240-247 and :326-328. */
@@ -667,7 +668,9 @@ int grk_decay_attn_bwd(const grk_decay_args* a, const void* dout, int64_t lddo, 
  * NULL: event i takes state i.  Events of one slot are that user's next events, taken in
  * the order of their index.  A negative slot holds no event (output row zero); one at or
  * past num_slots as well, and sets *err_flag (optional).  Workspace:
- * grk_decay_attn_step_workspace(n, slots != NULL) bytes, aligned to 8. */
+ * grk_decay_attn_step_workspace(n, slots != NULL) bytes, aligned to 8.  itype +
+ * GRK_SLOTS_DIFFER: no two events have one slot of the pool, so that nothing looks for them
+ * (where two have, their state is left undefined); no workspace. */
 size_t grk_decay_attn_step_workspace(int64_t n, int has_slots);
 int grk_decay_attn_step(const void* q, int64_t ldq, const void* k, int64_t ldk, const void* v, int64_t ldv, int dtype,
                         const float* log_decay, int64_t n, int heads, int head_dim, float scale, float* state,

@@ -26,6 +26,7 @@ GRK_F32, GRK_BF16, GRK_F16 = 0, 1, 2
 GRK_F32_BF16 = 3  # pair logits: fp32 h, bf16 item embeddings
 GRK_FP8_E4M3 = 4  # attention q/k/v: OCP fp8 e4m3
 GRK_I32, GRK_I64 = 0, 1
+GRK_SLOTS_DIFFER = 256
 FEAT_SKIP_ROW0 = 1   # GRK_FEAT_SKIP_ROW0
 GRK_GEMM_EP_NONE, GRK_GEMM_EP_RELU = 0, 1
 BWD_ORDERED, BWD_CHUNKED, BWD_DENSE_BF16 = 0, 1, 2  # grk_embedding_backward flags (bf16 dense: | with CHUNKED)

@@ -381,6 +381,7 @@ struct StepParams {
   const float* log_decay;
   float* state; int64_t num_slots;
   const void* slots; int slots64;
+  int differ;                    // no two events have one slot
   int64_t n;
   int heads, hd;
   float scale;
@@ -494,7 +495,7 @@ __global__ void __launch_bounds__(kStepThreads) k_decay_step(StepParams p) {
   for (int64_t i = i0; i >= 0;) {
     // the slot's other events
     int64_t next = -1;
-    if (p.slots) {
+    if (p.slots && !p.differ) {
       if (p.links) {
         if (i == i0 && p.links[2 * i]) return;
         next = p.links[2 * i + 1];
@@ -767,6 +768,8 @@ extern "C" int grk_decay_attn_step(const void* q, int64_t ldq, const void* k, in
                                    float* state, int64_t num_slots, const void* slots, int itype, int32_t* err_flag,
                                    void* out, int64_t ldo, void* ws, size_t ws_bytes, void* stream) {
   clear_error();
+  const bool differ = itype & GRK_SLOTS_DIFFER;
+  itype &= ~GRK_SLOTS_DIFFER;
   GRK_CHECK_ARG(known_dtype(dtype), "dtype must be fp32, bf16 or fp16");
   GRK_CHECK_ARG(itype == GRK_I32 || itype == GRK_I64, "slots must be int32 or int64");
   GRK_CHECK_ARG(n >= 0 && heads > 0 && num_slots >= 0 && n < (1 << 24) &&
@@ -781,13 +784,13 @@ extern "C" int grk_decay_attn_step(const void* q, int64_t ldq, const void* k, in
   GRK_CHECK_ARG(n == 1 || (ldq >= cols && ldk >= cols && ldv >= cols && ldo >= cols),
                 "row strides must be at least heads * head_dim");
   GRK_CHECK_ARG(slots || num_slots >= n, "without slots event i takes state i: num_slots must be at least n");
-  const size_t need = grk_decay_attn_step_workspace(n, slots != nullptr);
+  const size_t need = grk_decay_attn_step_workspace(n, slots && !differ);
   GRK_CHECK_ARG(need == 0 || (ws && ws_bytes >= need), "workspace too small");
   GRK_CHECK_ARG(need == 0 || (uintptr_t)ws % 8 == 0, "workspace must be aligned to 8 bytes");
   StepParams p;
   memset(&p, 0, sizeof(p));
   p.q = q; p.ldq = ldq; p.k = k; p.ldk = ldk; p.v = v; p.ldv = ldv; p.log_decay = log_decay; p.state = state;
-  p.num_slots = num_slots; p.slots = slots; p.slots64 = itype == GRK_I64; p.n = n; p.heads = heads; p.hd = head_dim;
+  p.num_slots = num_slots; p.slots = slots; p.slots64 = itype == GRK_I64; p.differ = differ; p.n = n; p.heads = heads; p.hd = head_dim;
   p.scale = scale; p.err = err_flag; p.out = out; p.ldo = ldo; p.links = need ? (int32_t*)ws : nullptr;
   hipStream_t s = (hipStream_t)stream;
   if (need && n > kStepPairs) {

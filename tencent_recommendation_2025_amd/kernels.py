@@ -1472,7 +1472,7 @@ def decay_attn_bwd(dout, q, k, v, log_decay, batch, seq_len, scale=None, key_val
     return tuple(grads)
 
 
-def decay_attn_step(q, k, v, log_decay, state, slots=None, scale=None, err_flag=None, out=None):
+def decay_attn_step(q, k, v, log_decay, state, slots=None, scale=None, err_flag=None, out=None, distinct=False):
     """One event of each of n users (grk_decay_attn_step): state[slot] <- g state[slot] +
     k v^T in place, and scale q state[slot] as a new [n, heads * head_dim] (or into out).
     No other operand may lie in the states.
@@ -1480,7 +1480,8 @@ def decay_attn_step(q, k, v, log_decay, state, slots=None, scale=None, err_flag=
     state fp32 [slots, heads, head_dim, head_dim]; slots int32 / int64 [n] (None: event i
     takes state i).  Events of one slot are taken in the order of their index.  A negative
     slot holds no event (output row zero), one past the states as well, and sets err_flag
-    (int32 [1])."""
+    (int32 [1]).  distinct: the caller's word that no two events have one slot of the pool;
+    nothing looks for them then, and where two have, their state is left undefined."""
     dev = _same_device(q, k, v, log_decay, state, slots, err_flag, out)
     if log_decay.dtype != torch.float32 or log_decay.dim() != 1 or not log_decay.is_contiguous() \
             or not log_decay.shape[0]:
@@ -1514,11 +1515,12 @@ def decay_attn_step(q, k, v, log_decay, state, slots=None, scale=None, err_flag=
             raise L.GrkError('out must not overlap state')
     op, ol = _head_rows(out, 'out', n, cols, dt)
     lib = L.lib()
-    nb = lib.grk_decay_attn_step_workspace(n, slots is not None)
+    nb = lib.grk_decay_attn_step_workspace(n, slots is not None and not distinct)
     ws = torch.empty(nb, dtype=torch.uint8, device=q.device) if nb else None
     _launch(lib.grk_decay_attn_step, 'grk_decay_attn_step', dev, qp, ql, kp, kl, vp, vl, code,
             log_decay.data_ptr(), n, H, hd, hd ** -0.5 if scale is None else scale, state.data_ptr(),
-            state.shape[0], _ptr(slots), L.itype_code(slots.dtype) if slots is not None else L.GRK_I64,
+            state.shape[0], _ptr(slots), (L.itype_code(slots.dtype) if slots is not None else L.GRK_I64)
+            + (L.GRK_SLOTS_DIFFER if distinct else 0),
             _ptr(err_flag), op, ol, _ptr(ws), nb)
     return out
 

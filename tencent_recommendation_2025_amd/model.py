@@ -345,11 +345,11 @@ class DecayAttention(torch.nn.Module):
 
         return self._serve(query.reshape(-1, D), positions, attend).view(B, T, D), state[0]
 
-    def step(self, x, positions, state, slots, err_flag=None):
+    def step(self, x, positions, state, slots, err_flag=None, distinct=False):
         """One event of each row's user [n, D] on the states of their slots, in place."""
         lg = self.log_decay.float()
         return self._serve(x, positions, lambda q, k, v: K.decay_attn_step(q, k, v, lg, state, slots,
-                                                                           err_flag=err_flag))
+                                                                           err_flag=err_flag, distinct=distinct))
 
 
 def _earlier_of_slot(slots, most):
@@ -1096,7 +1096,8 @@ class BaselineModel(torch.nn.Module):
         if token_type.shape[0] != n:
             raise ValueError(f'{n} events, {token_type.shape[0]} token types')
         event = token_type.to(dev).reshape(-1) != 0
-        if slots is None:
+        in_order = slots is None
+        if in_order:
             if n != stream.position.numel():
                 raise ValueError(f'{n} events for the {stream.position.numel()} users of the stream: slots needed')
             slots = torch.where(event, torch.arange(n, device=dev), -1)
@@ -1118,7 +1119,7 @@ class BaselineModel(torch.nn.Module):
             stream.position += passed
 
             def layer(i, x):
-                y = self.attention_layers[i].step(x.reshape(n, -1), pos, stream.states[i], slots, stream.err)
+                y = self.attention_layers[i].step(x.reshape(n, -1), pos, stream.states[i], slots, stream.err, in_order)
                 return y.view(x.shape)
 
             return self._prenorm_blocks(seqs, layer)[:, -1, :]

@@ -147,3 +147,20 @@ def test_states_may_not_lie_on_operands(K):
     K.decay_attn_step(*(r for r in rows[:12].view(3, 4, 32)), lg, pool[3:], slots=torch.arange(4, device=DEV) - 1)
     K.decay_attn_step(rows[:0], rows[:0], rows[:0], lg, pool)
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize('n', [5, 300, 9000])
+def test_slots_that_are_said_to_differ(K, n):
+    """The same bits without the look for repeated slots, rows without an event among them."""
+    q, k, v, state, lg, slots = draw(n, n + 9, 2, 16, torch.bfloat16, 'distinct', n)
+    slots[1::7] = -1
+    slots[2] = n + 20
+    a, b = state.clone(), state.clone()
+    flags = torch.zeros(2, 1, dtype=torch.int32, device=DEV)
+    want = K.decay_attn_step(q, k, v, lg, a, slots, err_flag=flags[0])
+    for s in (slots, slots.int()):
+        b.copy_(state)
+        o = K.decay_attn_step(q, k, v, lg, b, s, err_flag=flags[1], distinct=True)
+        assert torch.equal(o, want) and torch.equal(a, b) and flags.tolist() == [[1], [1]]
+    own = K.decay_attn_step(q, k, v, lg, a.copy_(state), distinct=True)
+    assert torch.equal(own, K.decay_attn_step(q, k, v, lg, b.copy_(state))) and torch.equal(a, b)
