@@ -790,8 +790,8 @@ extern "C" int grk_decay_attn_step(const void* q, int64_t ldq, const void* k, in
   StepParams p;
   memset(&p, 0, sizeof(p));
   p.q = q; p.ldq = ldq; p.k = k; p.ldk = ldk; p.v = v; p.ldv = ldv; p.log_decay = log_decay; p.state = state;
-  p.num_slots = num_slots; p.slots = slots; p.slots64 = itype == GRK_I64; p.differ = differ; p.n = n; p.heads = heads; p.hd = head_dim;
-  p.scale = scale; p.err = err_flag; p.out = out; p.ldo = ldo; p.links = need ? (int32_t*)ws : nullptr;
+  p.num_slots = num_slots; p.slots = slots; p.slots64 = itype == GRK_I64; p.differ = differ; p.n = n;
+  p.heads = heads; p.hd = head_dim; p.scale = scale; p.err = err_flag; p.out = out; p.ldo = ldo; p.links = need ? (int32_t*)ws : nullptr;
   hipStream_t s = (hipStream_t)stream;
   if (need && n > kStepPairs) {
     const int rc = step_sort_links(p, s);

@@ -14,7 +14,7 @@
 // Bound: heads of 64, memory's latency -- a wave takes some 20 MFMA, 190 VALU operations and
 // 26 LDS accesses for 32 steps, half of the time that their 16 KB take from HBM on one CU
 // of 256; what is left is the wait of a chunk's two barriers, which the next chunk's loads
-// (to registers, while this one is computed) and 4 waves a SIMD cover in part.  128
+// (to registers, while this one is computed) and 4 to 5 waves a SIMD cover in part.  128
 // sequences of up to 201 events (16 K packed rows) of 8 heads of 64: forward 17.6 us (66
 // MB, 3.8 TB/s), gradients 35.9 us (116 MB, 3.2 TB/s).  Heads of 128: LDS, read for every
 // operand of 4 products a chunk.  8 x 4096 events of 4 heads: 39 us and gradients 89 us

@@ -1502,10 +1502,11 @@ def decay_attn_step(q, k, v, log_decay, state, slots=None, scale=None, err_flag=
     dt = q.dtype
     code = _row_code(dt)
     (qp, ql), (kp, kl), (vp, vl) = [_head_rows(t, m, n, cols, dt) for t, m in ((q, 'q'), (k, 'k'), (v, 'v'))]
-    first = state.data_ptr()
+    first, lg, es = state.data_ptr(), log_decay.data_ptr(), dt.itemsize
     behind = first + 4 * state.numel()
-    for p, ld in ((qp, ql), (kp, kl), (vp, vl), (log_decay.data_ptr(), 0)):
-        if p < behind and first < p + ((n - 1) * ld + cols) * dt.itemsize and n:
+    for p, end in ((qp, qp + ((n - 1) * ql + cols) * es), (kp, kp + ((n - 1) * kl + cols) * es),
+                   (vp, vp + ((n - 1) * vl + cols) * es), (lg, lg + 4 * H)):
+        if n and p < behind and first < end:
             raise L.GrkError('q, k, v and log_decay must not overlap state, which is written')
     if out is None:
         out = torch.empty((n, cols), dtype=dt, device=q.device)

@@ -164,3 +164,18 @@ def test_slots_that_are_said_to_differ(K, n):
         assert torch.equal(o, want) and torch.equal(a, b) and flags.tolist() == [[1], [1]]
     own = K.decay_attn_step(q, k, v, lg, a.copy_(state), distinct=True)
     assert torch.equal(own, K.decay_attn_step(q, k, v, lg, b.copy_(state))) and torch.equal(a, b)
+
+
+def test_decays_right_before_or_behind_the_states(K):
+    """Neighbours in memory are no overlap, however narrow the gap."""
+    H, hd = 2, 16
+    buf = torch.zeros(2 + 3 * H * hd * hd + 2, device=DEV)
+    state = buf[2:-2].view(3, H, hd, hd)
+    x = torch.ones(3, H * hd, device=DEV)
+    for lg in (buf[:2], buf[-2:]):
+        lg.fill_(-0.1)
+        K.decay_attn_step(x, x, x, lg, state)
+    rows = torch.zeros(2 * 3 * H * hd + 3 * H * hd * hd, device=DEV)
+    a, b = rows[:3 * H * hd].view(3, -1), rows[-3 * H * hd:].view(3, -1)
+    K.decay_attn_step(a, b, x, lg, rows[3 * H * hd:-3 * H * hd].view(3, H, hd, hd))
+    torch.cuda.synchronize()
