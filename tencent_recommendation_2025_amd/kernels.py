@@ -1502,12 +1502,11 @@ def decay_attn_step(q, k, v, log_decay, state, slots=None, scale=None, err_flag=
     dt = q.dtype
     code = _row_code(dt)
     (qp, ql), (kp, kl), (vp, vl) = [_head_rows(t, m, n, cols, dt) for t, m in ((q, 'q'), (k, 'k'), (v, 'v'))]
-    first, lg, es = state.data_ptr(), log_decay.data_ptr(), dt.itemsize
-    behind = first + 4 * state.numel()
-    for p, end in ((qp, qp + ((n - 1) * ql + cols) * es), (kp, kp + ((n - 1) * kl + cols) * es),
-                   (vp, vp + ((n - 1) * vl + cols) * es), (lg, lg + 4 * H)):
-        if n and p < behind and first < end:
-            raise L.GrkError('q, k, v and log_decay must not overlap state, which is written')
+    sp, lp, es = state.data_ptr(), log_decay.data_ptr(), dt.itemsize
+    behind = sp + 4 * state.numel()
+    if n and (qp < behind and sp < qp + ((n - 1) * ql + cols) * es or kp < behind and sp < kp + ((n - 1) * kl + cols) * es
+              or vp < behind and sp < vp + ((n - 1) * vl + cols) * es or lp < behind and sp < lp + 4 * H):
+        raise L.GrkError('q, k, v and log_decay must not overlap state, which is written')
     if out is None:
         out = torch.empty((n, cols), dtype=dt, device=q.device)
     else:
@@ -1519,7 +1518,7 @@ def decay_attn_step(q, k, v, log_decay, state, slots=None, scale=None, err_flag=
     nb = lib.grk_decay_attn_step_workspace(n, slots is not None and not distinct)
     ws = torch.empty(nb, dtype=torch.uint8, device=q.device) if nb else None
     _launch(lib.grk_decay_attn_step, 'grk_decay_attn_step', dev, qp, ql, kp, kl, vp, vl, code,
-            log_decay.data_ptr(), n, H, hd, hd ** -0.5 if scale is None else scale, state.data_ptr(),
+            lp, n, H, hd, hd ** -0.5 if scale is None else scale, sp,
             state.shape[0], _ptr(slots), (L.itype_code(slots.dtype) if slots is not None else L.GRK_I64)
             + (L.GRK_SLOTS_DIFFER if distinct else 0),
             _ptr(err_flag), op, ol, _ptr(ws), nb)
